@@ -1,0 +1,1086 @@
+// Keys and values held in 4 bits, and the attention over their pages; compiled for one head size (CO_HEAD_DIM, a
+// multiple of 32 up to 256).
+//
+// A row's channels are taken in groups of 32.  A group of values x has, in bfloat16,
+//   minimum m = min(x),   scale s = (max(x) - min(x)) / 15   (float32 arithmetic, then rounded),
+// and per channel a code c = clamp(rint((x - m) / s), 0, 15); it stands for s c + m, at most s / 2 (and the rounding of
+// s and m) from x.  A group that is constant has s = 0.  A group that holds a value that is not finite has s and m not
+// a number.  5 bits a value with the pairs: 3.2 times as many positions as bfloat16 in the same memory.
+//
+// A page keeps, per kv head, page_size / 16 tiles of 16 positions; a tile is TB = 10 HD bytes, codes first, pairs behind.
+// Both tiles lie as the fragments of mma.sync.m16n8k16 want them, so that a lane's codes and pairs come by loads of 8
+// and 16 bytes that no two lanes contend for and no code has to change its lane (lane = 4 g + t):
+//  * keys: rows of HD / 2 bytes; word t NG + u of a row (NG = HD / 32) holds channels 32 u + 8 t + 0..7, lowest bits
+//    first; then 16 rows of NG pairs (s low half, m high half).
+//  * values: for group u, lane (g, t), p = 0, 1 a word: low half row 4 t + 2 p, high half row 4 t + 2 p + 1, each
+//    channels 32 u + 4 g + 0..3; then for (u, t) the scales of rows 4 t..4 t + 3 and their minima.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+#ifndef CO_HEAD_DIM
+#define CO_HEAD_DIM 128
+#endif
+
+namespace {
+typedef __nv_bfloat16 bf16;
+constexpr int HD = CO_HEAD_DIM;
+constexpr int NG = HD / 32;           // groups of a row
+constexpr int TB = 10 * HD;           // bytes of a tile
+constexpr int CODES = 8 * HD;         // of which codes
+static_assert(HD % 32 == 0 && HD >= 32 && HD <= 256, "head size must be a multiple of 32 in 32..256");
+
+constexpr int BAD_INDEX = 41;         // status: a slot, a position or a block-table entry lies outside its table
+
+__device__ __forceinline__ float lo_bf16(unsigned w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_bf16(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
+__device__ __forceinline__ __nv_bfloat162 pair_of(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+__device__ __forceinline__ unsigned pack(float a, float b) { return bits(__floats2bfloat162_rn(a, b)); }
+
+// The start of the tile that holds row `row` of a page.
+__device__ __forceinline__ size_t tile_at(long long page, int nkv, int kvh, int page_size, int row) {
+  return (((size_t)page * nkv + kvh) * (page_size >> 4) + (row >> 4)) * TB;
+}
+
+// ------------------------------------------------------------------------------------
+// Rotation and write.  A thread has 8 neighbouring channels of one head of one token; the four threads of a group agree
+// on its minimum and maximum by two shuffles.  Queries are rotated into their own rows; keys are rotated and rounded to
+// the compute type, as a cache in that type would hold them, and then quantised, values quantised as they are.  Every
+// product and sum of the rotation is rounded by itself (no fused multiply-add): the codes are then the same
+// function of the inputs wherever it is computed.
+//
+// Bound by the bytes of a prompt (2,048 tokens of 28 + 8 heads of 128: 19 MB read, 15 MB written) and by one launch at
+// decoding.
+// ------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<bf16>(const bf16* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { x[2 * i] = lo_bf16(w[i]); x[2 * i + 1] = hi_bf16(w[i]); }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void store8<bf16>(bf16* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
+                 const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
+                 T* __restrict__ q_out, int tokens, int nh, int nkv, int rot, int page_size, int first_head, int* __restrict__ status) {
+  constexpr int TPH = HD / 8;                     // threads of a head
+  co_pdl_launch_dependents();
+  const int heads = nh + 2 * nkv - first_head;    // without a rotation there is nothing to do for the queries
+  const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long row_head = id / TPH;
+  const int piece = (int)(id % TPH);
+  const bool live = row_head < (long long)tokens * heads;
+  const int token = live ? (int)(row_head / heads) : 0;
+  const int head = first_head + (live ? (int)(row_head % heads) : 0);
+  const int c0 = piece * 8;
+  co_pdl_wait();
+  const T* src = qkv + (size_t)token * ld + (size_t)head * HD;
+  float x[8];
+  load8(src + c0, x);
+  if (rot && head < nh + nkv) {
+    const int half = rot >> 1;
+    const int pos = positions[token];
+    if (pos < 0 || pos >= n_cos) {
+      if (live && status) *status = BAD_INDEX;
+    } else {
+      const float2* cs = cos_sin + (size_t)pos * half;
+      if ((half & 7) == 0) {
+        if (c0 < rot) {
+          const bool upper = c0 >= half;
+          float y[8];
+          load8(src + (upper ? c0 - half : c0 + half), y);
+          const float4* turn = reinterpret_cast<const float4*>(cs + (upper ? c0 - half : c0));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 t = turn[i];
+            const float a = __fmul_rn(y[2 * i], t.y), b = __fmul_rn(y[2 * i + 1], t.w);
+            const float d = __fmul_rn(x[2 * i], t.x), e = __fmul_rn(x[2 * i + 1], t.z);
+            x[2 * i] = upper ? __fadd_rn(d, a) : __fsub_rn(d, a);
+            x[2 * i + 1] = upper ? __fadd_rn(e, b) : __fsub_rn(e, b);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = c0 + i;
+          if (c >= rot) continue;
+          const bool upper = c >= half;
+          const float2 t = cs[upper ? c - half : c];
+          const float y = __fmul_rn(co_to_float<T>(src[upper ? c - half : c + half]), t.y), d = __fmul_rn(x[i], t.x);
+          x[i] = upper ? __fadd_rn(d, y) : __fsub_rn(d, y);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = co_to_float<T>(co_from_float<T>(x[i]));
+    }
+  }
+  if (head < nh) {
+    if (live) store8(q_out + (size_t)token * nh * HD + (size_t)head * HD + c0, x);
+  }
+  // The group's range: all four threads take part, whatever their head is.
+  float lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    finite = finite && fabsf(x[i]) < INFINITY;
+  }
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
+  }
+  if (!live || head < nh) return;
+  const int slot = slots[token];
+  if (slot < 0) return;                           // a row that is not kept
+  const int page = slot / page_size, row = slot - page * page_size;
+  if (page >= num_pages) {
+    if (status) *status = BAD_INDEX;
+    return;
+  }
+  bf16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), m16 = __float2bfloat16_rn(lo);
+  float s = __bfloat162float(s16), m = __bfloat162float(m16);
+  if (!(finite && fabsf(s) < INFINITY && fabsf(m) < INFINITY)) {
+    s16 = m16 = __ushort_as_bfloat16(0x7fff);
+    s = 0.f;
+  }
+  unsigned word = 0;
+  if (s > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], m), s)), 0.f), 15.f);
+      word |= (unsigned)c << (4 * i);
+    }
+  }
+  const int u = piece >> 2, t = piece & 3, r = row & 15;
+  if (head < nh + nkv) {
+    unsigned char* tile = k_cache + tile_at(page, nkv, head - nh, page_size, row);
+    reinterpret_cast<unsigned*>(tile)[r * (4 * NG) + t * NG + u] = word;
+    if (t == 0)
+      reinterpret_cast<unsigned*>(tile + CODES)[r * NG + u] = (unsigned)__bfloat16_as_ushort(s16) | (unsigned)__bfloat16_as_ushort(m16) << 16;
+  } else {
+    unsigned char* tile = v_cache + tile_at(page, nkv, head - nh - nkv, page_size, row);
+    unsigned short* half = reinterpret_cast<unsigned short*>(tile) + ((((u * 8 + 2 * t) * 4 + (r >> 2)) * 2 + ((r >> 1) & 1)) * 2 + (r & 1));
+    half[0] = (unsigned short)word;
+    half[16] = (unsigned short)(word >> 16);      // the next g: four lanes of two words
+    if (t == 0) {
+      bf16* pairs = reinterpret_cast<bf16*>(tile + CODES) + (u * 4 + (r >> 2)) * 8 + (r & 3);
+      pairs[0] = s16;
+      pairs[4] = m16;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// Pages as values: [entry, kv head, page_size, HD] in float32 or bfloat16.  One block per (page, kv head).
+// With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length are
+// zeros, entries that lie wholly behind it or in front of the window of its first new token are left out, and
+// `out_table` gets the entry's place among the output pages, or -1.
+// Bound by the bytes written (16 of 21 bits a value).
+// ------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+template <>
+__device__ __forceinline__ void store4<bf16>(bf16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack(a, b), pack(c, d));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128)
+kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
+                 const int* __restrict__ table, int table_ld, int width, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
+                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, int* __restrict__ status) {
+  co_pdl_launch_dependents();
+  co_pdl_wait();
+  const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const long long entry = (long long)b * width + j;
+  int valid = page_size;                           // rows of the page that hold something
+  if (lens) {
+    const int len = lens[b], first_new = len - (cu_q[b + 1] - cu_q[b]);
+    const int first_key = window > 0 ? max(0, first_new - window + 1) : 0;
+    valid = min(page_size, len - j * page_size);
+    if (valid <= 0 || (j + 1) * page_size <= first_key) {
+      if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
+      return;
+    }
+  }
+  const int page = table[(size_t)b * table_ld + j];
+  const bool known = page >= 0 && page < num_pages;
+  if (!known) valid = 0;
+  if (kvh == 0 && threadIdx.x == 0) {
+    if (out_table) out_table[entry] = known ? (int)entry : -1;
+    if (!known && status) *status = BAD_INDEX;
+  }
+  T* ko = k_out + ((size_t)entry * nkv + kvh) * page_size * HD;
+  T* vo = v_out + ((size_t)entry * nkv + kvh) * page_size * HD;
+  for (int tile = 0; tile < page_size >> 4; ++tile) {
+    const unsigned char* kt = k_cache + tile_at(known ? page : 0, nkv, kvh, page_size, tile * 16);
+    const unsigned char* vt = v_cache + tile_at(known ? page : 0, nkv, kvh, page_size, tile * 16);
+    for (int i = threadIdx.x; i < 16 * 4 * NG; i += 128) {
+      const int r = i / (4 * NG), w = i % (4 * NG), u = w >> 2, t = w & 3;    // u, t: consecutive threads, consecutive channels
+      float x[8];
+      const bool keep = tile * 16 + r < valid;
+      const unsigned word = reinterpret_cast<const unsigned*>(kt)[r * (4 * NG) + t * NG + u];
+      const unsigned sm = reinterpret_cast<const unsigned*>(kt + CODES)[r * NG + u];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] = keep ? fmaf(lo_bf16(sm), (float)((word >> (4 * c)) & 15), hi_bf16(sm)) : 0.f;
+      store8(ko + (size_t)(tile * 16 + r) * HD + u * 32 + t * 8, x);
+    }
+    for (int i = threadIdx.x; i < 32 * NG; i += 128) {
+      const int t = i / (8 * NG), w = i % (8 * NG), u = w >> 3, g = w & 7;
+      const uint2 words = reinterpret_cast<const uint2*>(vt)[u * 32 + g * 4 + t];
+      const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
+      const float sc[4] = {lo_bf16(sm.x), hi_bf16(sm.x), lo_bf16(sm.y), hi_bf16(sm.y)};
+      const float mn[4] = {lo_bf16(sm.z), hi_bf16(sm.z), lo_bf16(sm.w), hi_bf16(sm.w)};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = tile * 16 + 4 * t + e;
+        const unsigned h = (e < 2 ? words.x : words.y) >> (16 * (e & 1));
+        float x[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = r < valid ? fmaf(sc[e], (float)((h >> (4 * c)) & 15), mn[e]) : 0.f;
+        store4(vo + (size_t)r * HD + u * 32 + g * 4, x[0], x[1], x[2], x[3]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// How the keys of a step are cut.  The visible positions of a request (from the 16 that hold the first one on) are
+// counted in units of UNIT positions; a work item is a run of units of one (request, kv head, tile of query rows).  All
+// items have about the same number of units, total / target of them, so that a long context beside short ones is cut
+// into as many items as it needs, from the lengths on the device: a captured launch serves every length.  The items of a
+// (request, kv head, row tile) are neighbours, and an item's number is its place in the scratch.
+// ------------------------------------------------------------------------------------
+constexpr int UNIT = 64;
+
+struct Cut {                       // of one request
+  int tok0, q_len, kv_len;
+  int lo16, units;                 // first tile of 16 positions, units from there on
+  int row_tiles;
+};
+__device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b, int G, int rows_per_tile, int max_rows, int window) {
+  Cut c;
+  c.tok0 = cu_q[b];
+  c.q_len = cu_q[b + 1] - c.tok0;
+  c.kv_len = kv_lens[b];
+  const int rows = c.q_len * G;
+  const int first = window > 0 ? max(0, c.kv_len - c.q_len - window + 1) : 0;
+  c.lo16 = first >> 4;
+  c.units = max(0, (c.kv_len - c.lo16 * 16 + UNIT - 1) / UNIT);
+  c.row_tiles = rows > 0 && rows <= max_rows ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
+  if (c.row_tiles == 0) c.units = 0;
+  return c;
+}
+struct Item {
+  int b, kvh, row_tile, part, parts, first;   // first: the number of part 0's item
+  Cut cut;
+};
+// Units per item when about `target` items are wanted, and the item of number `index` (b = -1: there is none).
+// One warp; all lanes get the answer.
+__device__ __forceinline__ Item find_item(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows,
+                                          int window, int target, int index) {
+  const int lane = threadIdx.x & 31;
+  long long total = 0;
+  for (int b = lane; b < B; b += 32) {
+    const Cut c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
+    total += (long long)c.units * c.row_tiles * nkv;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const int per = (int)max(1LL, (total + target - 1) / target);
+  Item it;
+  it.b = -1;
+  int before = 0;
+  for (int b0 = 0; b0 < B && it.b < 0; b0 += 32) {
+    const int b = b0 + lane;
+    Cut c = {0, 0, 0, 0, 0, 0};
+    if (b < B) c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
+    // A request with rows and no key has one item, which writes zeros.
+    const int parts = c.row_tiles ? max(1, (c.units + per - 1) / per) : 0;
+    const int mine = parts * c.row_tiles * nkv;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const int start = before + sum - mine;
+    const unsigned hit = __ballot_sync(0xffffffffu, index >= start && index < start + mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int s = __shfl_sync(0xffffffffu, start, src);
+      it.b = b0 + src;
+      it.parts = __shfl_sync(0xffffffffu, parts, src);
+      it.cut.tok0 = __shfl_sync(0xffffffffu, c.tok0, src);
+      it.cut.q_len = __shfl_sync(0xffffffffu, c.q_len, src);
+      it.cut.kv_len = __shfl_sync(0xffffffffu, c.kv_len, src);
+      it.cut.lo16 = __shfl_sync(0xffffffffu, c.lo16, src);
+      it.cut.units = __shfl_sync(0xffffffffu, c.units, src);
+      it.cut.row_tiles = __shfl_sync(0xffffffffu, c.row_tiles, src);
+      const int in = index - s;
+      it.part = in % it.parts;
+      it.row_tile = in / it.parts % it.cut.row_tiles;
+      it.kvh = in / (it.parts * it.cut.row_tiles);
+      it.first = index - it.part;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return it;
+}
+
+// The merge of partial results (maximum, sum, accumulator) in ascending order; a maximum of -inf carries nothing.
+__device__ __forceinline__ float factor(float m, float M) { return m == -INFINITY ? 0.f : exp2f(m - M); }
+
+// ------------------------------------------------------------------------------------
+// Attention in float32 arithmetic: any compute type, any alignment, any rows.  A CTA per (token, kv head) walks the
+// visible tiles with its warps side by side; a lane has two halves of one key row for the scores and four channels of
+// a group for the sums.  HC heads of the group at a time share a tile's codes.
+// ------------------------------------------------------------------------------------
+constexpr int HC = 4;
+constexpr int SW = 8;                        // warps
+constexpr int VU = (HD / 4 + 31) / 32;       // units of four channels per lane
+
+template <typename T>
+__global__ void __launch_bounds__(32 * SW)
+kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
+                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ table, int table_ld,
+                  const int* __restrict__ token_req, const int* __restrict__ positions, int nh, int nkv, int page_size, int window,
+                  float scale_log2, int* __restrict__ status) {
+  __shared__ float qs[HC][HD];
+  __shared__ float sp[SW][HC][16];
+  __shared__ float merge[SW][HC][HD + 2];
+  co_pdl_launch_dependents();
+  co_pdl_wait();
+  const int token = blockIdx.x, kvh = blockIdx.y, G = nh / nkv;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pos = positions[token];
+  const int* pages = table + (size_t)token_req[token] * table_ld;
+  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+  for (int h0 = 0; h0 < G; h0 += HC) {
+    const int n = min(HC, G - h0);
+    __syncthreads();
+    for (int i = tid; i < HC * HD; i += 32 * SW) {
+      const int h = i / HD;
+      qs[h][i % HD] = h < n ? co_to_float<T>(q[(size_t)token * q_ld + (size_t)(kvh * G + h0 + h) * HD + i % HD]) : 0.f;
+    }
+    __syncthreads();
+    float m[HC], l[HC], acc[HC][VU][4];
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int v = 0; v < VU; ++v)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[h][v][c] = 0.f;
+    }
+    for (int tile = (lo >> 4) + warp; tile * 16 <= pos; tile += SW) {
+      const int blk = tile * 16 / page_size;
+      const int page = blk < table_ld ? pages[blk] : -1;
+      if (page < 0 || page >= num_pages) {
+        if (lane == 0 && status) *status = BAD_INDEX;
+        continue;
+      }
+      const unsigned char* kt = k_cache + tile_at(page, nkv, kvh, page_size, tile * 16 - blk * page_size);
+      const unsigned char* vt = v_cache + tile_at(page, nkv, kvh, page_size, tile * 16 - blk * page_size);
+      // Scores: lane = (row, half); words t = 2 half, 2 half + 1 of every group.
+      const int r = lane >> 1, half = lane & 1;
+      float s[HC];
+#pragma unroll
+      for (int h = 0; h < HC; ++h) s[h] = 0.f;
+      for (int u = 0; u < NG; ++u) {
+        const unsigned sm = reinterpret_cast<const unsigned*>(kt + CODES)[r * NG + u];
+        const float sc = lo_bf16(sm), mn = hi_bf16(sm);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int t = 2 * half + w;
+          const unsigned word = reinterpret_cast<const unsigned*>(kt)[r * (4 * NG) + t * NG + u];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float x = fmaf(sc, (float)((word >> (4 * c)) & 15), mn);
+#pragma unroll
+            for (int h = 0; h < HC; ++h) s[h] = fmaf(qs[h][u * 32 + t * 8 + c], x, s[h]);
+          }
+        }
+      }
+      const int p = tile * 16 + r;
+      const bool seen = p >= lo && p <= pos;
+#pragma unroll
+      for (int h = 0; h < HC; ++h) {
+        s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
+        s[h] = seen ? s[h] * scale_log2 : -INFINITY;
+        const float M = fmaxf(m[h], co_warp_max(s[h]));
+        const float f = factor(m[h], M);
+        const float e = s[h] == -INFINITY ? 0.f : exp2f(s[h] - M);
+        m[h] = M;
+        l[h] = l[h] * f + (half == 0 ? e : 0.f);
+        if (half == 0) sp[warp][h][r] = e;
+#pragma unroll
+        for (int v = 0; v < VU; ++v)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[h][v][c] *= f;
+      }
+      __syncwarp();
+      // Sums: a lane has four channels of VU groups.
+#pragma unroll
+      for (int v = 0; v < VU; ++v) {
+        const int unit = v * 32 + lane, u = unit >> 3, g = unit & 7;
+        if (unit >= HD / 4) break;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint2 words = reinterpret_cast<const uint2*>(vt)[u * 32 + g * 4 + t];
+          const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
+          const float sc[4] = {lo_bf16(sm.x), hi_bf16(sm.x), lo_bf16(sm.y), hi_bf16(sm.y)};
+          const float mn[4] = {lo_bf16(sm.z), hi_bf16(sm.z), lo_bf16(sm.w), hi_bf16(sm.w)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = 4 * t + e;
+            if (tile * 16 + row < lo || tile * 16 + row > pos) continue;
+            const unsigned hw = (e < 2 ? words.x : words.y) >> (16 * (e & 1));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float x = fmaf(sc[e], (float)((hw >> (4 * c)) & 15), mn[e]);
+#pragma unroll
+              for (int h = 0; h < HC; ++h) acc[h][v][c] = fmaf(sp[warp][h][row], x, acc[h][v][c]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      const float sum = co_warp_sum(l[h]);
+      if (lane == 0) { merge[warp][h][HD] = m[h]; merge[warp][h][HD + 1] = sum; }
+#pragma unroll
+      for (int v = 0; v < VU; ++v) {
+        const int unit = v * 32 + lane;
+        if (unit < HD / 4)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) merge[warp][h][unit * 4 + c] = acc[h][v][c];
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < n * HD; i += 32 * SW) {
+      const int h = i / HD, c = i % HD;
+      float M = -INFINITY, den = 0.f, num = 0.f;
+#pragma unroll
+      for (int w = 0; w < SW; ++w) M = fmaxf(M, merge[w][h][HD]);
+#pragma unroll
+      for (int w = 0; w < SW; ++w) {
+        const float f = factor(merge[w][h][HD], M);
+        den += f * merge[w][h][HD + 1];
+        num += f * merge[w][h][c];
+      }
+      out[(size_t)token * out_ld + (size_t)(kvh * G + h0 + h) * HD + c] = co_from_float<T>(den == 0.f ? 0.f : num / den);
+    }
+  }
+}
+// ------------------------------------------------------------------------------------
+// Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
+// each with tiles of 16 positions of its own (tile i of the item goes to warp i mod 4) in a ring of its own that
+// cp.async fills, so that warps never wait for one another before the end.  Decoding is bound by the cache's bytes, and
+// with 5 bits a value nearly as much by the instructions that turn codes into operands; hence:
+//  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
+//    of up to 8 heads wastes no product;
+//  * keys: code c enters the product as the bfloat16 128 + c (one lop3 for two codes); the accumulator starts at
+//    -128 sum(q), so that it ends as sum(q c), and the group's s and m multiply float32 sums: score += s D + m sum(q).
+//    No key is rounded;
+//  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs);
+//  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
+//  * the running maximum moves (and the accumulators are scaled) only when a tile holds a larger score than the warp has
+//    seen in any row of it.
+// The rows' sums stay per lane and meet once at the end, as do the warps.
+// ------------------------------------------------------------------------------------
+constexpr int WARPS = 4;
+constexpr int STAGES = 4;
+constexpr int PIECES = 2 * TB / 16;      // 16-byte pieces of a key and a value tile
+
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // src-size 0 fills the 16 bytes with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned transposed(unsigned v) {
+  unsigned r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));   // ex2(-inf) = +0
+  return y;
+}
+// Codes j and j + 4 of a word as the bfloat16 pair 128 + c.
+__device__ __forceinline__ unsigned codes128(unsigned word, int j) { return ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
+template <int N>
+__device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+      w[2 * i] = v.x; w[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = p[i];
+  }
+}
+template <int NT>
+constexpr size_t items_smem() {
+  const size_t ring = (size_t)WARPS * STAGES * 2 * TB, merge = (size_t)WARPS * 8 * NT * (HD + 4) * sizeof(float);
+  return ring > merge ? ring : merge;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(32 * WARPS)
+kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
+                 const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
+                 const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
+                 float scale_log2, int max_rows, int target, float* __restrict__ scratch, int items, int* __restrict__ status) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int COLS = 8 * NT;
+  co_pdl_wait();
+  co_pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int G = nh / nkv;
+  const Item it = find_item(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, target, blockIdx.x);
+  if (it.b < 0) return;
+  const Cut c = it.cut;
+  const int rows = min(COLS, c.q_len * G - it.row_tile * COLS);      // of this tile
+  const int row0 = it.row_tile * COLS;
+  const int* table = block_tables + (size_t)it.b * table_ld;
+  const int u_first = (int)((long long)c.units * it.part / it.parts), u_end = (int)((long long)c.units * (it.part + 1) / it.parts);
+  const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
+  const int tile0 = c.lo16 + u_first * (UNIT / 16) + warp;
+  const int n_tiles = tile_end > tile0 ? (tile_end - tile0 + WARPS - 1) / WARPS : 0;    // of this warp
+  const int base_pos = c.kv_len - c.q_len;
+
+  unsigned char* ring = smem + (size_t)warp * STAGES * 2 * TB;
+  const unsigned ring_addr = smem_addr(ring);
+  // Block-table entries of the warp's tiles, 32 tiles at a time, a lane each.
+  int entry = -1;
+  auto fetch_entries = [&](int i0) {
+    const int tile = tile0 + (i0 + lane) * WARPS;
+    const int blk = tile * 16 / page_size;
+    entry = i0 + lane < n_tiles && blk < table_ld ? table[blk] : -1;
+    if (i0 + lane < n_tiles && (entry < 0 || entry >= num_pages)) {
+      entry = -1;
+      if (status) *status = BAD_INDEX;
+    }
+  };
+  unsigned known = 0;      // bit i % STAGES: the tile in that stage came from a page of the pool
+  auto issue = [&](int i) {
+    if (i < n_tiles) {
+      if ((i & 31) == 0) fetch_entries(i);
+      const int page = __shfl_sync(0xffffffffu, entry, i & 31);
+      const int pos = (tile0 + i * WARPS) * 16;
+      const size_t at = page < 0 ? 0 : tile_at(page, nkv, it.kvh, page_size, pos % page_size);
+      const unsigned dst = ring_addr + (i % STAGES) * 2 * TB;
+#pragma unroll
+      for (int p0 = 0; p0 < PIECES; p0 += 32) {
+        const int p = p0 + lane;
+        if (PIECES % 32 == 0 || p < PIECES)
+          cp_async16(dst + p * 16, p < TB / 16 ? k_cache + at + p * 16 : v_cache + at + p * 16 - TB, page >= 0);
+      }
+      known = (known & ~(1u << (i % STAGES))) | (page >= 0 ? 1u << (i % STAGES) : 0u);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) issue(i);
+
+  // The queries as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
+  unsigned qf[NT][NG][4];
+  float sq[NT][NG][2];        // sum of the group's channels of rows 2 t, 2 t + 1
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g, row = row0 + r;
+    const bf16* src = q + (size_t)(c.tok0 + row / G) * q_ld + (size_t)(it.kvh * G + row % G) * HD;
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows) v = *reinterpret_cast<const uint4*>(src + u * 32 + t * 8);
+      qf[nt][u][0] = __byte_perm(v.x, v.z, 0x5410);       // channels 0, 4
+      qf[nt][u][1] = __byte_perm(v.x, v.z, 0x7632);       // 1, 5
+      qf[nt][u][2] = __byte_perm(v.y, v.w, 0x5410);
+      qf[nt][u][3] = __byte_perm(v.y, v.w, 0x7632);
+      float sum = ((lo_bf16(v.x) + hi_bf16(v.x)) + (lo_bf16(v.y) + hi_bf16(v.y))) + ((lo_bf16(v.z) + hi_bf16(v.z)) + (lo_bf16(v.w) + hi_bf16(v.w)));
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sq[nt][u][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+      sq[nt][u][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+    }
+  }
+  int hi[NT][2], lo[NT][2];   // visible positions of rows 2 t, 2 t + 1 of every eight
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + 2 * t + e;
+      hi[nt][e] = r < rows ? base_pos + (row0 + r) / G : -1;
+      lo[nt][e] = window > 0 ? max(0, hi[nt][e] - window + 1) : 0;
+    }
+  // Positions [all_lo, all_hi] are visible to every row of the tile.
+  const int all_hi = base_pos + row0 / G, last = base_pos + (row0 + rows - 1) / G;
+  const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
+
+  float o[NG][2][NT][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int u = 0; u < NG; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[u][h][nt][i] = 0.f;
+  }
+  const int r0 = 4 * (g >> 1) + (g & 1);        // this lane's rows of a tile in the first product: r0 and r0 + 2
+  const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
+
+#pragma unroll 1
+  for (int i = 0; i < n_tiles; ++i) {
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();                               // landed for all lanes; all are done with the stage of tile i - 1
+    const bool usable = (known >> (i % STAGES)) & 1;
+    issue(i + STAGES - 1);
+    if (!usable) continue;
+    const unsigned char* kt = ring + (i % STAGES) * 2 * TB;
+    const unsigned char* vt = kt + TB;
+    const int key0 = (tile0 + i * WARPS) * 16;
+
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    {
+      unsigned ka[NG], kb[NG], pa[NG], pb[NG];
+      load_words<NG>(reinterpret_cast<const unsigned*>(kt) + r0 * (4 * NG) + t * NG, ka);
+      load_words<NG>(reinterpret_cast<const unsigned*>(kt) + (r0 + 2) * (4 * NG) + t * NG, kb);
+      load_words<NG>(reinterpret_cast<const unsigned*>(kt + CODES) + r0 * NG, pa);
+      load_words<NG>(reinterpret_cast<const unsigned*>(kt + CODES) + (r0 + 2) * NG, pb);
+#pragma unroll
+      for (int u = 0; u < NG; ++u) {
+        unsigned a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { a[j] = codes128(ka[u], j); b[j] = codes128(kb[u], j); }
+        const float sa = lo_bf16(pa[u]), ma = hi_bf16(pa[u]), sb = lo_bf16(pb[u]), mb = hi_bf16(pb[u]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float d[4] = {-128.f * sq[nt][u][0], -128.f * sq[nt][u][1], -128.f * sq[nt][u][0], -128.f * sq[nt][u][1]};
+          mma_bf16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
+          mma_bf16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
+          s[nt][0] = fmaf(sa, d[0], fmaf(ma, sq[nt][u][0], s[nt][0]));
+          s[nt][1] = fmaf(sa, d[1], fmaf(ma, sq[nt][u][1], s[nt][1]));
+          s[nt][2] = fmaf(sb, d[2], fmaf(mb, sq[nt][u][0], s[nt][2]));
+          s[nt][3] = fmaf(sb, d[3], fmaf(mb, sq[nt][u][1], s[nt][3]));
+        }
+      }
+    }
+    const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
+    bool grew = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int e = x & 1, pos = key0 + r0 + (x & 2);
+        s[nt][x] = whole || (pos <= hi[nt][e] && pos >= lo[nt][e]) ? s[nt][x] * scale_log2 : -INFINITY;
+        grew = grew || s[nt][x] > m[nt][e];
+      }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float M = fmaxf(fmaxf(s[nt][e], s[nt][2 + e]), m[nt][e]);
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+          const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - M);
+          m[nt][e] = M;
+          l[nt][e] *= f;
+#pragma unroll
+          for (int u = 0; u < NG; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { o[u][h][nt][e] *= f; o[u][h][nt][2 + e] *= f; }
+        }
+    }
+    unsigned pf[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[nt][x] = s[nt][x] == -INFINITY ? 0.f : ex2(s[nt][x] - m[nt][x & 1]);
+        l[nt][x & 1] += s[nt][x];
+      }
+      pf[nt][0] = transposed(pack(s[nt][0], s[nt][1]));
+      pf[nt][1] = transposed(pack(s[nt][2], s[nt][3]));
+    }
+    // Rows of the tile outside what any query of this tile sees may hold anything (a stale row, a page's end): their
+    // pairs are taken as zero, so that nothing which is not finite meets a probability of zero.
+    unsigned keep01 = 0xffffffffu, keep23 = 0xffffffffu;
+    if (!whole) {
+      const int p = key0 + 4 * t;
+      auto seen = [&](int x) { return x <= last && x >= c.lo16 * 16 && (window <= 0 || x > all_hi - window); };
+      keep01 = (seen(p) ? 0x0000ffffu : 0u) | (seen(p + 1) ? 0xffff0000u : 0u);
+      keep23 = (seen(p + 2) ? 0x0000ffffu : 0u) | (seen(p + 3) ? 0xffff0000u : 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
+      const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
+      const __nv_bfloat162 s01 = pair_of(sm.x & keep01), s23 = pair_of(sm.y & keep23), m01 = pair_of(sm.z & keep01), m23 = pair_of(sm.w & keep23);
+      unsigned a[4], b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
+        b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_bf16(o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
+        mma_bf16(o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();               // the rings become the merge area: [warp][row][HD channels, maximum, sum]
+  constexpr int MLD = HD + 4;
+  float* merge = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = l[nt][e];
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      float* dst = merge + (size_t)(warp * COLS + nt * 8 + 2 * t + e) * MLD;
+      if (g == 0) { dst[HD] = m[nt][e]; dst[HD + 1] = sum; }
+#pragma unroll
+      for (int u = 0; u < NG; ++u)
+        *reinterpret_cast<float4*>(dst + u * 32 + g * 4) = make_float4(o[u][0][nt][e], o[u][0][nt][2 + e], o[u][1][nt][e], o[u][1][nt][2 + e]);
+    }
+  __syncthreads();
+  float* acc_out = scratch + (size_t)blockIdx.x * COLS * HD;
+  float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)items * COLS * HD) + (size_t)blockIdx.x * COLS;
+  for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
+    const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
+    float M = -INFINITY, den = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, merge[(size_t)(w * COLS + r) * MLD + HD]);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float* src = merge + (size_t)(w * COLS + r) * MLD;
+      const float f = factor(src[HD], M);
+      const float4 v = *reinterpret_cast<const float4*>(src + ch);
+      den += f * src[HD + 1];
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+    }
+    if (it.parts == 1) {
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      const int row = row0 + r;
+      bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(it.kvh * G + row % G) * HD + ch;
+      store4<bf16>(dst, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+      *reinterpret_cast<float4*>(acc_out + (size_t)r * HD + ch) = acc;
+      if (ch == 0) ml_out[r] = make_float2(M, den);
+    }
+  }
+}
+
+// Joins the items of a row: one CTA per (row of a request's kv head, kv head, request), its warps side by side over the
+// parts, four channels per lane, and the warps' sums in order at the end.
+constexpr int CW = 4;
+__global__ void __launch_bounds__(32 * CW)
+kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q,
+                const int* __restrict__ kv_lens, int B, int nh, int nkv, int cols, int window, int max_rows, int target) {
+  constexpr int V = (HD + 127) / 128;
+  __shared__ float part[CW][HD];
+  __shared__ float2 part_ml[CW];
+  __shared__ int found[2];
+  co_pdl_launch_dependents();
+  const int r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = nh / nkv;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Safe ahead of the wait: the items' kernel starts this one only after its own wait for whatever made the lengths.
+  const Cut c = cut_of(cu_q, kv_lens, b, G, cols, max_rows, window);
+  if (c.row_tiles == 0 || r >= c.q_len * G) return;
+  if (warp == 0) {
+    long long total = 0;
+    for (int x = lane; x < B; x += 32) {
+      const Cut d = cut_of(cu_q, kv_lens, x, G, cols, max_rows, window);
+      total += (long long)d.units * d.row_tiles * nkv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int per = (int)max(1LL, (total + target - 1) / target);
+    int before = 0;
+    for (int x = lane; x < b; x += 32) {
+      const Cut d = cut_of(cu_q, kv_lens, x, G, cols, max_rows, window);
+      before += d.row_tiles ? max(1, (d.units + per - 1) / per) * d.row_tiles * nkv : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const int parts = max(1, (c.units + per - 1) / per);
+    if (lane == 0) {
+      found[0] = parts;
+      found[1] = before + (kvh * c.row_tiles + r / cols) * parts;
+    }
+  }
+  __syncthreads();
+  const int parts = found[0], first = found[1], col = r % cols;
+  if (parts == 1) return;
+  co_pdl_wait();
+  const float2* ml = reinterpret_cast<const float2*>(scratch + (size_t)items * cols * HD) + (size_t)first * cols + col;
+  const float* acc_in = scratch + ((size_t)first * cols + col) * HD;
+  float M = -INFINITY;
+  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[(size_t)p * cols].x);
+  M = co_warp_max(M);
+  float den = 0.f;
+  float4 acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = warp * 8; p0 < parts; p0 += CW * 8) {
+    float f = 0.f;
+    if (lane < 8 && p0 + lane < parts) {
+      const float2 x = ml[(size_t)(p0 + lane) * cols];
+      f = factor(x.x, M);
+      den += f * x.y;
+    }
+    float4 in[8][V];
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int ch = v * 128 + lane * 4;
+        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(acc_in + (size_t)(p0 + p) * cols * HD + ch)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float fp = __shfl_sync(0xffffffffu, f, p);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        acc[v].x += fp * in[p][v].x; acc[v].y += fp * in[p][v].y; acc[v].z += fp * in[p][v].z; acc[v].w += fp * in[p][v].w;
+      }
+    }
+  }
+  den = co_warp_sum(den);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int ch = v * 128 + lane * 4;
+    if (ch < HD) *reinterpret_cast<float4*>(&part[warp][ch]) = acc[v];
+  }
+  if (lane == 0) part_ml[warp] = make_float2(M, den);
+  __syncthreads();
+  const int ch = threadIdx.x * 4;
+  if (ch < HD) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float d = 0.f;
+#pragma unroll
+    for (int w = 0; w < CW; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(&part[w][ch]);
+      sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      d += part_ml[w].y;
+    }
+    const float inv = d == 0.f ? 0.f : 1.f / d;
+    store4<bf16>(out + (size_t)(c.tok0 + r / G) * out_ld + (size_t)(kvh * G + r % G) * HD + ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  }
+}
+
+// Resident CTAs that an item count aims at.
+int items_target() { return 148 * 4; }
+int tiles_of(int max_rows) { return max_rows <= 8 || HD > 128 ? 1 : 2; }
+long long items_bound(int B, int nkv, int max_rows, int max_kv_len) {
+  const long long row_tiles = (max_rows + 8 * tiles_of(max_rows) - 1) / (8 * tiles_of(max_rows));
+  const long long most = (long long)B * nkv * row_tiles, units = ((long long)max_kv_len + 15) / UNIT + 1;
+  const long long by_length = most * units, by_target = items_target() + most;
+  return by_length < by_target ? by_length : by_target;
+}
+
+template <int NT>
+int launch_items(const void* q, long q_ld, void* out, long out_ld, const void* k_cache, const void* v_cache, int num_pages, const int* table,
+                 int table_ld, const int* cu_q, const int* kv_lens, int B, int nh, int nkv, int page_size, int window, float scale_log2,
+                 int max_rows, int items, float* scratch, int* status, cudaStream_t stream) {
+  constexpr size_t SMEM = items_smem<NT>();
+  if (SMEM > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kv4_items_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    if (e != cudaSuccess) CO_FAIL("kv4_attention: %zu bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+  }
+  co_launch(kv4_items_kernel<NT>, dim3((unsigned)items), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
+            (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
+            window, scale_log2, max_rows, items_target(), scratch, items, status);
+  CO_CHECK_LAUNCH("kv4_items");
+  return 0;
+}
+}  // namespace
+
+CO_EXPORT int coheryn_kv4_head_dim() { return HD; }
+
+static int check_pages(const char* what, int nkv, int page_size, int num_pages) {
+  if (nkv < 1 || page_size < 16 || page_size % 16) CO_FAIL("%s: %d kv heads, pages of %d positions (a multiple of 16)", what, nkv, page_size);
+  if (num_pages < 1 || (long long)num_pages * page_size > 0x7fffffffLL)
+    CO_FAIL("%s: %d pages of %d positions do not fit 32-bit slots", what, num_pages, page_size);
+  return 0;
+}
+
+CO_EXPORT int coheryn_kv4_write(const void* qkv, long ld, int dtype, const int* positions, const float* cos_sin, int n_cos, const int* slots,
+                                void* k_cache, void* v_cache, int num_pages, void* q_out, int T, int nh, int nkv, int rot, int page_size,
+                                int* status, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (check_pages("kv4_write", nkv, page_size, num_pages)) return 1;
+  if (rot < 0 || rot > HD || (rot & 1)) CO_FAIL("kv4_write: %d rotated channels of %d", rot, HD);
+  if (nh < 0) CO_FAIL("kv4_write: %d heads", nh);
+  const int align = dtype == CO_F32 ? 4 : 8;
+  if (((uintptr_t)qkv & 15) || ld % align || ((uintptr_t)q_out & 15) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) ||
+      ((uintptr_t)cos_sin & 15))
+    CO_FAIL("kv4_write: operands must be 16-byte aligned");
+  const int first = rot ? 0 : nh;
+  const long long blocks = ((long long)T * (nh + 2 * nkv - first) * (HD / 8) + 255) / 256;
+  if (blocks > 0x7fffffffLL) CO_FAIL("kv4_write: %d tokens of %d heads", T, nh + 2 * nkv);
+  if (dtype == CO_F32)
+    co_launch(kv4_write_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, (const float*)qkv, ld, positions, (const float2*)cos_sin,
+              n_cos, slots, (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (float*)q_out, T, nh, nkv, rot, page_size, first, status);
+  else
+    co_launch(kv4_write_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, stream, (const bf16*)qkv, ld, positions, (const float2*)cos_sin,
+              n_cos, slots, (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (bf16*)q_out, T, nh, nkv, rot, page_size, first, status);
+  CO_CHECK_LAUNCH("kv4_write");
+  return 0;
+}
+
+static int launch_pages(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
+                        int width, int n, const int* cu_q, const int* lens, int window, void* k_out, void* v_out, int dtype, int* out_table,
+                        int* status, cudaStream_t stream) {
+  if (nkv > 65535 || n > 65535) CO_FAIL("kv4_pages: %d requests, %d kv heads", n, nkv);
+  const dim3 grid((unsigned)width, (unsigned)nkv, (unsigned)n);
+  if (dtype == CO_F32)
+    co_launch(kv4_pages_kernel<float>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
+              page_size, table, table_ld, width, cu_q, lens, window, (float*)k_out, (float*)v_out, out_table, status);
+  else
+    co_launch(kv4_pages_kernel<bf16>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
+              page_size, table, table_ld, width, cu_q, lens, window, (bf16*)k_out, (bf16*)v_out, out_table, status);
+  CO_CHECK_LAUNCH("kv4_pages");
+  return 0;
+}
+
+// pages [n] -> k_out, v_out [n, nkv, page_size, HD].
+CO_EXPORT int coheryn_kv4_pages(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* pages, int n,
+                                void* k_out, void* v_out, int dtype, int* status, cudaStream_t stream) {
+  if (n <= 0) return 0;
+  if (check_pages("kv4_pages", nkv, page_size, num_pages)) return 1;
+  if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
+    CO_FAIL("kv4_pages: operands must be 16-byte aligned");
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, status,
+                      stream);
+}
+
+CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, long out_ld, int dtype, const void* k_cache, const void* v_cache,
+                                           int num_pages, const int* table, int table_ld, const int* token_req, const int* positions, int T,
+                                           int nh, int nkv, int page_size, int window, float scale, int* status, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (check_pages("kv4_attention", nkv, page_size, num_pages)) return 1;
+  if (nh < 1 || nh % nkv || nkv > 65535) CO_FAIL("kv4_attention: %d heads do not group over %d kv heads", nh, nkv);
+  if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15)) CO_FAIL("kv4_attention: caches must be 16-byte aligned");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  const dim3 grid((unsigned)T, (unsigned)nkv);
+  if (dtype == CO_F32)
+    co_launch(kv4_simple_kernel<float>, grid, dim3(32 * SW), 0, stream, (const float*)q, q_ld, (float*)out, out_ld, (const unsigned char*)k_cache,
+              (const unsigned char*)v_cache, num_pages, table, table_ld, token_req, positions, nh, nkv, page_size, window, scale_log2, status);
+  else
+    co_launch(kv4_simple_kernel<bf16>, grid, dim3(32 * SW), 0, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld, (const unsigned char*)k_cache,
+              (const unsigned char*)v_cache, num_pages, table, table_ld, token_req, positions, nh, nkv, page_size, window, scale_log2, status);
+  CO_CHECK_LAUNCH("kv4_attention_simple");
+  return 0;
+}
+
+// Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests that it takes.
+CO_EXPORT long coheryn_kv4_scratch_floats(int B, int nkv, int max_rows, int max_kv_len) {
+  return (long)(items_bound(B, nkv, max_rows, max_kv_len) * 8 * tiles_of(max_rows) * (HD + 2));
+}
+
+// Attention of the requests with at most `max_rows` query rows per kv head, in bfloat16: q [T, nh * HD] of stride q_ld, out likewise;
+// request b's rows are tokens cu_q[b] .. cu_q[b + 1], at the last positions of its kv_lens[b].  Other requests' rows are left.
+CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long out_ld, const void* k_cache, const void* v_cache, int num_pages,
+                                    const int* table, int table_ld, const int* cu_q, const int* kv_lens, int B, int nh, int nkv, int page_size,
+                                    int window, float scale, int max_rows, int max_kv_len, float* scratch, long scratch_floats, int* status,
+                                    cudaStream_t stream) {
+  if (B <= 0 || max_rows <= 0) return 0;
+  if (check_pages("kv4_attention", nkv, page_size, num_pages)) return 1;
+  if (nh < 1 || nh % nkv || nkv > 65535) CO_FAIL("kv4_attention: %d heads do not group over %d kv heads", nh, nkv);
+  if ((q_ld & 7) || (out_ld & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15))
+    CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
+  if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
+  const int nt = tiles_of(max_rows);
+  const long long items = items_bound(B, nkv, max_rows, max_kv_len);
+  if (items > 0x7fffffffLL) CO_FAIL("kv4_attention: %d requests of %d kv heads", B, nkv);
+  if (scratch_floats < coheryn_kv4_scratch_floats(B, nkv, max_rows, max_kv_len) || ((uintptr_t)scratch & 15))
+    CO_FAIL("kv4_attention: the scratch is too small or not 16-byte aligned");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  const int rc = nt == 1 ? launch_items<1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
+                                           window, scale_log2, max_rows, (int)items, scratch, status, stream)
+                         : launch_items<HD <= 128 ? 2 : 1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
+                                           window, scale_log2, max_rows, (int)items, scratch, status, stream);
+  if (rc || max_kv_len + 15 <= UNIT) return rc;    // no request is longer than one unit: nothing to join
+  co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, (int)items,
+            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows, items_target());
+  CO_CHECK_LAUNCH("kv4_join");
+  return 0;
+}
+
+// The pages of requests b = 0..n-1 of a block table in bfloat16, dense: entry (b, j) becomes page b * width + j of k_out and v_out
+// [n * width, nkv, page_size, HD] and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length are zeros.
+CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
+                                 int width, int n, const int* cu_q, const int* kv_lens, int window, void* k_out, void* v_out, int* out_table,
+                                 int* status, cudaStream_t stream) {
+  if (n <= 0 || width <= 0) return 0;
+  if (check_pages("kv4_expand", nkv, page_size, num_pages)) return 1;
+  if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
+    CO_FAIL("kv4_expand: operands must be 16-byte aligned");
+  if (width > table_ld) CO_FAIL("kv4_expand: %d entries of rows of %d", width, table_ld);
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, n, cu_q, kv_lens, window, k_out, v_out, CO_BF16,
+                      out_table, status, stream);
+}

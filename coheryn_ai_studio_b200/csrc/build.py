@@ -30,7 +30,7 @@ BASE_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompil
 # The core library: everything that is not specialised by a compile-time size.
 CORE_SOURCES = ["runtime.cu", "elementwise.cu", "gemm_simt.cu", "attention_simple.cu",
                 "sampling.cu", "gemm_bf16_small.cu", "gemm_tc.cu", "gemm_tc_few.cu", "gemm_f32_tc.cu", "seeded_fill.cu", "selftest.cu",
-                "block_runner.cu", "mixer_runner.cu", "stream_ops.cu"]
+                "block_runner.cu", "mixer_runner.cu", "stream_ops.cu", "step_layout.cu"]
 ROUTED_SOURCES = ["routed.cu", "runtime.cu"]
 RECURRENT_SOURCES = ["recurrent.cu", "recurrent_one.cu", "delta_chunks.cu", "memory_chunks.cu", "memory_chunks_tc.cu", "runtime.cu"]
 VARIANT_SOURCES = ["attention_variants.cu", "runtime.cu"]
@@ -249,6 +249,14 @@ def attention_options_library(dk: int, dv: int) -> ctypes.CDLL:
     return load_library(f"attn_options_{dk}_{dv}", ["attention_tc.cu", "runtime.cu"], {"CO_HEAD_DIM": dk, "CO_VALUE_DIM": dv})
 
 
+def kv4_library(head_dim: int) -> ctypes.CDLL:
+    """The kernels of a cache that keeps keys and values in 4 bits (write, read back, attention over its pages), compiled for
+    one head size when a cache of that kind is first used."""
+    if head_dim % 32 != 0 or not 32 <= head_dim <= 256:
+        raise BuildError(f"the 4-bit cache takes head sizes 32..256 in steps of 32, not {head_dim}")
+    return load_library(f"kv4_hd{head_dim}", ["attention_kv4.cu", "runtime.cu"], {"CO_HEAD_DIM": head_dim})
+
+
 def recurrent_library() -> ctypes.CDLL:
     """The kernels of mixers with a state of fixed size per request (short convolution, gated delta rule,
     matrix memory), compiled when a model with such a mixer is first run."""
@@ -333,6 +341,8 @@ def build_all(head_dims: Sequence[int] = (16, 32, 64, 128)) -> List[str]:
     for dk, dv, maps in ((64, 128, 2), (64, 64, 1)):
         paths.append(build_library(f"maps_{dk}_{dv}_{maps}", ["attention_maps_tc.cu", "runtime.cu"],
                                    {"CO_MAPS_DK": dk, "CO_MAPS_DV": dv, "CO_MAPS_N": maps}))
+    for hd in (64, 128):
+        paths.append(build_library(f"kv4_hd{hd}", ["attention_kv4.cu", "runtime.cu"], {"CO_HEAD_DIM": hd}))
     for hd in head_dims:
         paths.append(build_library(f"attn_hd{hd}", ["attention_bf16.cu", "attention_tc.cu", "runtime.cu"],
                                    {"CO_HEAD_DIM": hd}))

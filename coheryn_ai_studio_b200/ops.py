@@ -58,7 +58,7 @@ def launch_count() -> int:
 def total_launch_count() -> int:
     """Kernel launches made through every library of this package that is loaded."""
     n = launch_count()
-    for lib in list(_attn_libs.values()) + list(_maps_libs.values()) + list(_options_libs.values()) + list(_pooled_tc_libs.values()) + [
+    for lib in list(_attn_libs.values()) + list(_maps_libs.values()) + list(_options_libs.values()) + list(_pooled_tc_libs.values()) + list(_kv4_libs.values()) + [
             l for l in (_recurrent, _variants, _routed, _linear_recurrence, _pooled, _linear_attention, _lightning) if l is not None]:
         n += int(lib.coheryn_launch_count())
     return n
@@ -633,7 +633,9 @@ def tc_status(device) -> torch.Tensor:
     return t
 
 
-STATUS_MESSAGES = {1: "a token id was outside the embedding table", 2: "non-finite logits"}
+STATUS_MESSAGES = {1: "a token id was outside the embedding table", 2: "non-finite logits",
+                   41: "a slot, a position or a block-table entry lies outside its table (4-bit cache)",
+                   51: "a step's lengths are negative or do not fit its arrays", 52: "a step's pages do not hold its positions"}
 
 
 def describe_status(code: int) -> str:
@@ -2121,3 +2123,241 @@ def lightning_attention(q, k, v, gate, powers: torch.Tensor, silu: bool, state: 
         _ptr(norm_weight), c_int(_code(norm_weight)), c_float(eps), c_int({"sigmoid": 0, "silu": 1}[gate_activation]),
         c_float(out_scale), _ptr(out), c_int(_code(out)), c_long(out.stride(0)), _ptr(scratch), c_long(floats), c_int(T), c_int(B),
         c_int(heads), c_int(dk), c_int(dv), c_int(longest), c_int(few), _stream()))
+
+
+# ------------------------------------------------------------------------------------
+# The step's index arrays made on the device.
+
+
+def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tensor, pages: torch.Tensor, page_size: int,
+                block_table: torch.Tensor, slots: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
+                kv_lens: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                token_req: Optional[torch.Tensor] = None, first: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> None:
+    """The index arrays of a step from its requests' lengths, in one launch (all int32 on the device).
+
+    Request b holds ``starts[b]`` positions, brings ``q_lens[b]`` tokens and owns the pages
+    ``pages[page_cu[b]:page_cu[b + 1]]``.  Written: ``block_table`` [B, W] (row b: its pages, then -1) and, where given,
+    ``cu_q`` [B + 1] (token offsets), ``kv_lens`` [B] (starts + q_lens), and per token ``positions``, ``token_req`` and
+    ``slots`` (page * page_size + offset; -1 where the page is missing), each [T].  Rows of the latter behind the last token
+    stay as they are.  With ``first`` [B] the listed pages are entries first[b].. of row b, and the rest of the row stays
+    as it is: a table that is kept from step to step gets only what it has gained.
+    ``status`` (int32 [1]) is set to 51 when a length is negative or the tokens do not fit the arrays, to 52 when the
+    lists do not hold the positions; nothing outside the arrays is read or written then.
+
+    An ordinary launch: the arrays are complete before the next kernel in the stream begins, so kernels that look at a
+    step's lengths ahead of their wait may follow it directly."""
+    _dev(starts, q_lens, page_cu, pages, block_table, slots, cu_q, kv_lens, positions, token_req, first, status)
+    B, T = starts.numel(), -1
+    for t, name, n in ((starts, "starts", B), (q_lens, "q_lens", B), (page_cu, "page_cu", B + 1), (pages, "pages", None),
+                       (block_table, "block_table", None), (cu_q, "cu_q", B + 1), (kv_lens, "kv_lens", B), (first, "first", B),
+                       (status, "status", 1)):
+        if t is not None:
+            _i32(t, name)
+            if n is not None and t.numel() != n:
+                raise KernelError(f"step_layout: {name} has {t.numel()} elements, not {n}")
+    for t, name in ((positions, "positions"), (token_req, "token_req"), (slots, "slots")):
+        if t is not None:
+            _i32(t, name)
+            if T >= 0 and t.numel() != T:
+                raise KernelError(f"step_layout: {name} has {t.numel()} elements, not {T}")
+            T = t.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise KernelError(f"step_layout: a block table of shape {tuple(block_table.shape)} for {B} requests")
+    if page_size < 1:
+        raise KernelError("step_layout: page_size must be positive")
+    if B == 0:
+        if cu_q is not None:
+            cu_q.zero_()
+        return
+    lib = core()
+    _check(lib, lib.coheryn_step_layout(_ptr(starts), _ptr(q_lens), _ptr(page_cu), _ptr(pages), c_int(pages.numel()), _ptr(first), c_int(B),
+                                        c_int(max(T, 0)), c_int(page_size), _ptr(cu_q), _ptr(kv_lens), _ptr(positions), _ptr(token_req),
+                                        _ptr(block_table), c_int(block_table.shape[1]), _ptr(slots), _ptr(status), _stream()))
+
+
+# ------------------------------------------------------------------------------------
+# A cache that keeps keys and values in 4 bits (csrc/attention_kv4.cu has the format).
+_kv4_libs = {}
+
+# Requests with at most this many query rows (tokens times heads of a group) read the 4-bit pages directly; longer portions
+# have their pages expanded to bfloat16 once and go through the prompt kernels.
+KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "64"))
+
+# The expanded pages of a call take at most about this many bytes at a time (one request always goes in one piece).
+KV4_EXPAND_BYTES = 1 << 30
+
+
+def kv4_lib(head_dim: int):
+    lib = _kv4_libs.get(head_dim)
+    if lib is None:
+        try:
+            lib = build.kv4_library(head_dim)
+        except build.BuildError as e:
+            raise KernelError(str(e)) from None
+        lib.coheryn_last_error.restype = ctypes.c_char_p
+        lib.coheryn_launch_count.restype = ctypes.c_ulonglong
+        lib.coheryn_kv4_scratch_floats.restype = c_long
+        if lib.coheryn_kv4_head_dim() != head_dim:
+            raise KernelError(f"the library of the 4-bit cache was built for head size {lib.coheryn_kv4_head_dim()}, not {head_dim}")
+        _kv4_libs[head_dim] = lib
+    return lib
+
+
+def kv4_page_shape(num_kv_heads: int, page_size: int, head_dim: int):
+    """The shape of one page of keys, or of values, in uint8: [kv heads, tiles of 16 positions, bytes of a tile]."""
+    if head_dim % 32 or not 32 <= head_dim <= 256:
+        raise KernelError(f"the 4-bit cache takes head sizes 32..256 in steps of 32, not {head_dim}")
+    if page_size % 16 or page_size < 16:
+        raise KernelError(f"the 4-bit cache takes pages of a multiple of 16 positions, not {page_size}")
+    return (num_kv_heads, page_size // 16, 10 * head_dim)
+
+
+def _kv4_caches(k_cache, v_cache, num_kv_heads: int, page_size: int, head_dim: int) -> None:
+    shape = kv4_page_shape(num_kv_heads, page_size, head_dim)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype != torch.uint8 or t.dim() != 4 or tuple(t.shape[1:]) != shape or not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous uint8 pages of shape {shape}, not {t.dtype} {tuple(t.shape)}")
+    if k_cache.shape[0] != v_cache.shape[0]:
+        raise KernelError("the key and the value cache have different numbers of pages")
+
+
+def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], slots: torch.Tensor,
+                   k_cache: torch.Tensor, v_cache: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
+                   page_size: int) -> torch.Tensor:
+    """Rotate q and k by position and write k and v into 4-bit pages at ``slots`` (page * page_size + offset; a row
+    with a negative slot is not kept).  ``qkv`` [T, (heads + 2 kv heads) * head_dim] (rows may be strided) stays as it is;
+    the rotated queries [T, heads * head_dim] are returned (a view of ``qkv`` when ``rotary_dim`` is 0; ``positions`` and
+    ``cos_sin`` may then be None).  Keys are rounded to the compute type before they are quantised.  A group of 32
+    channels with a value that is not finite is kept as not-a-number.  Two rows with one slot: one of them is kept, or a
+    mixture."""
+    _dev(qkv, positions, cos_sin, slots, k_cache, v_cache)
+    _i32(slots, "slots")
+    T = qkv.shape[0]
+    _kv4_caches(k_cache, v_cache, num_kv_heads, page_size, head_dim)
+    nq = num_heads * head_dim
+    if qkv.dim() != 2 or qkv.shape[1] != nq + 2 * num_kv_heads * head_dim or qkv.stride(1) != 1 or slots.numel() != T:
+        raise KernelError(f"rope_kv4_write: rows of {num_heads} + 2 x {num_kv_heads} heads of {head_dim} and a slot each, not "
+                          f"{tuple(qkv.shape)} with {slots.numel()} slots")
+    if rotary_dim:
+        if positions is None or cos_sin is None or positions.numel() != T:
+            raise KernelError("rope_kv4_write: a rotation needs a position for every row and a table")
+        _i32(positions, "positions")
+        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or tuple(cos_sin.shape[1:]) != (rotary_dim // 2, 2):
+            raise KernelError(f"rope_kv4_write: cos_sin must be float32 [positions, {rotary_dim // 2}, 2]")
+        q = torch.empty((T, nq), dtype=qkv.dtype, device=qkv.device)
+    else:
+        q = qkv[:, :nq]
+    lib = kv4_lib(head_dim)
+    _check(lib, lib.coheryn_kv4_write(
+        _ptr(qkv), c_long(qkv.stride(0)), c_int(_code(qkv)), _ptr(positions), _ptr(cos_sin), c_int(cos_sin.shape[0] if rotary_dim else 0),
+        _ptr(slots), _ptr(k_cache), _ptr(v_cache), c_int(k_cache.shape[0]), _ptr(q if rotary_dim else None), c_int(T), c_int(num_heads),
+        c_int(num_kv_heads), c_int(rotary_dim), c_int(page_size), _ptr(tc_status(qkv.device)), _stream()))
+    return q
+
+
+def kv4_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor, head_dim: int, page_size: int, dtype: torch.dtype):
+    """Pages of a 4-bit cache as the values they stand for: (keys, values), each [n, kv heads, page_size, head_dim] in
+    ``dtype``.  A page number outside the cache reads as zeros."""
+    _dev(k_cache, v_cache, pages)
+    _i32(pages, "pages")
+    nkv = k_cache.shape[1]
+    _kv4_caches(k_cache, v_cache, nkv, page_size, head_dim)
+    if dtype not in _CODES:
+        raise KernelError(f"dtype {dtype} is not handled by the kernels")
+    n = pages.numel()
+    k = torch.empty((n, nkv, page_size, head_dim), dtype=dtype, device=k_cache.device)
+    v = torch.empty_like(k)
+    lib = kv4_lib(head_dim)
+    _check(lib, lib.coheryn_kv4_pages(_ptr(k_cache), _ptr(v_cache), c_int(k_cache.shape[0]), c_int(nkv), c_int(page_size), _ptr(pages), c_int(n),
+                                      _ptr(k), _ptr(v), c_int(_CODES[dtype]), _ptr(tc_status(k_cache.device)), _stream()))
+    return k, v
+
+
+def attention_kv4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, step, group: int, num_heads: int,
+                  num_kv_heads: int, head_dim: int, page_size: int, window: Optional[int], scale: float) -> None:
+    """``attention`` over the 4-bit pages of ``group``."""
+    attention_kv4_rows(q, out, k_cache, v_cache, step.block_tables[group], step.token_req, step.positions, num_heads, num_kv_heads,
+                       head_dim, page_size, window, scale, cu_q=step.cu_q, kv_lens=step.kv_lens, q_lens=step.q_lens,
+                       max_kv_len=step.max_kv_len)
+
+
+def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads, num_kv_heads, head_dim, page_size, window,
+                       scale, cu_q=None, kv_lens=None, q_lens=None, max_kv_len=None, force_simple=False) -> None:
+    """Attention of rows (request token_req[i] at position positions[i]) over the 4-bit pages of a cache, causal, with an
+    optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros.
+    bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
+    ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``KV4_DIRECT_ROWS`` rows per kv
+    head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to bfloat16 and
+    go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
+    _dev(q, out, k_cache, v_cache, block_tables, token_req, positions, cu_q, kv_lens)
+    _i32(block_tables, "block_tables")
+    _kv4_caches(k_cache, v_cache, num_kv_heads, page_size, head_dim)
+    if num_heads % num_kv_heads:
+        raise KernelError(f"{num_heads} heads do not group over {num_kv_heads} kv heads")
+    T, nq = q.shape[0], num_heads * head_dim
+    if q.dim() != 2 or q.shape[1] != nq or tuple(out.shape) != (T, nq) or q.stride(1) != 1 or out.stride(1) != 1 or out.dtype != q.dtype:
+        raise KernelError(f"attention_kv4: q and out must be [tokens, {nq}] of one type with contiguous rows")
+    if block_tables.dim() != 2:
+        raise KernelError("attention_kv4: block_tables must be [requests, entries]")
+    if window is not None and window < 1:
+        raise KernelError("an attention window must hold at least one position")
+    if T == 0:
+        return
+    lib = kv4_lib(head_dim)
+    fast = (not force_simple and q.dtype == torch.bfloat16 and cu_q is not None and kv_lens is not None and q_lens is not None
+            and max_kv_len is not None and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 4 == 0
+            and out.data_ptr() % 8 == 0)
+    status = tc_status(q.device)
+    num_pages, W = k_cache.shape[0], block_tables.shape[1]
+    if not fast:
+        _i32(token_req, "token_req"); _i32(positions, "positions")
+        if token_req.numel() != T or positions.numel() != T:
+            raise KernelError("attention_kv4: every row needs a request and a position")
+        _check(lib, lib.coheryn_kv4_attention_simple(
+            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), c_int(_code(q)), _ptr(k_cache), _ptr(v_cache), c_int(num_pages),
+            _ptr(block_tables), c_int(W), _ptr(token_req), _ptr(positions), c_int(T), c_int(num_heads), c_int(num_kv_heads),
+            c_int(page_size), c_int(window or 0), c_float(scale), _ptr(status), _stream()))
+        return
+    _i32(cu_q, "cu_q"); _i32(kv_lens, "kv_lens")
+    B, G = len(q_lens), num_heads // num_kv_heads
+    if cu_q.numel() != B + 1 or kv_lens.numel() != B or block_tables.shape[0] != B:
+        raise KernelError(f"attention_kv4: lengths and block tables of {B} requests are needed")
+    limit = max(KV4_DIRECT_ROWS // G, 1)         # tokens that a request may bring to be read directly
+    direct = max((n for n in q_lens if n <= limit), default=0)
+    if direct:
+        floats = int(lib.coheryn_kv4_scratch_floats(c_int(B), c_int(num_kv_heads), c_int(direct * G), c_int(max_kv_len)))
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        _check(lib, lib.coheryn_kv4_attention(
+            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), _ptr(k_cache), _ptr(v_cache), c_int(num_pages),
+            _ptr(block_tables), c_int(W), _ptr(cu_q), _ptr(kv_lens), c_int(B), c_int(num_heads), c_int(num_kv_heads), c_int(page_size),
+            c_int(window or 0), c_float(scale), c_int(direct * G), c_int(max_kv_len), _ptr(scratch), c_long(floats), _ptr(status), _stream()))
+    if max(q_lens) <= limit:
+        return
+    # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.
+    width = min(W, -(-max_kv_len // page_size))
+    most = max(1, min(65535, KV4_EXPAND_BYTES // max(1, width * num_kv_heads * page_size * head_dim * 4)))
+    prompt = attention_lib(head_dim)
+    b = 0
+    while b < B:
+        e = b
+        while e < B and e - b < most and q_lens[e] > limit:
+            e += 1
+        if e == b:
+            b += 1
+            continue
+        n = e - b
+        k = torch.empty((n * width, num_kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
+        v = torch.empty_like(k)
+        table = torch.empty((n, width), dtype=torch.int32, device=q.device)
+        cu, lens = c_void_p(cu_q.data_ptr() + 4 * b), c_void_p(kv_lens.data_ptr() + 4 * b)
+        _check(lib, lib.coheryn_kv4_expand(
+            _ptr(k_cache), _ptr(v_cache), c_int(num_pages), c_int(num_kv_heads), c_int(page_size),
+            c_void_p(block_tables.data_ptr() + 4 * W * b), c_int(W), c_int(width), c_int(n), cu, lens, c_int(window or 0), _ptr(k), _ptr(v),
+            _ptr(table), _ptr(status), _stream()))
+        rows = max(q_lens[b:e]) * G
+        _check(prompt, prompt.coheryn_attention_bf16(
+            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), _ptr(k), _ptr(v), _ptr(table), c_int(width), cu, lens, c_int(n),
+            c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
+            c_int(max_kv_len), c_void_p(0), c_long(0), _ptr(status), c_int(T), c_int(n * width), c_int(0), _stream()))
+        b = e
