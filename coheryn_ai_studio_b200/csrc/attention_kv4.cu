@@ -15,8 +15,9 @@
 //  * values: for group u, lane (g, t), p = 0, 1 a word: low half row 4 t + 2 p, high half row 4 t + 2 p + 1, each
 //    channels 32 u + 4 g + 0..3; then for (u, t) the scales of rows 4 t..4 t + 3 and their minima.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "tc_common.cuh"
 
 #ifndef CO_HEAD_DIM
 #define CO_HEAD_DIM 128
@@ -506,35 +507,43 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 }
 // ------------------------------------------------------------------------------------
 // Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
-// each with tiles of 16 positions of its own (tile i of the item goes to warp i mod 4) in a ring of its own that
-// cp.async fills, so that warps never wait for one another before the end.  Decoding is bound by the cache's bytes, and
-// with 5 bits a value nearly as much by the instructions that turn codes into operands; hence:
+// each with tiles of 16 positions of its own (tile i of the item goes to warp i mod 4) in a ring of its own that bulk
+// copies fill (two per tile, one thread), so that warps never wait for one another before the end.  Decoding is
+// bound by the cache's bytes, and with 5 bits a value nearly as much by the instructions that turn codes into operands,
+// those of the half-rate integer pipe first; hence:
 //  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
 //    of up to 8 heads wastes no product;
-//  * keys: code c enters the product as the bfloat16 128 + c (one lop3 for two codes); the accumulator starts at
-//    -128 sum(q), so that it ends as sum(q c), and the group's s and m multiply float32 sums: score += s D + m sum(q).
-//    No key is rounded;
+//  * keys: code c enters the product as the float16 1024 + c (places 0 and 2 of a half word) or 64 + c (places 1 and 3): one
+//    lop3 for two codes, one shift for eight.  The accumulator starts at minus the sum of q times those constants, so that
+//    it ends as sum(q c), and the group's scale multiplies float32 sums; the minima's share, sum over the groups of
+//    m sum(q), is one product more, with sum(q) as three bfloat16 terms.  No key is rounded.  Queries enter as
+//    float16 divided by the power of two that brings the row's largest to 1..2: exact, but for elements under 2^-14
+//    of it, which are off by at most 2^-25 of it;
 //  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs);
 //  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
 //  * the running maximum moves (and the accumulators are scaled) only when a tile holds a larger score than the warp has
 //    seen in any row of it.
-// The rows' sums stay per lane and meet once at the end, as do the warps.
+// The rows' sums stay per lane and meet once at the end, as do the warps.  Every wait is bounded: on expiry the
+// kernel records a code in `status` and winds down.
 // ------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
-constexpr int STAGES = 4;
-constexpr int PIECES = 2 * TB / 16;      // 16-byte pieces of a key and a value tile
+constexpr int STAGES = 4;                // a power of two
+constexpr int GAVE_UP = 40;              // status: a bounded wait ran out
+constexpr float NOTHING = -3.0e38f;      // a running maximum that no score has met
 
-__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;  // src-size 0 fills the 16 bytes with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -548,8 +557,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));   // ex2(-inf) = +0
   return y;
 }
-// Codes j and j + 4 of a word as the bfloat16 pair 128 + c.
+// Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair 1024 + c (j even) or 64 + c (j odd).
 __device__ __forceinline__ unsigned codes128(unsigned word, int j) { return ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ unsigned codes16(unsigned word, int j) {
+  const unsigned w = j < 2 ? word : word >> 8;
+  return j & 1 ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u;
+}
+__device__ __forceinline__ unsigned pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
 template <int N>
 __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) {
   if constexpr (N % 4 == 0) {
@@ -576,22 +593,28 @@ constexpr size_t items_smem() {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * WARPS)
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 && HD <= 128 ? 4 : 1)
 kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
                  const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
                  float scale_log2, int max_rows, int target, float* __restrict__ scratch, int items, int* __restrict__ status) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int COLS = 8 * NT;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ unsigned long long bars[WARPS][STAGES];
+  constexpr int COLS = 8 * NT, MG = (NG + 3) / 4;      // MG: products for the minima
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[warp][i], 1);
+    fence_proxy_async();
+  }
+  __syncwarp();
   co_pdl_wait();
   co_pdl_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int G = nh / nkv;
   const Item it = find_item(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, target, blockIdx.x);
   if (it.b < 0) return;
   const Cut c = it.cut;
-  const int rows = min(COLS, c.q_len * G - it.row_tile * COLS);      // of this tile
-  const int row0 = it.row_tile * COLS;
+  const int row0 = it.row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
   const int* table = block_tables + (size_t)it.b * table_ld;
   const int u_first = (int)((long long)c.units * it.part / it.parts), u_end = (int)((long long)c.units * (it.part + 1) / it.parts);
   const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
@@ -600,70 +623,90 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   const int base_pos = c.kv_len - c.q_len;
 
   unsigned char* ring = smem + (size_t)warp * STAGES * 2 * TB;
-  const unsigned ring_addr = smem_addr(ring);
-  // Block-table entries of the warp's tiles, 32 tiles at a time, a lane each.
-  int entry = -1;
-  auto fetch_entries = [&](int i0) {
-    const int tile = tile0 + (i0 + lane) * WARPS;
-    const int blk = tile * 16 / page_size;
-    entry = i0 + lane < n_tiles && blk < table_ld ? table[blk] : -1;
-    if (i0 + lane < n_tiles && (entry < 0 || entry >= num_pages)) {
-      entry = -1;
-      if (status) *status = BAD_INDEX;
+  // Where the warp's tiles lie in a cache, 32 tiles at a time, a lane each; -1: not in the pool.
+  long long place = -1;
+  auto fetch_places = [&](int i0) {
+    const int tile = tile0 + (i0 + lane) * WARPS, per_page = page_size >> 4;
+    place = -1;
+    if (i0 + lane < n_tiles) {
+      const int blk = tile / per_page, page = blk < table_ld ? table[blk] : -1;
+      if (page >= 0 && page < num_pages) place = (((long long)page * nkv + it.kvh) * per_page + (tile - blk * per_page)) * TB;
+      else if (status) *status = BAD_INDEX;
     }
   };
-  unsigned known = 0;      // bit i % STAGES: the tile in that stage came from a page of the pool
+  unsigned known = 0;      // bit of a stage: its tile came from a page of the pool, so copies fill it
   auto issue = [&](int i) {
-    if (i < n_tiles) {
-      if ((i & 31) == 0) fetch_entries(i);
-      const int page = __shfl_sync(0xffffffffu, entry, i & 31);
-      const int pos = (tile0 + i * WARPS) * 16;
-      const size_t at = page < 0 ? 0 : tile_at(page, nkv, it.kvh, page_size, pos % page_size);
-      const unsigned dst = ring_addr + (i % STAGES) * 2 * TB;
-#pragma unroll
-      for (int p0 = 0; p0 < PIECES; p0 += 32) {
-        const int p = p0 + lane;
-        if (PIECES % 32 == 0 || p < PIECES)
-          cp_async16(dst + p * 16, p < TB / 16 ? k_cache + at + p * 16 : v_cache + at + p * 16 - TB, page >= 0);
-      }
-      known = (known & ~(1u << (i % STAGES))) | (page >= 0 ? 1u << (i % STAGES) : 0u);
+    if (i >= n_tiles) return;
+    if ((i & 31) == 0) fetch_places(i);
+    const long long at = __shfl_sync(0xffffffffu, place, i & 31);
+    const int stage = i % STAGES;
+    known = at < 0 ? known & ~(1u << stage) : known | 1u << stage;
+    if (at >= 0 && lane == 0) {
+      unsigned char* dst = ring + stage * 2 * TB;
+      mbar_expect_tx(&bars[warp][stage], 2 * TB);
+      bulk_load(dst, k_cache + at, TB, &bars[warp][stage]);
+      bulk_load(dst + TB, v_cache + at, TB, &bars[warp][stage]);
     }
-    cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
   // The queries as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
   unsigned qf[NT][NG][4];
-  float sq[NT][NG][2];        // sum of the group's channels of rows 2 t, 2 t + 1
+  float start[NT][NG][2];         // of the accumulators of rows 2 t, 2 t + 1
+  unsigned sums[NT][MG][2];       // sum(q) of row g, group 4 i + t, in three terms
+  float cs[NT][2];                // what the scores of rows 2 t, 2 t + 1 are multiplied by
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g, row = row0 + r;
     const bf16* src = q + (size_t)(c.tok0 + row / G) * q_ld + (size_t)(it.kvh * G + row % G) * HD;
+    uint4 v[NG];
+    float most = 0.f;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) v = *reinterpret_cast<const uint4*>(src + u * 32 + t * 8);
-      qf[nt][u][0] = __byte_perm(v.x, v.z, 0x5410);       // channels 0, 4
-      qf[nt][u][1] = __byte_perm(v.x, v.z, 0x7632);       // 1, 5
-      qf[nt][u][2] = __byte_perm(v.y, v.w, 0x5410);
-      qf[nt][u][3] = __byte_perm(v.y, v.w, 0x7632);
-      float sum = ((lo_bf16(v.x) + hi_bf16(v.x)) + (lo_bf16(v.y) + hi_bf16(v.y))) + ((lo_bf16(v.z) + hi_bf16(v.z)) + (lo_bf16(v.w) + hi_bf16(v.w)));
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sq[nt][u][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-      sq[nt][u][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows) v[u] = *reinterpret_cast<const uint4*>(src + u * 32 + t * 8);
+      const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(lo_bf16(w[i])), fabsf(hi_bf16(w[i]))));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^-e with 2^e <= most < 2^(e + 1), e from -126 to 126
+    const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
+    const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
+    cs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t);
+    cs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t + 4);
+#pragma unroll
+    for (int i = 0; i < MG; ++i) sums[nt][i][0] = sums[nt][i][1] = 0;
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __half2float(__float2half_rn(lo_bf16(w[i]) * down));
+        x[2 * i + 1] = __half2float(__float2half_rn(hi_bf16(w[i]) * down));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[nt][u][j] = pack_f16(x[j], x[j + 4]);
+      float even = (x[0] + x[4]) + (x[2] + x[6]), odd = (x[1] + x[5]) + (x[3] + x[7]);
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        even += __shfl_xor_sync(0xffffffffu, even, o);
+        odd += __shfl_xor_sync(0xffffffffu, odd, o);
+      }
+      const float first = -(1024.f * even + 64.f * odd);
+      start[nt][u][0] = __shfl_sync(0xffffffffu, first, 8 * t);
+      start[nt][u][1] = __shfl_sync(0xffffffffu, first, 8 * t + 4);
+      if (t == (u & 3)) {
+        const float sum = even + odd;
+        const float a = __bfloat162float(__float2bfloat16_rn(sum)), b = __bfloat162float(__float2bfloat16_rn(sum - a));
+        sums[nt][u >> 2][0] = pack(a, b);
+        sums[nt][u >> 2][1] = pack(sum - a - b, 0.f);
+      }
     }
   }
-  int hi[NT][2], lo[NT][2];   // visible positions of rows 2 t, 2 t + 1 of every eight
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = nt * 8 + 2 * t + e;
-      hi[nt][e] = r < rows ? base_pos + (row0 + r) / G : -1;
-      lo[nt][e] = window > 0 ? max(0, hi[nt][e] - window + 1) : 0;
-    }
   // Positions [all_lo, all_hi] are visible to every row of the tile.
   const int all_hi = base_pos + row0 / G, last = base_pos + (row0 + rows - 1) / G;
   const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
@@ -672,7 +715,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   float m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
+    m[nt][0] = m[nt][1] = NOTHING;
     l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int u = 0; u < NG; ++u)
@@ -683,55 +726,90 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   }
   const int r0 = 4 * (g >> 1) + (g & 1);        // this lane's rows of a tile in the first product: r0 and r0 + 2
   const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
+  unsigned phases = 0;
+  bool gave_up = false;
 
 #pragma unroll 1
   for (int i = 0; i < n_tiles; ++i) {
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();                               // landed for all lanes; all are done with the stage of tile i - 1
-    const bool usable = (known >> (i % STAGES)) & 1;
+    const int stage = i % STAGES;
+    const bool usable = (known >> stage) & 1;
+    if (usable) {
+      gave_up = !mbar_wait(&bars[warp][stage], (phases >> stage) & 1) || gave_up;
+      phases ^= 1u << stage;
+    }
+    __syncwarp();                               // all lanes are done with the stage of tile i - 1
+    if (__any_sync(0xffffffffu, gave_up)) {     // copies that are still in flight end before the memory is used again
+      for (int j = i + 1; j < min(n_tiles, i + STAGES - 1); ++j)
+        if ((known >> (j % STAGES)) & 1) mbar_wait(&bars[warp][j % STAGES], (phases >> (j % STAGES)) & 1);
+      gave_up = true;
+      break;
+    }
     issue(i + STAGES - 1);
     if (!usable) continue;
-    const unsigned char* kt = ring + (i % STAGES) * 2 * TB;
+    const unsigned char* kt = ring + stage * 2 * TB;
     const unsigned char* vt = kt + TB;
     const int key0 = (tile0 + i * WARPS) * 16;
 
     float s[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
     {
       unsigned ka[NG], kb[NG], pa[NG], pb[NG];
       load_words<NG>(reinterpret_cast<const unsigned*>(kt) + r0 * (4 * NG) + t * NG, ka);
       load_words<NG>(reinterpret_cast<const unsigned*>(kt) + (r0 + 2) * (4 * NG) + t * NG, kb);
-      load_words<NG>(reinterpret_cast<const unsigned*>(kt + CODES) + r0 * NG, pa);
-      load_words<NG>(reinterpret_cast<const unsigned*>(kt + CODES) + (r0 + 2) * NG, pb);
+      const unsigned* pairs = reinterpret_cast<const unsigned*>(kt + CODES);
+      load_words<NG>(pairs + r0 * NG, pa);
+      load_words<NG>(pairs + (r0 + 2) * NG, pb);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int x = 0; x < MG; ++x) {
+        const int u = min(4 * x + t, NG - 1);
+        const unsigned wa = pairs[r0 * NG + u], wb = pairs[(r0 + 2) * NG + u];
+        const unsigned a = __byte_perm(wa, wa, 0x3232), b = __byte_perm(wb, wb, 0x3232);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], a, b, a, b, sums[nt][x][0], sums[nt][x][1]);
+      }
 #pragma unroll
       for (int u = 0; u < NG; ++u) {
         unsigned a[4], b[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { a[j] = codes128(ka[u], j); b[j] = codes128(kb[u], j); }
-        const float sa = lo_bf16(pa[u]), ma = hi_bf16(pa[u]), sb = lo_bf16(pb[u]), mb = hi_bf16(pb[u]);
+        for (int j = 0; j < 4; ++j) { a[j] = codes16(ka[u], j); b[j] = codes16(kb[u], j); }
+        const float sa = lo_bf16(pa[u]), sb = lo_bf16(pb[u]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {-128.f * sq[nt][u][0], -128.f * sq[nt][u][1], -128.f * sq[nt][u][0], -128.f * sq[nt][u][1]};
-          mma_bf16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
-          mma_bf16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
-          s[nt][0] = fmaf(sa, d[0], fmaf(ma, sq[nt][u][0], s[nt][0]));
-          s[nt][1] = fmaf(sa, d[1], fmaf(ma, sq[nt][u][1], s[nt][1]));
-          s[nt][2] = fmaf(sb, d[2], fmaf(mb, sq[nt][u][0], s[nt][2]));
-          s[nt][3] = fmaf(sb, d[3], fmaf(mb, sq[nt][u][1], s[nt][3]));
+          float d[4] = {start[nt][u][0], start[nt][u][1], start[nt][u][0], start[nt][u][1]};
+          mma_f16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
+          mma_f16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
+          s[nt][0] = fmaf(sa, d[0], s[nt][0]);
+          s[nt][1] = fmaf(sa, d[1], s[nt][1]);
+          s[nt][2] = fmaf(sb, d[2], s[nt][2]);
+          s[nt][3] = fmaf(sb, d[3], s[nt][3]);
         }
       }
     }
-    const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
-    bool grew = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int e = x & 1, pos = key0 + r0 + (x & 2);
-        s[nt][x] = whole || (pos <= hi[nt][e] && pos >= lo[nt][e]) ? s[nt][x] * scale_log2 : -INFINITY;
-        grew = grew || s[nt][x] > m[nt][e];
-      }
+      for (int x = 0; x < 4; ++x) s[nt][x] *= cs[nt][x & 1];
+    // Rows of the tile outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
+    // values are taken as zero, so that nothing which is not finite meets a probability of zero.
+    unsigned keep01 = 0xffffffffu, keep23 = 0xffffffffu;
+    if (!(key0 >= all_lo && key0 + 15 <= all_hi)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = nt * 8 + 2 * t + (x & 1), pos = key0 + r0 + (x & 2);
+          const int hi = r < rows ? base_pos + (row0 + r) / G : -1;
+          if (pos > hi || (window > 0 && pos <= hi - window)) s[nt][x] = -INFINITY;
+        }
+      const int p = key0 + 4 * t;
+      auto seen = [&](int x) { return x <= last && (window <= 0 || x > all_hi - window); };
+      keep01 = (seen(p) ? 0x0000ffffu : 0u) | (seen(p + 1) ? 0xffff0000u : 0u);
+      keep23 = (seen(p + 2) ? 0x0000ffffu : 0u) | (seen(p + 3) ? 0xffff0000u : 0u);
+    }
+    bool grew = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) grew = grew || fmaxf(s[nt][0], s[nt][2]) > m[nt][0] || fmaxf(s[nt][1], s[nt][3]) > m[nt][1];
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -740,7 +818,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
           float M = fmaxf(fmaxf(s[nt][e], s[nt][2 + e]), m[nt][e]);
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-          const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - M);
+          const float f = ex2(m[nt][e] - M);
           m[nt][e] = M;
           l[nt][e] *= f;
 #pragma unroll
@@ -754,20 +832,11 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        s[nt][x] = s[nt][x] == -INFINITY ? 0.f : ex2(s[nt][x] - m[nt][x & 1]);
+        s[nt][x] = ex2(s[nt][x] - m[nt][x & 1]);
         l[nt][x & 1] += s[nt][x];
       }
       pf[nt][0] = transposed(pack(s[nt][0], s[nt][1]));
       pf[nt][1] = transposed(pack(s[nt][2], s[nt][3]));
-    }
-    // Rows of the tile outside what any query of this tile sees may hold anything (a stale row, a page's end): their
-    // pairs are taken as zero, so that nothing which is not finite meets a probability of zero.
-    unsigned keep01 = 0xffffffffu, keep23 = 0xffffffffu;
-    if (!whole) {
-      const int p = key0 + 4 * t;
-      auto seen = [&](int x) { return x <= last && x >= c.lo16 * 16 && (window <= 0 || x > all_hi - window); };
-      keep01 = (seen(p) ? 0x0000ffffu : 0u) | (seen(p + 1) ? 0xffff0000u : 0u);
-      keep23 = (seen(p + 2) ? 0x0000ffffu : 0u) | (seen(p + 3) ? 0xffff0000u : 0u);
     }
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
@@ -787,7 +856,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       }
     }
   }
-  cp_async_wait<0>();
+  if (gave_up && lane == 0 && status) *status = GAVE_UP;
   __syncthreads();               // the rings become the merge area: [warp][row][HD channels, maximum, sum]
   constexpr int MLD = HD + 4;
   float* merge = reinterpret_cast<float*>(smem);
@@ -809,14 +878,14 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)items * COLS * HD) + (size_t)blockIdx.x * COLS;
   for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
     const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
-    float M = -INFINITY, den = 0.f;
+    float M = NOTHING, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M = fmaxf(M, merge[(size_t)(w * COLS + r) * MLD + HD]);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float* src = merge + (size_t)(w * COLS + r) * MLD;
-      const float f = factor(src[HD], M);
+      const float f = exp2f(src[HD] - M);
       const float4 v = *reinterpret_cast<const float4*>(src + ch);
       den += f * src[HD + 1];
       acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
@@ -877,7 +946,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
   co_pdl_wait();
   const float2* ml = reinterpret_cast<const float2*>(scratch + (size_t)items * cols * HD) + (size_t)first * cols + col;
   const float* acc_in = scratch + ((size_t)first * cols + col) * HD;
-  float M = -INFINITY;
+  float M = NOTHING;
   for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[(size_t)p * cols].x);
   M = co_warp_max(M);
   float den = 0.f;
@@ -888,7 +957,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
     float f = 0.f;
     if (lane < 8 && p0 + lane < parts) {
       const float2 x = ml[(size_t)(p0 + lane) * cols];
-      f = factor(x.x, M);
+      f = exp2f(x.x - M);
       den += f * x.y;
     }
     float4 in[8][V];
@@ -932,13 +1001,19 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
   }
 }
 
-// Resident CTAs that an item count aims at.
-int items_target() { return 148 * 4; }
 int tiles_of(int max_rows) { return max_rows <= 8 || HD > 128 ? 1 : 2; }
+long long lists_of(int B, int nkv, int max_rows) {        // (request, kv head, row tile) at most
+  return (long long)B * nkv * ((max_rows + 8 * tiles_of(max_rows) - 1) / (8 * tiles_of(max_rows)));
+}
+// How many items are aimed at.  Cutting rounds up, once for each list, so at most target + lists items come out: with few
+// lists they fill the resident CTAs once, with many they are cut smaller, so that the last round costs little.
+int items_target(long long lists) {
+  const int slots = 148 * 4;
+  return lists * 8 <= slots ? slots - (int)lists : 4 * slots;
+}
 long long items_bound(int B, int nkv, int max_rows, int max_kv_len) {
-  const long long row_tiles = (max_rows + 8 * tiles_of(max_rows) - 1) / (8 * tiles_of(max_rows));
-  const long long most = (long long)B * nkv * row_tiles, units = ((long long)max_kv_len + 15) / UNIT + 1;
-  const long long by_length = most * units, by_target = items_target() + most;
+  const long long lists = lists_of(B, nkv, max_rows), units = ((long long)max_kv_len + 15) / UNIT + 1;
+  const long long by_length = lists * units, by_target = items_target(lists) + lists;
   return by_length < by_target ? by_length : by_target;
 }
 
@@ -953,7 +1028,7 @@ int launch_items(const void* q, long q_ld, void* out, long out_ld, const void* k
   }
   co_launch(kv4_items_kernel<NT>, dim3((unsigned)items), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
             (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-            window, scale_log2, max_rows, items_target(), scratch, items, status);
+            window, scale_log2, max_rows, items_target(lists_of(B, nkv, max_rows)), scratch, items, status);
   CO_CHECK_LAUNCH("kv4_items");
   return 0;
 }
@@ -1066,7 +1141,8 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
                                            window, scale_log2, max_rows, (int)items, scratch, status, stream);
   if (rc || max_kv_len + 15 <= UNIT) return rc;    // no request is longer than one unit: nothing to join
   co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, (int)items,
-            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows, items_target());
+            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows,
+            items_target(lists_of(B, nkv, max_rows)));
   CO_CHECK_LAUNCH("kv4_join");
   return 0;
 }

@@ -642,11 +642,11 @@ def describe_status(code: int) -> str:
     """What a non-zero device status word means."""
     if code in STATUS_MESSAGES:
         return STATUS_MESSAGES[code]
-    if 11 <= code <= 39:
+    if 11 <= code <= 40:
         return (f"a kernel gave up a bounded wait and left its output unfinished (code {code}: 11-14 tensor-core product: "
                 "producer, MMA issuer, epilogue, split of float32 operands; 12 and 13 also the matrix memory in chunks: MMA issuer, the "
                 "others; 19 self-test; 31-39 prompt attention: 31 producer, 32-36 MMA issuer, "
-                "37-39 softmax)")
+                "37-39 softmax; 40 attention over a 4-bit cache)")
     return f"device status {code}"
 
 

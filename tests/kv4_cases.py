@@ -105,11 +105,11 @@ def attend(q, k, v, first_pos, scale, window=None):
 def bound(out, mass, most, hd, keys, dtype, rounded_keys=False):
     """How far a kernel may be from ``attend``.  With A = sum of p |v| (``mass``): a probability and a value that enter a product in
     bfloat16 are each off by at most 2^-8 of themselves (A 2^-7 together), the output by 2^-8 of itself; a score summed in float32
-    from hd products is off by at most (hd + 8) 2^-23 of sum |q k| (twice the products' roundings, for sums that go through
-    128 + code: 16 times, the share by which that raises the terms), by 2^-8 of it more where the keys were rounded to bfloat16;
+    from hd products is off by at most (hd + 8) 2^-23 of sum |q k| (twice the products' roundings; sums that go through 1024 + code in
+    the place of a code, about 7.5 from a group's middle: 136 times, the share by which that raises the terms), by 2^-8 of it more where the keys were rounded to bfloat16;
     errors up to d in the scores move a probability by a factor within exp(-2 d)..exp(2 d); exponentials and the sums over the keys are off by 2^-21 and
     keys 2^-23 of A."""
-    d = most * (hd + 8) * 2.0 ** -23 * (1 if dtype == torch.float32 else 16)
+    d = most * (hd + 8) * 2.0 ** -23 * (1 if dtype == torch.float32 else 136)
     if rounded_keys:
         d = d + most * 2.0 ** -8
     A = mass
