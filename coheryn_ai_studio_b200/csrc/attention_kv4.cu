@@ -514,22 +514,23 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 //  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
 //    of up to 8 heads wastes no product;
 //  * keys: code c enters the product as the float16 1024 + c (places 0 and 2 of a half word) or 64 + c (places 1 and 3): one
-//    lop3 for two codes, one shift for eight.  The accumulator starts at minus the sum of q times those constants, so that
-//    it ends as sum(q c), and the group's scale multiplies float32 sums; the minima's share, sum over the groups of
-//    m sum(q), is one product more, with sum(q) as three bfloat16 terms.  No key is rounded.  Queries enter as
+//    lop3 for two codes, one shift for eight.  The group's scale s multiplies float32 sums.  What the constants add, sum over
+//    the groups of s C with C = sum of q times 1024 or 64, and the minima's share, sum of m sum(q), are two products more
+//    over the groups in the place of the channels, with C and sum(q) as three bfloat16 terms each.  No key is rounded.  Queries enter as
 //    float16 divided by the power of two that brings the row's largest to 1..2: exact, but for elements under 2^-14
 //    of it, which are off by at most 2^-25 of it;
 //  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs);
 //  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
-//  * the running maximum moves (and the accumulators are scaled) only when a tile holds a larger score than the warp has
-//    seen in any row of it.
+//  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
+//    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
 // The rows' sums stay per lane and meet once at the end, as do the warps.  Every wait is bounded: on expiry the
 // kernel records a code in `status` and winds down.
 // ------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int STAGES = 4;                // a power of two
 constexpr int GAVE_UP = 40;              // status: a bounded wait ran out
-constexpr float NOTHING = -3.0e38f;      // a running maximum that no score has met
+constexpr float NOTHING = -3.0e38f;      // a reference that no score has met
+constexpr float SLACK = 8.f;
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
@@ -557,11 +558,17 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));   // ex2(-inf) = +0
   return y;
 }
+// (word & mask) | constant as one instruction: written out, since the two constants would otherwise make two of it.
+__device__ __forceinline__ unsigned masked(unsigned word, unsigned mask, unsigned constant) {
+  unsigned r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(word), "r"(mask), "r"(constant));
+  return r;
+}
 // Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair 1024 + c (j even) or 64 + c (j odd).
-__device__ __forceinline__ unsigned codes128(unsigned word, int j) { return ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ unsigned codes128(unsigned word, int j) { return masked(word >> (4 * j), 0x000f000fu, 0x43004300u); }
 __device__ __forceinline__ unsigned codes16(unsigned word, int j) {
   const unsigned w = j < 2 ? word : word >> 8;
-  return j & 1 ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u;
+  return j & 1 ? masked(w, 0x00f000f0u, 0x54005400u) : masked(w, 0x000f000fu, 0x64006400u);
 }
 __device__ __forceinline__ unsigned pack_f16(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
@@ -653,8 +660,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 
   // The queries as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
   unsigned qf[NT][NG][4];
-  float start[NT][NG][2];         // of the accumulators of rows 2 t, 2 t + 1
-  unsigned sums[NT][MG][2];       // sum(q) of row g, group 4 i + t, in three terms
+  unsigned sums[NT][MG][4];       // of row g, group 4 i + t: sum(q) in three terms, minus C in three terms
   float cs[NT][2];                // what the scores of rows 2 t, 2 t + 1 are multiplied by
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -678,7 +684,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     cs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t);
     cs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t + 4);
 #pragma unroll
-    for (int i = 0; i < MG; ++i) sums[nt][i][0] = sums[nt][i][1] = 0;
+    for (int i = 0; i < MG; ++i) sums[nt][i][0] = sums[nt][i][1] = sums[nt][i][2] = sums[nt][i][3] = 0;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
@@ -696,14 +702,14 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         even += __shfl_xor_sync(0xffffffffu, even, o);
         odd += __shfl_xor_sync(0xffffffffu, odd, o);
       }
-      const float first = -(1024.f * even + 64.f * odd);
-      start[nt][u][0] = __shfl_sync(0xffffffffu, first, 8 * t);
-      start[nt][u][1] = __shfl_sync(0xffffffffu, first, 8 * t + 4);
       if (t == (u & 3)) {
-        const float sum = even + odd;
-        const float a = __bfloat162float(__float2bfloat16_rn(sum)), b = __bfloat162float(__float2bfloat16_rn(sum - a));
-        sums[nt][u >> 2][0] = pack(a, b);
-        sums[nt][u >> 2][1] = pack(sum - a - b, 0.f);
+        const float both[2] = {even + odd, -(1024.f * even + 64.f * odd)};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float a = __bfloat162float(__float2bfloat16_rn(both[i])), b = __bfloat162float(__float2bfloat16_rn(both[i] - a));
+          sums[nt][u >> 2][2 * i] = pack(a, b);
+          sums[nt][u >> 2][2 * i + 1] = pack(both[i] - a - b, 0.f);
+        }
       }
     }
   }
@@ -764,9 +770,13 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       for (int x = 0; x < MG; ++x) {
         const int u = min(4 * x + t, NG - 1);
         const unsigned wa = pairs[r0 * NG + u], wb = pairs[(r0 + 2) * NG + u];
-        const unsigned a = __byte_perm(wa, wa, 0x3232), b = __byte_perm(wb, wb, 0x3232);
+        const unsigned ma = __byte_perm(wa, wa, 0x3232), mb = __byte_perm(wb, wb, 0x3232);
+        const unsigned sa = __byte_perm(wa, wa, 0x1010), sb = __byte_perm(wb, wb, 0x1010);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], a, b, a, b, sums[nt][x][0], sums[nt][x][1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_bf16(s[nt], ma, mb, ma, mb, sums[nt][x][0], sums[nt][x][1]);
+          mma_bf16(s[nt], sa, sb, sa, sb, sums[nt][x][2], sums[nt][x][3]);
+        }
       }
 #pragma unroll
       for (int u = 0; u < NG; ++u) {
@@ -776,7 +786,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         const float sa = lo_bf16(pa[u]), sb = lo_bf16(pb[u]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {start[nt][u][0], start[nt][u][1], start[nt][u][0], start[nt][u][1]};
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
           mma_f16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
           mma_f16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
           s[nt][0] = fmaf(sa, d[0], s[nt][0]);
@@ -790,9 +800,6 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[nt][x] *= cs[nt][x & 1];
-    // Rows of the tile outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
-    // values are taken as zero, so that nothing which is not finite meets a probability of zero.
-    unsigned keep01 = 0xffffffffu, keep23 = 0xffffffffu;
     if (!(key0 >= all_lo && key0 + 15 <= all_hi)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -802,14 +809,20 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
           const int hi = r < rows ? base_pos + (row0 + r) / G : -1;
           if (pos > hi || (window > 0 && pos <= hi - window)) s[nt][x] = -INFINITY;
         }
-      const int p = key0 + 4 * t;
-      auto seen = [&](int x) { return x <= last && (window <= 0 || x > all_hi - window); };
-      keep01 = (seen(p) ? 0x0000ffffu : 0u) | (seen(p + 1) ? 0xffff0000u : 0u);
-      keep23 = (seen(p + 2) ? 0x0000ffffu : 0u) | (seen(p + 3) ? 0xffff0000u : 0u);
+      // Rows of the tile outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
+      // values become zero, so that nothing which is not finite meets a probability of zero.
+      const int row = lane & 15, pos = key0 + row;
+      if (pos > last || (window > 0 && pos <= all_hi - window)) {
+        unsigned short* pairs = reinterpret_cast<unsigned short*>(ring + stage * 2 * TB + TB + CODES) + (row >> 2) * 8 + (row & 3) + (lane >> 4) * 4;
+#pragma unroll
+        for (int u = 0; u < NG; ++u) pairs[u * 32] = 0;
+      }
+      fence_proxy_async();        // the stage is written by a copy next
+      __syncwarp();
     }
     bool grew = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) grew = grew || fmaxf(s[nt][0], s[nt][2]) > m[nt][0] || fmaxf(s[nt][1], s[nt][3]) > m[nt][1];
+    for (int nt = 0; nt < NT; ++nt) grew = grew || fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + SLACK || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + SLACK;
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -842,7 +855,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     for (int u = 0; u < NG; ++u) {
       const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
       const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
-      const __nv_bfloat162 s01 = pair_of(sm.x & keep01), s23 = pair_of(sm.y & keep23), m01 = pair_of(sm.z & keep01), m23 = pair_of(sm.w & keep23);
+      const __nv_bfloat162 s01 = pair_of(sm.x), s23 = pair_of(sm.y), m01 = pair_of(sm.z), m23 = pair_of(sm.w);
       unsigned a[4], b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
