@@ -280,7 +280,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 // into as many items as it needs, from the lengths on the device: a captured launch serves every length.  The items of a
 // (request, kv head, row tile) are neighbours, and an item's number is its place in the scratch.
 // ------------------------------------------------------------------------------------
-constexpr int UNIT = 64;
+constexpr int UNIT = 128;
 
 struct Cut {                       // of one request
   int tok0, q_len, kv_len;
@@ -507,8 +507,8 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 }
 // ------------------------------------------------------------------------------------
 // Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
-// each with tiles of 16 positions of its own (tile i of the item goes to warp i mod 4) in a ring of its own that bulk
-// copies fill (two per tile, one thread), so that warps never wait for one another before the end.  Decoding is
+// each with pairs of tiles of its own (pair i of the item goes to warp i mod 4) in a ring of its own that bulk copies
+// fill (a tile of keys and one of values each, one thread), so that warps never wait for one another before the end.  Decoding is
 // bound by the cache's bytes, and with 5 bits a value nearly as much by the instructions that turn codes into operands,
 // those of the half-rate integer pipe first; hence:
 //  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
@@ -527,7 +527,8 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 // kernel records a code in `status` and winds down.
 // ------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
-constexpr int STAGES = 4;                // a power of two
+constexpr int STAGES = HD <= 64 ? 4 : 2;  // a power of two
+constexpr int PAIR = 4 * TB;             // bytes of a stage: keys and values of a tile, and of the next
 constexpr int GAVE_UP = 40;              // status: a bounded wait ran out
 constexpr float NOTHING = -3.0e38f;      // a reference that no score has met
 constexpr float SLACK = 8.f;
@@ -595,7 +596,7 @@ __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) 
 }
 template <int NT>
 constexpr size_t items_smem() {
-  const size_t ring = (size_t)WARPS * STAGES * 2 * TB, merge = (size_t)WARPS * 8 * NT * (HD + 4) * sizeof(float);
+  const size_t ring = (size_t)WARPS * STAGES * PAIR, merge = (size_t)WARPS * 8 * NT * (HD + 4) * sizeof(float);
   return ring > merge ? ring : merge;
 }
 
@@ -625,34 +626,37 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   const int* table = block_tables + (size_t)it.b * table_ld;
   const int u_first = (int)((long long)c.units * it.part / it.parts), u_end = (int)((long long)c.units * (it.part + 1) / it.parts);
   const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
-  const int tile0 = c.lo16 + u_first * (UNIT / 16) + warp;
-  const int n_tiles = tile_end > tile0 ? (tile_end - tile0 + WARPS - 1) / WARPS : 0;    // of this warp
+  const int tile0 = c.lo16 + u_first * (UNIT / 16) + 2 * warp;
+  const int n_pairs = tile_end > tile0 ? (tile_end - tile0 + 2 * WARPS - 1) / (2 * WARPS) : 0;    // of this warp
   const int base_pos = c.kv_len - c.q_len;
 
-  unsigned char* ring = smem + (size_t)warp * STAGES * 2 * TB;
-  // Where the warp's tiles lie in a cache, 32 tiles at a time, a lane each; -1: not in the pool.
+  unsigned char* ring = smem + (size_t)warp * STAGES * PAIR;
+  // Where the warp's tiles lie in a cache, 16 pairs at a time, a tile per lane; -1: not in the pool, or behind the item.
   long long place = -1;
   auto fetch_places = [&](int i0) {
-    const int tile = tile0 + (i0 + lane) * WARPS, per_page = page_size >> 4;
+    const int tile = tile0 + (i0 + (lane >> 1)) * 2 * WARPS + (lane & 1), per_page = page_size >> 4;
     place = -1;
-    if (i0 + lane < n_tiles) {
+    if (tile < tile_end) {
       const int blk = tile / per_page, page = blk < table_ld ? table[blk] : -1;
       if (page >= 0 && page < num_pages) place = (((long long)page * nkv + it.kvh) * per_page + (tile - blk * per_page)) * TB;
       else if (status) *status = BAD_INDEX;
     }
   };
-  unsigned known = 0;      // bit of a stage: its tile came from a page of the pool, so copies fill it
+  unsigned known = 0;      // bits 2 stage, 2 stage + 1: the tile came from a page of the pool, so copies fill it
   auto issue = [&](int i) {
-    if (i >= n_tiles) return;
-    if ((i & 31) == 0) fetch_places(i);
-    const long long at = __shfl_sync(0xffffffffu, place, i & 31);
+    if (i >= n_pairs) return;
+    if ((i & 15) == 0) fetch_places(i);
     const int stage = i % STAGES;
-    known = at < 0 ? known & ~(1u << stage) : known | 1u << stage;
-    if (at >= 0 && lane == 0) {
-      unsigned char* dst = ring + stage * 2 * TB;
-      mbar_expect_tx(&bars[warp][stage], 2 * TB);
-      bulk_load(dst, k_cache + at, TB, &bars[warp][stage]);
-      bulk_load(dst + TB, v_cache + at, TB, &bars[warp][stage]);
+    const unsigned there = (__ballot_sync(0xffffffffu, place >= 0) >> (2 * (i & 15))) & 3u;
+    known = (known & ~(3u << (2 * stage))) | there << (2 * stage);
+    // The lane that knows a tile's place copies it; the first of a pair's lanes that does announces the bytes of both.
+    const bool mine = (lane >> 1) == (i & 15) && place >= 0;
+    if (mine && (lane & 1) == (there == 2u)) mbar_expect_tx(&bars[warp][stage], there == 3u ? PAIR : PAIR / 2);
+    __syncwarp();
+    if (mine) {
+      unsigned char* dst = ring + stage * PAIR + (lane & 1) * 2 * TB;
+      bulk_load(dst, k_cache + place, TB, &bars[warp][stage]);
+      bulk_load(dst + TB, v_cache + place, TB, &bars[warp][stage]);
     }
   };
 #pragma unroll
@@ -736,28 +740,29 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   bool gave_up = false;
 
 #pragma unroll 1
-  for (int i = 0; i < n_tiles; ++i) {
+  for (int i = 0; i < n_pairs; ++i) {
     const int stage = i % STAGES;
-    const bool usable = (known >> stage) & 1;
-    if (usable) {
+    const unsigned there = (known >> (2 * stage)) & 3u;
+    if (there) {
       gave_up = !mbar_wait(&bars[warp][stage], (phases >> stage) & 1) || gave_up;
       phases ^= 1u << stage;
     }
-    __syncwarp();                               // all lanes are done with the stage of tile i - 1
+    // All lanes are done with the stage of pair i - 1.
     if (__any_sync(0xffffffffu, gave_up)) {     // copies that are still in flight end before the memory is used again
-      for (int j = i + 1; j < min(n_tiles, i + STAGES - 1); ++j)
-        if ((known >> (j % STAGES)) & 1) mbar_wait(&bars[warp][j % STAGES], (phases >> (j % STAGES)) & 1);
+      for (int j = i + 1; j < min(n_pairs, i + STAGES - 1); ++j)
+        if ((known >> (2 * (j % STAGES))) & 3u) mbar_wait(&bars[warp][j % STAGES], (phases >> (j % STAGES)) & 1);
       gave_up = true;
       break;
     }
     issue(i + STAGES - 1);
-    if (!usable) continue;
-    const unsigned char* kt = ring + stage * 2 * TB;
-    const unsigned char* vt = kt + TB;
-    const int key0 = (tile0 + i * WARPS) * 16;
+    if (!there) continue;
+    unsigned char* pair = ring + stage * PAIR;
+    const int key0 = (tile0 + i * 2 * WARPS) * 16;
 
-    float s[NT][4];
-    {
+    float s[2][NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* kt = pair + h * 2 * TB;
       unsigned ka[NG], kb[NG], pa[NG], pb[NG];
       load_words<NG>(reinterpret_cast<const unsigned*>(kt) + r0 * (4 * NG) + t * NG, ka);
       load_words<NG>(reinterpret_cast<const unsigned*>(kt) + (r0 + 2) * (4 * NG) + t * NG, kb);
@@ -765,7 +770,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       load_words<NG>(pairs + r0 * NG, pa);
       load_words<NG>(pairs + (r0 + 2) * NG, pb);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt) s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
 #pragma unroll
       for (int x = 0; x < MG; ++x) {
         const int u = min(4 * x + t, NG - 1);
@@ -774,8 +779,8 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         const unsigned sa = __byte_perm(wa, wa, 0x1010), sb = __byte_perm(wb, wb, 0x1010);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(s[nt], ma, mb, ma, mb, sums[nt][x][0], sums[nt][x][1]);
-          mma_bf16(s[nt], sa, sb, sa, sb, sums[nt][x][2], sums[nt][x][3]);
+          mma_bf16(s[h][nt], ma, mb, ma, mb, sums[nt][x][0], sums[nt][x][1]);
+          mma_bf16(s[h][nt], sa, sb, sa, sb, sums[nt][x][2], sums[nt][x][3]);
         }
       }
 #pragma unroll
@@ -789,46 +794,54 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
           float d[4] = {0.f, 0.f, 0.f, 0.f};
           mma_f16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
           mma_f16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
-          s[nt][0] = fmaf(sa, d[0], s[nt][0]);
-          s[nt][1] = fmaf(sa, d[1], s[nt][1]);
-          s[nt][2] = fmaf(sb, d[2], s[nt][2]);
-          s[nt][3] = fmaf(sb, d[3], s[nt][3]);
+          s[h][nt][0] = fmaf(sa, d[0], s[h][nt][0]);
+          s[h][nt][1] = fmaf(sa, d[1], s[h][nt][1]);
+          s[h][nt][2] = fmaf(sb, d[2], s[h][nt][2]);
+          s[h][nt][3] = fmaf(sb, d[3], s[h][nt][3]);
         }
       }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[nt][x] *= cs[nt][x & 1];
-    if (!(key0 >= all_lo && key0 + 15 <= all_hi)) {
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[h][nt][x] *= cs[nt][x & 1];
+    if (!(there == 3u && key0 >= all_lo && key0 + 31 <= all_hi)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int r = nt * 8 + 2 * t + (x & 1), pos = key0 + r0 + (x & 2);
-          const int hi = r < rows ? base_pos + (row0 + r) / G : -1;
-          if (pos > hi || (window > 0 && pos <= hi - window)) s[nt][x] = -INFINITY;
-        }
-      // Rows of the tile outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
-      // values become zero, so that nothing which is not finite meets a probability of zero.
-      const int row = lane & 15, pos = key0 + row;
-      if (pos > last || (window > 0 && pos <= all_hi - window)) {
-        unsigned short* pairs = reinterpret_cast<unsigned short*>(ring + stage * 2 * TB + TB + CODES) + (row >> 2) * 8 + (row & 3) + (lane >> 4) * 4;
+          const int r = nt * 8 + 2 * t + (x & 1), hi = r < rows ? base_pos + (row0 + r) / G : -1;
 #pragma unroll
-        for (int u = 0; u < NG; ++u) pairs[u * 32] = 0;
+          for (int h = 0; h < 2; ++h) {
+            const int pos = key0 + 16 * h + r0 + (x & 2);
+            if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) s[h][nt][x] = -INFINITY;
+          }
+        }
+      // Rows of the tiles outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
+      // values become zero, so that nothing which is not finite meets a probability of zero.
+      const int row = lane & 15, h = lane >> 4, pos = key0 + lane;
+      if (!((there >> h) & 1u) || pos > last || (window > 0 && pos <= all_hi - window)) {
+        unsigned short* pairs = reinterpret_cast<unsigned short*>(pair + h * 2 * TB + TB + CODES) + (row >> 2) * 8 + (row & 3);
+#pragma unroll
+        for (int u = 0; u < NG; ++u) pairs[u * 32] = pairs[u * 32 + 4] = 0;
       }
-      fence_proxy_async();        // the stage is written by a copy next
+      fence_proxy_async();        // the stage is written by copies next
       __syncwarp();
     }
     bool grew = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) grew = grew || fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + SLACK || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + SLACK;
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        grew = grew || fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e])) > m[nt][e] + SLACK;
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float M = fmaxf(fmaxf(s[nt][e], s[nt][2 + e]), m[nt][e]);
+          float M = fmaxf(fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e])), m[nt][e]);
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
           const float f = ex2(m[nt][e] - M);
@@ -840,34 +853,39 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
             for (int h = 0; h < 2; ++h) { o[u][h][nt][e] *= f; o[u][h][nt][2 + e] *= f; }
         }
     }
-    unsigned pf[NT][2];
+    unsigned pf[2][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        s[nt][x] = ex2(s[nt][x] - m[nt][x & 1]);
-        l[nt][x & 1] += s[nt][x];
-      }
-      pf[nt][0] = transposed(pack(s[nt][0], s[nt][1]));
-      pf[nt][1] = transposed(pack(s[nt][2], s[nt][3]));
-    }
-#pragma unroll
-    for (int u = 0; u < NG; ++u) {
-      const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
-      const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
-      const __nv_bfloat162 s01 = pair_of(sm.x), s23 = pair_of(sm.y), m01 = pair_of(sm.z), m23 = pair_of(sm.w);
-      unsigned a[4], b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
-        b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
-      }
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma_bf16(o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
-        mma_bf16(o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s[h][nt][x] = ex2(s[h][nt][x] - m[nt][x & 1]);
+          l[nt][x & 1] += s[h][nt][x];
+        }
+        pf[h][nt][0] = transposed(pack(s[h][nt][0], s[h][nt][1]));
+        pf[h][nt][1] = transposed(pack(s[h][nt][2], s[h][nt][3]));
       }
-    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < NG; ++u) {
+        const unsigned char* vt = pair + h * 2 * TB + TB;
+        const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
+        const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
+        const __nv_bfloat162 s01 = pair_of(sm.x), s23 = pair_of(sm.y), m01 = pair_of(sm.z), m23 = pair_of(sm.w);
+        unsigned a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
+          b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_bf16(o[u][0][nt], a[0], a[1], b[0], b[1], pf[h][nt][0], pf[h][nt][1]);
+          mma_bf16(o[u][1][nt], a[2], a[3], b[2], b[3], pf[h][nt][0], pf[h][nt][1]);
+        }
+      }
   }
   if (gave_up && lane == 0 && status) *status = GAVE_UP;
   __syncthreads();               // the rings become the merge area: [warp][row][HD channels, maximum, sum]
