@@ -19,6 +19,9 @@
 
 #include "tc_common.cuh"
 
+#ifndef KV4_MINB
+#define KV4_MINB 4
+#endif
 #ifndef CO_HEAD_DIM
 #define CO_HEAD_DIM 128
 #endif
@@ -275,17 +278,18 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 
 // ------------------------------------------------------------------------------------
 // How the keys of a step are cut.  The visible positions of a request (from the 16 that hold the first one on) are
-// counted in units of UNIT positions; a work item is a run of units of one (request, kv head, tile of query rows).  All
-// items have about the same number of units, total / target of them, so that a long context beside short ones is cut
-// into as many items as it needs, from the lengths on the device: a captured launch serves every length.  The items of a
-// (request, kv head, row tile) are neighbours, and an item's number is its place in the scratch.
+// counted in units of UNIT positions, of which every list (request, kv head, tile of query rows) has the same number.  All
+// units of the step, list after list, are cut into equal shares, one per CTA, from the lengths on the device: a long
+// context beside short ones keeps no CTA waiting, and a captured launch serves every length.  A share may end inside a
+// list and go on with the next; what a CTA has of a list that it does not hold whole goes to the scratch, at place
+// 2 * CTA for the list that its share begins in and 2 * CTA + 1 for the one that it begins inside the share.
 // ------------------------------------------------------------------------------------
 constexpr int UNIT = 128;
 
 struct Cut {                       // of one request
   int tok0, q_len, kv_len;
-  int lo16, units;                 // first tile of 16 positions, units from there on
-  int row_tiles;
+  int lo16, units;                 // first tile of 16 positions; units from there on, at least one if there are rows
+  int row_tiles;                   // 0: the request is not for this kernel
 };
 __device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b, int G, int rows_per_tile, int max_rows, int window) {
   Cut c;
@@ -295,38 +299,40 @@ __device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b
   const int rows = c.q_len * G;
   const int first = window > 0 ? max(0, c.kv_len - c.q_len - window + 1) : 0;
   c.lo16 = first >> 4;
-  c.units = max(0, (c.kv_len - c.lo16 * 16 + UNIT - 1) / UNIT);
   c.row_tiles = rows > 0 && rows <= max_rows ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
-  if (c.row_tiles == 0) c.units = 0;
+  c.units = c.row_tiles ? max(1, (c.kv_len - c.lo16 * 16 + UNIT - 1) / UNIT) : 0;
   return c;
 }
-struct Item {
-  int b, kvh, row_tile, part, parts, first;   // first: the number of part 0's item
+// All units of the step.  One warp; all lanes get the answer.
+__device__ __forceinline__ int all_units(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows, int window) {
+  int total = 0;
+  for (int b = threadIdx.x & 31; b < B; b += 32) {
+    const Cut c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
+    total += c.units * c.row_tiles * nkv;
+  }
+  return __reduce_add_sync(0xffffffffu, total);
+}
+// The shares: share i of `shares` is units [share_start(i), share_start(i + 1)).
+__device__ __forceinline__ int share_start(int i, int shares, int total) { return (int)((long long)total * i / shares); }
+// The share that holds unit x.
+__device__ __forceinline__ int share_of(int x, int shares, int total) { return (int)((((long long)x + 1) * shares - 1) / total); }
+
+struct Place {                     // a unit's request, and the request's first unit
+  int b, first;
   Cut cut;
 };
-// Units per item when about `target` items are wanted, and the item of number `index` (b = -1: there is none).
 // One warp; all lanes get the answer.
-__device__ __forceinline__ Item find_item(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows,
-                                          int window, int target, int index) {
+__device__ __forceinline__ Place find_unit(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows,
+                                           int window, int unit, int b_from, int first) {
   const int lane = threadIdx.x & 31;
-  long long total = 0;
-  for (int b = lane; b < B; b += 32) {
-    const Cut c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
-    total += (long long)c.units * c.row_tiles * nkv;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int per = (int)max(1LL, (total + target - 1) / target);
-  Item it;
-  it.b = -1;
-  int before = 0;
-  for (int b0 = 0; b0 < B && it.b < 0; b0 += 32) {
+  Place p;
+  p.b = -1;
+  int before = first;
+  for (int b0 = b_from; b0 < B && p.b < 0; b0 += 32) {
     const int b = b0 + lane;
     Cut c = {0, 0, 0, 0, 0, 0};
     if (b < B) c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
-    // A request with rows and no key has one item, which writes zeros.
-    const int parts = c.row_tiles ? max(1, (c.units + per - 1) / per) : 0;
-    const int mine = parts * c.row_tiles * nkv;
+    const int mine = c.units * c.row_tiles * nkv;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -334,27 +340,21 @@ __device__ __forceinline__ Item find_item(const int* cu_q, const int* kv_lens, i
       if (lane >= o) sum += up;
     }
     const int start = before + sum - mine;
-    const unsigned hit = __ballot_sync(0xffffffffu, index >= start && index < start + mine);
+    const unsigned hit = __ballot_sync(0xffffffffu, unit >= start && unit < start + mine);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int s = __shfl_sync(0xffffffffu, start, src);
-      it.b = b0 + src;
-      it.parts = __shfl_sync(0xffffffffu, parts, src);
-      it.cut.tok0 = __shfl_sync(0xffffffffu, c.tok0, src);
-      it.cut.q_len = __shfl_sync(0xffffffffu, c.q_len, src);
-      it.cut.kv_len = __shfl_sync(0xffffffffu, c.kv_len, src);
-      it.cut.lo16 = __shfl_sync(0xffffffffu, c.lo16, src);
-      it.cut.units = __shfl_sync(0xffffffffu, c.units, src);
-      it.cut.row_tiles = __shfl_sync(0xffffffffu, c.row_tiles, src);
-      const int in = index - s;
-      it.part = in % it.parts;
-      it.row_tile = in / it.parts % it.cut.row_tiles;
-      it.kvh = in / (it.parts * it.cut.row_tiles);
-      it.first = index - it.part;
+      p.b = b0 + src;
+      p.first = __shfl_sync(0xffffffffu, start, src);
+      p.cut.tok0 = __shfl_sync(0xffffffffu, c.tok0, src);
+      p.cut.q_len = __shfl_sync(0xffffffffu, c.q_len, src);
+      p.cut.kv_len = __shfl_sync(0xffffffffu, c.kv_len, src);
+      p.cut.lo16 = __shfl_sync(0xffffffffu, c.lo16, src);
+      p.cut.units = __shfl_sync(0xffffffffu, c.units, src);
+      p.cut.row_tiles = __shfl_sync(0xffffffffu, c.row_tiles, src);
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  return it;
+  return p;
 }
 
 // The merge of partial results (maximum, sum, accumulator) in ascending order; a maximum of -inf carries nothing.
@@ -507,8 +507,9 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 }
 // ------------------------------------------------------------------------------------
 // Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
-// each with pairs of tiles of its own (pair i of the item goes to warp i mod 4) in a ring of its own that bulk copies
-// fill (a tile of keys and one of values each, one thread), so that warps never wait for one another before the end.  Decoding is
+// each with pairs of tiles of its own (pair i of the item goes to warp i mod 4) in a ring of its own that it fills with
+// cp.async, so that warps never wait for one another before the end (bulk copies of whole tiles by one lane took more
+// instructions: their operands go through uniform registers).  Decoding is
 // bound by the cache's bytes, and with 5 bits a value nearly as much by the instructions that turn codes into operands,
 // those of the half-rate integer pipe first; hence:
 //  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
@@ -523,19 +524,25 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 //  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
 //  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
 //    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
-// The rows' sums stay per lane and meet once at the end, as do the warps.  Every wait is bounded: on expiry the
-// kernel records a code in `status` and winds down.
+// The rows' sums stay per lane and meet once at the end, as do the warps.
 // ------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int STAGES = HD <= 64 ? 4 : 2;  // a power of two
 constexpr int PAIR = 4 * TB;             // bytes of a stage: keys and values of a tile, and of the next
-constexpr int GAVE_UP = 40;              // status: a bounded wait ran out
 constexpr float NOTHING = -3.0e38f;      // a reference that no score has met
 constexpr float SLACK = 8.f;
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar)) : "memory");
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// A tile, by a warp: 16 bytes per lane and round; zeros when `bytes` is 0 (16: the copy).
+__device__ __forceinline__ void copy_tile(unsigned dst, const unsigned char* src, int lane, int bytes) {
+  constexpr int WHOLE = TB / 512, REST = TB % 512 / 16;
+#pragma unroll
+  for (int i = 0; i < WHOLE; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * i), "l"(src + 512 * i), "r"(bytes) : "memory");
+  if (REST && lane < REST)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * WHOLE), "l"(src + 512 * WHOLE), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
@@ -548,6 +555,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from nothing: an accumulator that starts at zero without a register set to it.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ unsigned transposed(unsigned v) {
   unsigned r;
@@ -601,30 +615,29 @@ constexpr size_t items_smem() {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * WARPS, NT == 1 && HD <= 128 ? 4 : 1)
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 && HD <= 128 ? KV4_MINB : 1)
 kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
                  const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
-                 float scale_log2, int max_rows, int target, float* __restrict__ scratch, int items, int* __restrict__ status) {
+                 float scale_log2, int max_rows, float* __restrict__ scratch, int* __restrict__ status) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ unsigned long long bars[WARPS][STAGES];
   constexpr int COLS = 8 * NT, MG = (NG + 3) / 4;      // MG: products for the minima
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[warp][i], 1);
-    fence_proxy_async();
-  }
-  __syncwarp();
   co_pdl_wait();
   co_pdl_launch_dependents();
   const int G = nh / nkv;
-  const Item it = find_item(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, target, blockIdx.x);
-  if (it.b < 0) return;
-  const Cut c = it.cut;
-  const int row0 = it.row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
-  const int* table = block_tables + (size_t)it.b * table_ld;
-  const int u_first = (int)((long long)c.units * it.part / it.parts), u_end = (int)((long long)c.units * (it.part + 1) / it.parts);
+  const int total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window), shares = min((int)gridDim.x, total);
+  if ((int)blockIdx.x >= shares) return;
+  int unit = share_start(blockIdx.x, shares, total);
+  const int unit_end = share_start(blockIdx.x + 1, shares, total);
+  Place at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
+  for (bool first_list = true;; first_list = false) {
+  if (at.b < 0) return;           // lengths that changed under the kernel
+  const Cut c = at.cut;
+  const int list = (unit - at.first) / c.units, u_first = unit - at.first - list * c.units, u_end = min(c.units, u_first + unit_end - unit);
+  const int row_tile = list % c.row_tiles, kvh = list / c.row_tiles;
+  const int row0 = row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
+  const int* table = block_tables + (size_t)at.b * table_ld;
   const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
   const int tile0 = c.lo16 + u_first * (UNIT / 16) + 2 * warp;
   const int n_pairs = tile_end > tile0 ? (tile_end - tile0 + 2 * WARPS - 1) / (2 * WARPS) : 0;    // of this warp
@@ -638,26 +651,30 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     place = -1;
     if (tile < tile_end) {
       const int blk = tile / per_page, page = blk < table_ld ? table[blk] : -1;
-      if (page >= 0 && page < num_pages) place = (((long long)page * nkv + it.kvh) * per_page + (tile - blk * per_page)) * TB;
+      if (page >= 0 && page < num_pages) place = (((long long)page * nkv + kvh) * per_page + (tile - blk * per_page)) * TB;
       else if (status) *status = BAD_INDEX;
     }
   };
-  unsigned known = 0;      // bits 2 stage, 2 stage + 1: the tile came from a page of the pool, so copies fill it
-  auto issue = [&](int i) {
-    if (i >= n_pairs) return;
-    if ((i & 15) == 0) fetch_places(i);
-    const int stage = i % STAGES;
-    const unsigned there = (__ballot_sync(0xffffffffu, place >= 0) >> (2 * (i & 15))) & 3u;
-    known = (known & ~(3u << (2 * stage))) | there << (2 * stage);
-    // The lane that knows a tile's place copies it; the first of a pair's lanes that does announces the bytes of both.
-    const bool mine = (lane >> 1) == (i & 15) && place >= 0;
-    if (mine && (lane & 1) == (there == 2u)) mbar_expect_tx(&bars[warp][stage], there == 3u ? PAIR : PAIR / 2);
-    __syncwarp();
-    if (mine) {
-      unsigned char* dst = ring + stage * PAIR + (lane & 1) * 2 * TB;
-      bulk_load(dst, k_cache + place, TB, &bars[warp][stage]);
-      bulk_load(dst + TB, v_cache + place, TB, &bars[warp][stage]);
+  unsigned known = 0;      // bits 2 stage, 2 stage + 1: the tile came from a page of the pool (zeros otherwise)
+  const unsigned ring_lane = smem_u32(ring) + lane * 16;
+  const unsigned char *k_lane = k_cache + lane * 16, *v_lane = v_cache + lane * 16;
+  auto issue = [&](int i) {          // one group per call, with or without copies
+    if (i < n_pairs) {
+      if ((i & 15) == 0) fetch_places(i);
+      const int stage = i % STAGES;
+      unsigned there = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long from = __shfl_sync(0xffffffffu, place, 2 * (i & 15) + h);
+        const int bytes = from < 0 ? 0 : 16;
+        const unsigned dst = ring_lane + stage * PAIR + h * 2 * TB;
+        copy_tile(dst, from < 0 ? k_cache : k_lane + from, lane, bytes);
+        copy_tile(dst + TB, from < 0 ? v_cache : v_lane + from, lane, bytes);
+        there |= from < 0 ? 0u : 1u << h;
+      }
+      known = (known & ~(3u << (2 * stage))) | there << (2 * stage);
     }
+    cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
@@ -669,7 +686,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g, row = row0 + r;
-    const bf16* src = q + (size_t)(c.tok0 + row / G) * q_ld + (size_t)(it.kvh * G + row % G) * HD;
+    const bf16* src = q + (size_t)(c.tok0 + row / G) * q_ld + (size_t)(kvh * G + row % G) * HD;
     uint4 v[NG];
     float most = 0.f;
 #pragma unroll
@@ -736,24 +753,13 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   }
   const int r0 = 4 * (g >> 1) + (g & 1);        // this lane's rows of a tile in the first product: r0 and r0 + 2
   const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
-  unsigned phases = 0;
-  bool gave_up = false;
 
 #pragma unroll 1
   for (int i = 0; i < n_pairs; ++i) {
     const int stage = i % STAGES;
     const unsigned there = (known >> (2 * stage)) & 3u;
-    if (there) {
-      gave_up = !mbar_wait(&bars[warp][stage], (phases >> stage) & 1) || gave_up;
-      phases ^= 1u << stage;
-    }
-    // All lanes are done with the stage of pair i - 1.
-    if (__any_sync(0xffffffffu, gave_up)) {     // copies that are still in flight end before the memory is used again
-      for (int j = i + 1; j < min(n_pairs, i + STAGES - 1); ++j)
-        if ((known >> (2 * (j % STAGES))) & 3u) mbar_wait(&bars[warp][j % STAGES], (phases >> (j % STAGES)) & 1);
-      gave_up = true;
-      break;
-    }
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();                               // landed for all lanes; all are done with the stage of pair i - 1
     issue(i + STAGES - 1);
     if (!there) continue;
     unsigned char* pair = ring + stage * PAIR;
@@ -791,8 +797,8 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         const float sa = lo_bf16(pa[u]), sb = lo_bf16(pb[u]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
+          float d[4];
+          mma_f16_first(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
           mma_f16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
           s[h][nt][0] = fmaf(sa, d[0], s[h][nt][0]);
           s[h][nt][1] = fmaf(sa, d[1], s[h][nt][1]);
@@ -801,12 +807,13 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         }
       }
     }
+    float y[2][NT][4];            // exponents: scores (times log2 e) from the row's reference
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[h][nt][x] *= cs[nt][x & 1];
+        for (int x = 0; x < 4; ++x) y[h][nt][x] = fmaf(s[h][nt][x], cs[nt][x & 1], -m[nt][x & 1]);
     if (!(there == 3u && key0 >= all_lo && key0 + 31 <= all_hi)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -816,7 +823,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pos = key0 + 16 * h + r0 + (x & 2);
-            if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) s[h][nt][x] = -INFINITY;
+            if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) y[h][nt][x] = -INFINITY;
           }
         }
       // Rows of the tiles outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
@@ -827,26 +834,32 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 #pragma unroll
         for (int u = 0; u < NG; ++u) pairs[u * 32] = pairs[u * 32 + 4] = 0;
       }
-      fence_proxy_async();        // the stage is written by copies next
       __syncwarp();
     }
     bool grew = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        grew = grew || fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e])) > m[nt][e] + SLACK;
+      for (int x = 0; x < 4; ++x) grew = grew || fmaxf(y[0][nt][x], y[1][nt][x]) > SLACK;
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float M = fmaxf(fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e])), m[nt][e]);
+          float M = m[nt][e];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = e; x < 4; x += 2) M = y[h][nt][x] == -INFINITY ? M : fmaxf(M, s[h][nt][x] * cs[nt][e]);
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
           const float f = ex2(m[nt][e] - M);
           m[nt][e] = M;
           l[nt][e] *= f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = e; x < 4; x += 2) y[h][nt][x] = y[h][nt][x] == -INFINITY ? -INFINITY : fmaf(s[h][nt][x], cs[nt][e], -M);
 #pragma unroll
           for (int u = 0; u < NG; ++u)
 #pragma unroll
@@ -860,7 +873,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          s[h][nt][x] = ex2(s[h][nt][x] - m[nt][x & 1]);
+          s[h][nt][x] = ex2(y[h][nt][x]);
           l[nt][x & 1] += s[h][nt][x];
         }
         pf[h][nt][0] = transposed(pack(s[h][nt][0], s[h][nt][1]));
@@ -887,7 +900,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         }
       }
   }
-  if (gave_up && lane == 0 && status) *status = GAVE_UP;
+  cp_async_wait<0>();
   __syncthreads();               // the rings become the merge area: [warp][row][HD channels, maximum, sum]
   constexpr int MLD = HD + 4;
   float* merge = reinterpret_cast<float*>(smem);
@@ -905,8 +918,10 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         *reinterpret_cast<float4*>(dst + u * 32 + g * 4) = make_float4(o[u][0][nt][e], o[u][0][nt][2 + e], o[u][1][nt][e], o[u][1][nt][2 + e]);
     }
   __syncthreads();
-  float* acc_out = scratch + (size_t)blockIdx.x * COLS * HD;
-  float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)items * COLS * HD) + (size_t)blockIdx.x * COLS;
+  const int slot = 2 * blockIdx.x + (first_list ? 0 : 1);
+  float* acc_out = scratch + (size_t)slot * COLS * HD;
+  float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)2 * gridDim.x * COLS * HD) + (size_t)slot * COLS;
+  const bool whole_list = u_first == 0 && u_end == c.units;
   for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
     const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
     float M = NOTHING, den = 0.f;
@@ -921,64 +936,66 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       den += f * src[HD + 1];
       acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
     }
-    if (it.parts == 1) {
+    if (whole_list) {
       const float inv = den == 0.f ? 0.f : 1.f / den;
       const int row = row0 + r;
-      bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(it.kvh * G + row % G) * HD + ch;
+      bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD + ch;
       store4<bf16>(dst, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     } else {
       *reinterpret_cast<float4*>(acc_out + (size_t)r * HD + ch) = acc;
       if (ch == 0) ml_out[r] = make_float2(M, den);
     }
   }
+  unit += u_end - u_first;
+  if (unit >= unit_end) return;
+  __syncthreads();               // the merge area becomes the rings again
+  if (unit - at.first >= c.units * c.row_tiles * nkv)
+    at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, at.b + 1, unit);
+  }
 }
 
-// Joins the items of a row: one CTA per (row of a request's kv head, kv head, request), its warps side by side over the
-// parts, four channels per lane, and the warps' sums in order at the end.
+// Joins the parts of a list's row: one CTA per (row of a request's kv head, kv head, request), its warps side by side over
+// the parts, four channels per lane, and the warps' sums in order at the end.
 constexpr int CW = 4;
 __global__ void __launch_bounds__(32 * CW)
-kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q,
-                const int* __restrict__ kv_lens, int B, int nh, int nkv, int cols, int window, int max_rows, int target) {
+kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q,
+                const int* __restrict__ kv_lens, int B, int nh, int nkv, int cols, int window, int max_rows) {
   constexpr int V = (HD + 127) / 128;
   __shared__ float part[CW][HD];
-  __shared__ float2 part_ml[CW];
-  __shared__ int found[2];
+  __shared__ float part_den[CW];
+  __shared__ int found[3];
   co_pdl_launch_dependents();
   const int r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = nh / nkv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Safe ahead of the wait: the items' kernel starts this one only after its own wait for whatever made the lengths.
+  // Safe ahead of the wait: the kernel before starts this one only after its own wait for whatever made the lengths.
   const Cut c = cut_of(cu_q, kv_lens, b, G, cols, max_rows, window);
   if (c.row_tiles == 0 || r >= c.q_len * G) return;
   if (warp == 0) {
-    long long total = 0;
-    for (int x = lane; x < B; x += 32) {
-      const Cut d = cut_of(cu_q, kv_lens, x, G, cols, max_rows, window);
-      total += (long long)d.units * d.row_tiles * nkv;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int per = (int)max(1LL, (total + target - 1) / target);
+    const int total = all_units(cu_q, kv_lens, B, nkv, G, cols, max_rows, window), shares = min(ctas, total);
     int before = 0;
     for (int x = lane; x < b; x += 32) {
       const Cut d = cut_of(cu_q, kv_lens, x, G, cols, max_rows, window);
-      before += d.row_tiles ? max(1, (d.units + per - 1) / per) * d.row_tiles * nkv : 0;
+      before += d.units * d.row_tiles * nkv;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    const int parts = max(1, (c.units + per - 1) / per);
+    const int first = __reduce_add_sync(0xffffffffu, before) + (kvh * c.row_tiles + r / cols) * c.units;
     if (lane == 0) {
-      found[0] = parts;
-      found[1] = before + (kvh * c.row_tiles + r / cols) * parts;
+      const int cta = share_of(first, shares, total);
+      found[0] = cta;
+      found[1] = share_of(first + c.units - 1, shares, total) - cta + 1;
+      found[2] = share_start(cta, shares, total) == first ? 0 : 1;
     }
   }
   __syncthreads();
-  const int parts = found[0], first = found[1], col = r % cols;
+  const int parts = found[1], col = r % cols;
   if (parts == 1) return;
+  // Part 0 is at place 2 cta or 2 cta + 1, part p at 2 (cta + p).
+  const int cta = found[0], odd = found[2];
+  const float2* ml = reinterpret_cast<const float2*>(scratch + (size_t)2 * ctas * cols * HD) + (size_t)2 * cta * cols + col;
+  const float* acc_in = scratch + ((size_t)2 * cta * cols + col) * HD;
+  auto place = [&](int p) { return (size_t)(2 * p + (p == 0 ? odd : 0)) * cols; };
   co_pdl_wait();
-  const float2* ml = reinterpret_cast<const float2*>(scratch + (size_t)items * cols * HD) + (size_t)first * cols + col;
-  const float* acc_in = scratch + ((size_t)first * cols + col) * HD;
   float M = NOTHING;
-  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[(size_t)p * cols].x);
+  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[place(p)].x);
   M = co_warp_max(M);
   float den = 0.f;
   float4 acc[V];
@@ -987,7 +1004,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
   for (int p0 = warp * 8; p0 < parts; p0 += CW * 8) {
     float f = 0.f;
     if (lane < 8 && p0 + lane < parts) {
-      const float2 x = ml[(size_t)(p0 + lane) * cols];
+      const float2 x = ml[place(p0 + lane)];
       f = exp2f(x.x - M);
       den += f * x.y;
     }
@@ -997,8 +1014,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int ch = v * 128 + lane * 4;
-        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(acc_in + (size_t)(p0 + p) * cols * HD + ch)
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(acc_in + place(p0 + p) * HD + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
@@ -1015,7 +1031,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
     const int ch = v * 128 + lane * 4;
     if (ch < HD) *reinterpret_cast<float4*>(&part[warp][ch]) = acc[v];
   }
-  if (lane == 0) part_ml[warp] = make_float2(M, den);
+  if (lane == 0) part_den[warp] = den;
   __syncthreads();
   const int ch = threadIdx.x * 4;
   if (ch < HD) {
@@ -1025,7 +1041,7 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
     for (int w = 0; w < CW; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(&part[w][ch]);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-      d += part_ml[w].y;
+      d += part_den[w];
     }
     const float inv = d == 0.f ? 0.f : 1.f / d;
     store4<bf16>(out + (size_t)(c.tok0 + r / G) * out_ld + (size_t)(kvh * G + r % G) * HD + ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
@@ -1033,33 +1049,26 @@ kv4_join_kernel(const float* __restrict__ scratch, int items, bf16* __restrict__
 }
 
 int tiles_of(int max_rows) { return max_rows <= 8 || HD > 128 ? 1 : 2; }
-long long lists_of(int B, int nkv, int max_rows) {        // (request, kv head, row tile) at most
-  return (long long)B * nkv * ((max_rows + 8 * tiles_of(max_rows) - 1) / (8 * tiles_of(max_rows)));
-}
-// How many items are aimed at.  Cutting rounds up, once for each list, so at most target + lists items come out: with few
-// lists they fill the resident CTAs once, with many they are cut smaller, so that the last round costs little.
-int items_target(long long lists) {
-  const int slots = 148 * 4;
-  return lists * 8 <= slots ? slots - (int)lists : 4 * slots;
-}
-long long items_bound(int B, int nkv, int max_rows, int max_kv_len) {
-  const long long lists = lists_of(B, nkv, max_rows), units = ((long long)max_kv_len + 15) / UNIT + 1;
-  const long long by_length = lists * units, by_target = items_target(lists) + lists;
-  return by_length < by_target ? by_length : by_target;
+// CTAs that cut the step's units: those that are resident at a time, or one per unit when there are fewer.
+int ctas_of(int B, int nkv, int max_rows, int max_kv_len) {
+  const int nt = tiles_of(max_rows);
+  static int slots = getenv("KV4_SLOTS") ? atoi(getenv("KV4_SLOTS")) : 148 * 4;
+  const long long lists = (long long)B * nkv * ((max_rows + 8 * nt - 1) / (8 * nt)), units = lists * (((long long)max_kv_len + 15) / UNIT + 1);
+  return (int)(units < slots ? units : slots);
 }
 
 template <int NT>
 int launch_items(const void* q, long q_ld, void* out, long out_ld, const void* k_cache, const void* v_cache, int num_pages, const int* table,
                  int table_ld, const int* cu_q, const int* kv_lens, int B, int nh, int nkv, int page_size, int window, float scale_log2,
-                 int max_rows, int items, float* scratch, int* status, cudaStream_t stream) {
+                 int max_rows, int ctas, float* scratch, int* status, cudaStream_t stream) {
   constexpr size_t SMEM = items_smem<NT>();
   if (SMEM > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kv4_items_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
     if (e != cudaSuccess) CO_FAIL("kv4_attention: %zu bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
   }
-  co_launch(kv4_items_kernel<NT>, dim3((unsigned)items), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
+  co_launch(kv4_items_kernel<NT>, dim3((unsigned)ctas), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
             (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-            window, scale_log2, max_rows, items_target(lists_of(B, nkv, max_rows)), scratch, items, status);
+            window, scale_log2, max_rows, scratch, status);
   CO_CHECK_LAUNCH("kv4_items");
   return 0;
 }
@@ -1145,7 +1154,7 @@ CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, 
 
 // Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests that it takes.
 CO_EXPORT long coheryn_kv4_scratch_floats(int B, int nkv, int max_rows, int max_kv_len) {
-  return (long)(items_bound(B, nkv, max_rows, max_kv_len) * 8 * tiles_of(max_rows) * (HD + 2));
+  return 2L * ctas_of(B, nkv, max_rows, max_kv_len) * 8 * tiles_of(max_rows) * (HD + 2);
 }
 
 // Attention of the requests with at most `max_rows` query rows per kv head, in bfloat16: q [T, nh * HD] of stride q_ld, out likewise;
@@ -1161,19 +1170,19 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
     CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
   if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
   const int nt = tiles_of(max_rows);
-  const long long items = items_bound(B, nkv, max_rows, max_kv_len);
-  if (items > 0x7fffffffLL) CO_FAIL("kv4_attention: %d requests of %d kv heads", B, nkv);
+  const int ctas = ctas_of(B, nkv, max_rows, max_kv_len);
+  if ((long long)B * nkv * ((max_rows + 7) / 8) * ((max_kv_len + 15LL) / UNIT + 1) > 0x7fffffffLL)
+    CO_FAIL("kv4_attention: %d requests of %d positions and %d kv heads", B, max_kv_len, nkv);
   if (scratch_floats < coheryn_kv4_scratch_floats(B, nkv, max_rows, max_kv_len) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_attention: the scratch is too small or not 16-byte aligned");
   const float scale_log2 = scale * 1.4426950408889634f;
   const int rc = nt == 1 ? launch_items<1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-                                           window, scale_log2, max_rows, (int)items, scratch, status, stream)
+                                           window, scale_log2, max_rows, ctas, scratch, status, stream)
                          : launch_items<HD <= 128 ? 2 : 1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-                                           window, scale_log2, max_rows, (int)items, scratch, status, stream);
-  if (rc || max_kv_len + 15 <= UNIT) return rc;    // no request is longer than one unit: nothing to join
-  co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, (int)items,
-            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows,
-            items_target(lists_of(B, nkv, max_rows)));
+                                           window, scale_log2, max_rows, ctas, scratch, status, stream);
+  if (rc || max_kv_len + 15 <= UNIT) return rc;    // no list is longer than one unit: nothing to join
+  co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, ctas,
+            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows);
   CO_CHECK_LAUNCH("kv4_join");
   return 0;
 }
