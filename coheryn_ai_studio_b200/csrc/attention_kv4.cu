@@ -19,9 +19,6 @@
 
 #include "tc_common.cuh"
 
-#ifndef KV4_MINB
-#define KV4_MINB 4
-#endif
 #ifndef CO_HEAD_DIM
 #define CO_HEAD_DIM 128
 #endif
@@ -282,7 +279,8 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 // units of the step, list after list, are cut into equal shares, one per CTA, from the lengths on the device: a long
 // context beside short ones keeps no CTA waiting, and a captured launch serves every length.  A share may end inside a
 // list and go on with the next; what a CTA has of a list that it does not hold whole goes to the scratch, at place
-// 2 * CTA for the list that its share begins in and 2 * CTA + 1 for the one that it begins inside the share.
+// 2 * CTA for the list that its share begins in and 2 * CTA + 1 for the one that it begins inside the share.  Whoever has a
+// list's first unit notes its number of parts and the place of the first for the kernel that joins them.
 // ------------------------------------------------------------------------------------
 constexpr int UNIT = 128;
 
@@ -514,21 +512,25 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 // those of the half-rate integer pipe first; hence:
 //  * positions are the M side of both products and the 8 NT query rows (token, head of the group) the N side, so a group
 //    of up to 8 heads wastes no product;
-//  * keys: code c enters the product as the float16 1024 + c (places 0 and 2 of a half word) or 64 + c (places 1 and 3): one
-//    lop3 for two codes, one shift for eight.  The group's scale s multiplies float32 sums.  What the constants add, sum over
-//    the groups of s C with C = sum of q times 1024 or 64, and the minima's share, sum of m sum(q), are two products more
-//    over the groups in the place of the channels, with C and sum(q) as three bfloat16 terms each.  No key is rounded.  Queries enter as
-//    float16 divided by the power of two that brings the row's largest to 1..2: exact, but for elements under 2^-14
-//    of it, which are off by at most 2^-25 of it;
-//  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs);
+//  * keys: the bits of code c, masked out of a half word, are the float16 c 2^-24 (a subnormal, which the tensor cores take
+//    as it is) or 16 c 2^-24, so two codes cost one logical operation and eight one shift; the queries of the
+//    odd channels are divided by 16.  The group's scale multiplies float32 sums, and the minima's share, sum over the groups
+//    of m sum(q), is one product more over the groups in the place of the channels, with sum(q) as three bfloat16 terms.
+//    No key is rounded.  Queries enter as float16 times the power of two that brings the row's largest to 2^14..2^15:
+//    exact, but for elements under 2^-24 of it;
+//  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs).  The scale
+//    put on the probability instead takes fewer instructions but rounds p s, whose error meets s c and not s c + m;
 //  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
 //  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
 //    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
+//  * the values' product of a pair and the scores of the next stand in one run of code without a branch, so that a warp
+//    has work of both kinds to issue.
 // The rows' sums stay per lane and meet once at the end, as do the warps.
 // ------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
-constexpr int STAGES = HD <= 64 ? 4 : 2;  // a power of two
-constexpr int PAIR = 4 * TB;             // bytes of a stage: keys and values of a tile, and of the next
+constexpr int K_STAGES = 2, V_STAGES = 3;      // pairs of key tiles and of value tiles in a warp's ring: values are used one pair later
+constexpr int PAIR = 2 * TB;
+constexpr int RING = (K_STAGES + V_STAGES) * PAIR;
 constexpr float NOTHING = -3.0e38f;      // a reference that no score has met
 constexpr float SLACK = 8.f;
 
@@ -545,27 +547,27 @@ __device__ __forceinline__ void copy_tile(unsigned dst, const unsigned char* src
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * WHOLE), "l"(src + 512 * WHOLE), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // The same from nothing: an accumulator that starts at zero without a register set to it.
 __device__ __forceinline__ void mma_f16_first(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ unsigned transposed(unsigned v) {
   unsigned r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -579,12 +581,9 @@ __device__ __forceinline__ unsigned masked(unsigned word, unsigned mask, unsigne
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(word), "r"(mask), "r"(constant));
   return r;
 }
-// Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair 1024 + c (j even) or 64 + c (j odd).
+// Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair c 2^-24 (j even) or 16 c 2^-24 (j odd).
 __device__ __forceinline__ unsigned codes128(unsigned word, int j) { return masked(word >> (4 * j), 0x000f000fu, 0x43004300u); }
-__device__ __forceinline__ unsigned codes16(unsigned word, int j) {
-  const unsigned w = j < 2 ? word : word >> 8;
-  return j & 1 ? masked(w, 0x00f000f0u, 0x54005400u) : masked(w, 0x000f000fu, 0x64006400u);
-}
+__device__ __forceinline__ unsigned codes16(unsigned word, int j) { return (j < 2 ? word : word >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ unsigned pack_f16(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const unsigned*>(&v);
@@ -608,85 +607,35 @@ __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) 
     for (int i = 0; i < N; ++i) w[i] = p[i];
   }
 }
+constexpr int MLD = HD + 4;              // a row of the warps' meeting: HD channels, reference, sum
 template <int NT>
 constexpr size_t items_smem() {
-  const size_t ring = (size_t)WARPS * STAGES * PAIR, merge = (size_t)WARPS * 8 * NT * (HD + 4) * sizeof(float);
+  const size_t ring = (size_t)WARPS * RING, merge = (size_t)WARPS * 8 * NT * MLD * sizeof(float);
   return ring > merge ? ring : merge;
 }
 
+// The query rows of a tile as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
+constexpr int MG = (NG + 3) / 4;         // products for the minima
 template <int NT>
-__global__ void __launch_bounds__(32 * WARPS, NT == 1 && HD <= 128 ? KV4_MINB : 1)
-kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
-                 const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
-                 const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
-                 float scale_log2, int max_rows, float* __restrict__ scratch, int* __restrict__ status) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  constexpr int COLS = 8 * NT, MG = (NG + 3) / 4;      // MG: products for the minima
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  co_pdl_wait();
-  co_pdl_launch_dependents();
-  const int G = nh / nkv;
-  const int total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window), shares = min((int)gridDim.x, total);
-  if ((int)blockIdx.x >= shares) return;
-  int unit = share_start(blockIdx.x, shares, total);
-  const int unit_end = share_start(blockIdx.x + 1, shares, total);
-  Place at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
-  for (bool first_list = true;; first_list = false) {
-  if (at.b < 0) return;           // lengths that changed under the kernel
-  const Cut c = at.cut;
-  const int list = (unit - at.first) / c.units, u_first = unit - at.first - list * c.units, u_end = min(c.units, u_first + unit_end - unit);
-  const int row_tile = list % c.row_tiles, kvh = list / c.row_tiles;
-  const int row0 = row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
-  const int* table = block_tables + (size_t)at.b * table_ld;
-  const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
-  const int tile0 = c.lo16 + u_first * (UNIT / 16) + 2 * warp;
-  const int n_pairs = tile_end > tile0 ? (tile_end - tile0 + 2 * WARPS - 1) / (2 * WARPS) : 0;    // of this warp
-  const int base_pos = c.kv_len - c.q_len;
+struct Queries {
+  unsigned f[NT][NG][4];
+  unsigned sums[NT][MG][2];              // sum(q) 2^-24 of row g, group 4 i + t, in three terms
+  float cs[NT][2];                       // what the scores of rows 2 t, 2 t + 1 are multiplied by
+};
+template <int NT>
+struct Sums {
+  float o[NG][2][NT][4];                 // channels 32 u + 4 g + 2 h, + 1 (first index of four: rows 2 t, 2 t + 1)
+  float m[NT][2], l[NT][2];              // reference and sum of rows 2 t, 2 t + 1
+};
 
-  unsigned char* ring = smem + (size_t)warp * STAGES * PAIR;
-  // Where the warp's tiles lie in a cache, 16 pairs at a time, a tile per lane; -1: not in the pool, or behind the item.
-  long long place = -1;
-  auto fetch_places = [&](int i0) {
-    const int tile = tile0 + (i0 + (lane >> 1)) * 2 * WARPS + (lane & 1), per_page = page_size >> 4;
-    place = -1;
-    if (tile < tile_end) {
-      const int blk = tile / per_page, page = blk < table_ld ? table[blk] : -1;
-      if (page >= 0 && page < num_pages) place = (((long long)page * nkv + kvh) * per_page + (tile - blk * per_page)) * TB;
-      else if (status) *status = BAD_INDEX;
-    }
-  };
-  unsigned known = 0;      // bits 2 stage, 2 stage + 1: the tile came from a page of the pool (zeros otherwise)
-  const unsigned ring_lane = smem_u32(ring) + lane * 16;
-  const unsigned char *k_lane = k_cache + lane * 16, *v_lane = v_cache + lane * 16;
-  auto issue = [&](int i) {          // one group per call, with or without copies
-    if (i < n_pairs) {
-      if ((i & 15) == 0) fetch_places(i);
-      const int stage = i % STAGES;
-      unsigned there = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long from = __shfl_sync(0xffffffffu, place, 2 * (i & 15) + h);
-        const int bytes = from < 0 ? 0 : 16;
-        const unsigned dst = ring_lane + stage * PAIR + h * 2 * TB;
-        copy_tile(dst, from < 0 ? k_cache : k_lane + from, lane, bytes);
-        copy_tile(dst + TB, from < 0 ? v_cache : v_lane + from, lane, bytes);
-        there |= from < 0 ? 0u : 1u << h;
-      }
-      known = (known & ~(3u << (2 * stage))) | there << (2 * stage);
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(i);
-
-  // The queries as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
-  unsigned qf[NT][NG][4];
-  unsigned sums[NT][MG][4];       // of row g, group 4 i + t: sum(q) in three terms, minus C in three terms
-  float cs[NT][2];                // what the scores of rows 2 t, 2 t + 1 are multiplied by
+template <int NT>
+__device__ __forceinline__ void load_queries(Queries<NT>& qr, const bf16* __restrict__ q, long q_ld, int tok0, int G, int kvh, int row0, int rows,
+                                             float scale_log2) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g, row = row0 + r;
-    const bf16* src = q + (size_t)(c.tok0 + row / G) * q_ld + (size_t)(kvh * G + row % G) * HD;
+    const bf16* src = q + (size_t)(tok0 + row / G) * q_ld + (size_t)(kvh * G + row % G) * HD;
     uint4 v[NG];
     float most = 0.f;
 #pragma unroll
@@ -699,323 +648,403 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // 2^-e with 2^e <= most < 2^(e + 1), e from -126 to 126
-    const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
-    const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
-    cs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t);
-    cs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t + 4);
+    // 2^(14 - e) with 2^e <= most < 2^(e + 1), and 2^24 times its inverse
+    const int e = min(max((int)(__float_as_uint(most) >> 23), 15), 240);
+    const float by = __uint_as_float((unsigned)(268 - e) << 23), back = __uint_as_float((unsigned)(e - 14) << 23) * 16777216.f;
+    qr.cs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t);
+    qr.cs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
-    for (int i = 0; i < MG; ++i) sums[nt][i][0] = sums[nt][i][1] = sums[nt][i][2] = sums[nt][i][3] = 0;
+    for (int i = 0; i < MG; ++i) qr.sums[nt][i][0] = qr.sums[nt][i][1] = 0;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      float x[8];
+      float x[8], sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __half2float(__float2half_rn(lo_bf16(w[i]) * down));
-        x[2 * i + 1] = __half2float(__float2half_rn(hi_bf16(w[i]) * down));
+        x[2 * i] = __half2float(__float2half_rn(lo_bf16(w[i]) * by));
+        x[2 * i + 1] = __half2float(__float2half_rn(hi_bf16(w[i]) * by * 0.0625f));
+        sum += fmaf(16.f, x[2 * i + 1], x[2 * i]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) qf[nt][u][j] = pack_f16(x[j], x[j + 4]);
-      float even = (x[0] + x[4]) + (x[2] + x[6]), odd = (x[1] + x[5]) + (x[3] + x[7]);
-#pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        even += __shfl_xor_sync(0xffffffffu, even, o);
-        odd += __shfl_xor_sync(0xffffffffu, odd, o);
-      }
+      for (int j = 0; j < 4; ++j) qr.f[nt][u][j] = pack_f16(x[j], x[j + 4]);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       if (t == (u & 3)) {
-        const float both[2] = {even + odd, -(1024.f * even + 64.f * odd)};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float a = __bfloat162float(__float2bfloat16_rn(both[i])), b = __bfloat162float(__float2bfloat16_rn(both[i] - a));
-          sums[nt][u >> 2][2 * i] = pack(a, b);
-          sums[nt][u >> 2][2 * i + 1] = pack(both[i] - a - b, 0.f);
-        }
+        sum *= 1.f / 16777216.f;
+        const float a = __bfloat162float(__float2bfloat16_rn(sum)), b = __bfloat162float(__float2bfloat16_rn(sum - a));
+        qr.sums[nt][u >> 2][0] = pack(a, b);
+        qr.sums[nt][u >> 2][1] = pack(sum - a - b, 0.f);
       }
     }
   }
-  // Positions [all_lo, all_hi] are visible to every row of the tile.
-  const int all_hi = base_pos + row0 / G, last = base_pos + (row0 + rows - 1) / G;
-  const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
+}
 
-  float o[NG][2][NT][4];
-  float m[NT][2], l[NT][2];
+// The scores of a tile's 16 positions, up to the rows' factors: s[nt] has positions r0, r0 and r0 + 2, r0 + 2 of rows 2 t, 2 t + 1,
+// r0 = 4 (g / 2) + g % 2.
+template <int NT>
+__device__ __forceinline__ void tile_scores(float (&s)[NT][4], const Queries<NT>& qr, const unsigned char* kt) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, r0 = 4 * (g >> 1) + (g & 1);
+  unsigned ka[NG], kb[NG], pa[NG], pb[NG];
+  load_words<NG>(reinterpret_cast<const unsigned*>(kt) + r0 * (4 * NG) + t * NG, ka);
+  load_words<NG>(reinterpret_cast<const unsigned*>(kt) + (r0 + 2) * (4 * NG) + t * NG, kb);
+  const unsigned* pairs = reinterpret_cast<const unsigned*>(kt + CODES);
+  load_words<NG>(pairs + r0 * NG, pa);
+  load_words<NG>(pairs + (r0 + 2) * NG, pb);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = NOTHING;
-    l[nt][0] = l[nt][1] = 0.f;
+  for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-    for (int u = 0; u < NG; ++u)
+  for (int x = 0; x < MG; ++x) {
+    const int u = min(4 * x + t, NG - 1);
+    const unsigned wa = pairs[r0 * NG + u], wb = pairs[(r0 + 2) * NG + u];
+    const unsigned ma = __byte_perm(wa, wa, 0x3232), mb = __byte_perm(wb, wb, 0x3232);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], ma, mb, ma, mb, qr.sums[nt][x][0], qr.sums[nt][x][1]);
+  }
+#pragma unroll
+  for (int u = 0; u < NG; ++u) {
+    unsigned a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { a[j] = codes16(ka[u], j); b[j] = codes16(kb[u], j); }
+    const float sa = lo_bf16(pa[u]), sb = lo_bf16(pb[u]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float d[4];
+      mma_f16_first(d, a[0], b[0], a[1], b[1], qr.f[nt][u][0], qr.f[nt][u][1]);
+      mma_f16(d, a[2], b[2], a[3], b[3], qr.f[nt][u][2], qr.f[nt][u][3]);
+      s[nt][0] = fmaf(sa, d[0], s[nt][0]);
+      s[nt][1] = fmaf(sa, d[1], s[nt][1]);
+      s[nt][2] = fmaf(sb, d[2], s[nt][2]);
+      s[nt][3] = fmaf(sb, d[3], s[nt][3]);
+    }
+  }
+}
+
+// Adds a tile's values, weighted: pf[nt] holds the probabilities of the 16 positions for row g of every eight.
+template <int NT>
+__device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[NT][2], const unsigned char* vt) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
+#pragma unroll
+  for (int u = 0; u < NG; ++u) {
+    const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
+    const uint4 pairs = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
+    const __nv_bfloat162 s01 = pair_of(pairs.x), s23 = pair_of(pairs.y), m01 = pair_of(pairs.z), m23 = pair_of(pairs.w);
+    unsigned a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
+      b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mma_bf16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
+      mma_bf16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
+    }
+  }
+}
+
+template <int NT, int PER_SM>
+__global__ void __launch_bounds__(32 * WARPS, PER_SM)
+kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
+                 const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
+                 const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
+                 float scale_log2, int max_rows, float* __restrict__ scratch, int* __restrict__ status) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int COLS = 8 * NT;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int r0 = 4 * (g >> 1) + (g & 1);        // see tile_scores
+  co_pdl_wait();
+  co_pdl_launch_dependents();
+  const int G = nh / nkv;
+  const int total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window), shares = min((int)gridDim.x, total);
+  if ((int)blockIdx.x >= shares) return;
+  int unit = share_start(blockIdx.x, shares, total);
+  const int unit_end = share_start(blockIdx.x + 1, shares, total);
+  Place at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
+  unsigned char* ring = smem + (size_t)warp * RING;       // keys, then values
+  const unsigned ring_lane = smem_u32(ring) + lane * 16;
+  const unsigned char *k_lane = k_cache + lane * 16, *v_lane = v_cache + lane * 16;
+
+  for (bool first_list = true; at.b >= 0; first_list = false) {
+    const Cut c = at.cut;
+    const int list = (unit - at.first) / c.units, u_first = unit - at.first - list * c.units, u_end = min(c.units, u_first + unit_end - unit);
+    const int row_tile = list % c.row_tiles, kvh = list / c.row_tiles;
+    const int row0 = row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
+    const int* table = block_tables + (size_t)at.b * table_ld;
+    const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
+    const int tile0 = c.lo16 + u_first * (UNIT / 16) + 2 * warp;
+    const int n_pairs = tile_end > tile0 ? (tile_end - tile0 + 2 * WARPS - 1) / (2 * WARPS) : 0;    // of this warp
+    const int base_pos = c.kv_len - c.q_len;
+
+    // Where the warp's tiles lie in a cache, 16 pairs at a time, a tile per lane; `valid`: the lanes whose tile exists.
+    long long place = 0;
+    unsigned valid = 0;
+    auto fetch_places = [&](int i0) {
+      const int tile = tile0 + (i0 + (lane >> 1)) * 2 * WARPS + (lane & 1), per_page = page_size >> 4;
+      bool ok = tile < tile_end;
+      place = 0;
+      if (ok) {
+        const int blk = tile / per_page, page = blk < table_ld ? table[blk] : -1;
+        ok = page >= 0 && page < num_pages;
+        if (ok) place = (((long long)page * nkv + kvh) * per_page + (tile - blk * per_page)) * TB;
+        else if (status) *status = BAD_INDEX;
+      }
+      valid = __ballot_sync(0xffffffffu, ok);
+    };
+    unsigned known = 0;              // two bits per pair, the latest lowest: the tile is there (zeros otherwise)
+    auto issue = [&](int i, int v_stage) {        // one group per call, with or without copies
+      known <<= 2;
+      if (i < n_pairs) {
+        if ((i & 15) == 0) fetch_places(i);
+        const unsigned there = (valid >> (2 * (i & 15))) & 3u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const long long from = __shfl_sync(0xffffffffu, place, 2 * (i & 15) + h);
+          const int bytes = (there >> h) & 1u ? 16 : 0;
+          copy_tile(ring_lane + (i & 1) * PAIR + h * TB, k_lane + from, lane, bytes);
+          copy_tile(ring_lane + (K_STAGES + v_stage) * PAIR + h * TB, v_lane + from, lane, bytes);
+        }
+        known |= there;
+      }
+      cp_async_commit();
+    };
+    issue(0, 0);
+    issue(1, 1);
+
+    Queries<NT> qr;
+    load_queries<NT>(qr, q, q_ld, c.tok0, G, kvh, row0, rows, scale_log2);
+    Sums<NT> sm;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sm.m[nt][0] = sm.m[nt][1] = NOTHING;
+      sm.l[nt][0] = sm.l[nt][1] = 0.f;
+#pragma unroll
+      for (int u = 0; u < NG; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sm.o[u][h][nt][i] = 0.f;
+    }
+    // Positions [all_lo, all_hi] are visible to every row of the tile.
+    const int all_hi = base_pos + row0 / G, last = base_pos + (row0 + rows - 1) / G;
+    const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
+
+    float s[2][NT][4];
+    unsigned pf[2][NT][2];
+    // From the scores s of pair i, whose values are at `values`, to its probabilities pf.
+    auto probabilities = [&](int i, unsigned char* values) {
+      const int key0 = (tile0 + i * 2 * WARPS) * 16;
+      const unsigned there = (known >> 2) & 3u;        // of pair i: pair i + 1 was issued last
+      float y[2][NT][4];            // exponents: scores (times log2 e) from the row's reference
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[u][h][nt][i] = 0.f;
-  }
-  const int r0 = 4 * (g >> 1) + (g & 1);        // this lane's rows of a tile in the first product: r0 and r0 + 2
-  const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
-
-#pragma unroll 1
-  for (int i = 0; i < n_pairs; ++i) {
-    const int stage = i % STAGES;
-    const unsigned there = (known >> (2 * stage)) & 3u;
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();                               // landed for all lanes; all are done with the stage of pair i - 1
-    issue(i + STAGES - 1);
-    if (!there) continue;
-    unsigned char* pair = ring + stage * PAIR;
-    const int key0 = (tile0 + i * 2 * WARPS) * 16;
-
-    float s[2][NT][4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const unsigned char* kt = pair + h * 2 * TB;
-      unsigned ka[NG], kb[NG], pa[NG], pb[NG];
-      load_words<NG>(reinterpret_cast<const unsigned*>(kt) + r0 * (4 * NG) + t * NG, ka);
-      load_words<NG>(reinterpret_cast<const unsigned*>(kt) + (r0 + 2) * (4 * NG) + t * NG, kb);
-      const unsigned* pairs = reinterpret_cast<const unsigned*>(kt + CODES);
-      load_words<NG>(pairs + r0 * NG, pa);
-      load_words<NG>(pairs + (r0 + 2) * NG, pb);
+          for (int x = 0; x < 4; ++x) y[h][nt][x] = fmaf(s[h][nt][x], qr.cs[nt][x & 1], -sm.m[nt][x & 1]);
+      if (!(there == 3u && key0 >= all_lo && key0 + 31 <= all_hi)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < MG; ++x) {
-        const int u = min(4 * x + t, NG - 1);
-        const unsigned wa = pairs[r0 * NG + u], wb = pairs[(r0 + 2) * NG + u];
-        const unsigned ma = __byte_perm(wa, wa, 0x3232), mb = __byte_perm(wb, wb, 0x3232);
-        const unsigned sa = __byte_perm(wa, wa, 0x1010), sb = __byte_perm(wb, wb, 0x1010);
+          for (int x = 0; x < 4; ++x) {
+            const int r = nt * 8 + 2 * t + (x & 1), hi = r < rows ? base_pos + (row0 + r) / G : -1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(s[h][nt], ma, mb, ma, mb, sums[nt][x][0], sums[nt][x][1]);
-          mma_bf16(s[h][nt], sa, sb, sa, sb, sums[nt][x][2], sums[nt][x][3]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < NG; ++u) {
-        unsigned a[4], b[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { a[j] = codes16(ka[u], j); b[j] = codes16(kb[u], j); }
-        const float sa = lo_bf16(pa[u]), sb = lo_bf16(pb[u]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float d[4];
-          mma_f16_first(d, a[0], b[0], a[1], b[1], qf[nt][u][0], qf[nt][u][1]);
-          mma_f16(d, a[2], b[2], a[3], b[3], qf[nt][u][2], qf[nt][u][3]);
-          s[h][nt][0] = fmaf(sa, d[0], s[h][nt][0]);
-          s[h][nt][1] = fmaf(sa, d[1], s[h][nt][1]);
-          s[h][nt][2] = fmaf(sb, d[2], s[h][nt][2]);
-          s[h][nt][3] = fmaf(sb, d[3], s[h][nt][3]);
-        }
-      }
-    }
-    float y[2][NT][4];            // exponents: scores (times log2 e) from the row's reference
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) y[h][nt][x] = fmaf(s[h][nt][x], cs[nt][x & 1], -m[nt][x & 1]);
-    if (!(there == 3u && key0 >= all_lo && key0 + 31 <= all_hi)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = nt * 8 + 2 * t + (x & 1), hi = r < rows ? base_pos + (row0 + r) / G : -1;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int pos = key0 + 16 * h + r0 + (x & 2);
-            if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) y[h][nt][x] = -INFINITY;
+            for (int h = 0; h < 2; ++h) {
+              const int pos = key0 + 16 * h + r0 + (x & 2);
+              if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) y[h][nt][x] = -INFINITY;
+            }
           }
-        }
-      // Rows of the tiles outside what any query sees may hold anything (a stale row, a page's end): their pairs of the
-      // values become zero, so that nothing which is not finite meets a probability of zero.
-      const int row = lane & 15, h = lane >> 4, pos = key0 + lane;
-      if (!((there >> h) & 1u) || pos > last || (window > 0 && pos <= all_hi - window)) {
-        unsigned short* pairs = reinterpret_cast<unsigned short*>(pair + h * 2 * TB + TB + CODES) + (row >> 2) * 8 + (row & 3);
+        // Rows of the tiles outside what any query sees may hold anything (a stale row, a page's end): their pairs of
+        // the values become zero, so that nothing which is not finite meets a probability of zero.
+        const int row = lane & 15, h = lane >> 4, pos = key0 + lane;
+        if (!((there >> h) & 1u) || pos > last || (window > 0 && pos <= all_hi - window)) {
+          unsigned short* pairs = reinterpret_cast<unsigned short*>(values + h * TB + CODES) + (row >> 2) * 8 + (row & 3);
 #pragma unroll
-        for (int u = 0; u < NG; ++u) pairs[u * 32] = pairs[u * 32 + 4] = 0;
+          for (int u = 0; u < NG; ++u) pairs[u * 32] = pairs[u * 32 + 4] = 0;
+        }
+        __syncwarp();
       }
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) grew = grew || fmaxf(y[0][nt][x], y[1][nt][x]) > SLACK;
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float M = sm.m[nt][e];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int x = e; x < 4; x += 2) M = y[h][nt][x] == -INFINITY ? M : fmaxf(M, s[h][nt][x] * qr.cs[nt][e]);
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+            const float f = ex2(sm.m[nt][e] - M);
+            sm.m[nt][e] = M;
+            sm.l[nt][e] *= f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int x = e; x < 4; x += 2) y[h][nt][x] = y[h][nt][x] == -INFINITY ? -INFINITY : fmaf(s[h][nt][x], qr.cs[nt][e], -M);
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) { sm.o[u][h][nt][e] *= f; sm.o[u][h][nt][2 + e] *= f; }
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            y[h][nt][x] = ex2(y[h][nt][x]);
+            sm.l[nt][x & 1] += y[h][nt][x];
+          }
+          pf[h][nt][0] = transposed(pack(y[h][nt][0], y[h][nt][1]));
+          pf[h][nt][1] = transposed(pack(y[h][nt][2], y[h][nt][3]));
+        }
+    };
+
+    unsigned char* values = ring + K_STAGES * PAIR;            // of pair i
+    if (n_pairs > 0) {
+      cp_async_wait<1>();
       __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) tile_scores<NT>(s[h], qr, ring + h * TB);
+      probabilities(0, values);
     }
-    bool grew = false;
+    int v_stage = 0;
+#pragma unroll 1
+    for (int i = 0; i < n_pairs; ++i) {
+      unsigned char* now = values;
+      if (i + 1 < n_pairs) {
+        // Keys of pair i + 2 go where pair i's were, values where pair i - 1's were.
+        issue(i + 2, v_stage == 0 ? V_STAGES - 1 : v_stage - 1);
+        v_stage = v_stage == V_STAGES - 1 ? 0 : v_stage + 1;
+        values = ring + (K_STAGES + v_stage) * PAIR;
+        cp_async_wait<1>();
+        __syncwarp();                // pair i + 1 landed for all lanes
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tile_values<NT>(sm, pf[h], now + h * TB);
+          tile_scores<NT>(s[h], qr, ring + ((i + 1) & 1) * PAIR + h * TB);
+        }
+        probabilities(i + 1, values);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tile_values<NT>(sm, pf[h], now + h * TB);
+      }
+      __syncwarp();                  // all lanes are done with pair i
+    }
+
+    cp_async_wait<0>();
+    __syncthreads();                 // the rings become the warps' meeting
+    float* merge = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) grew = grew || fmaxf(y[0][nt][x], y[1][nt][x]) > SLACK;
-    if (__any_sync(0xffffffffu, grew)) {
+      for (int e = 0; e < 2; ++e) {
+        float sum = sm.l[nt][e];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        float* dst = merge + (size_t)(warp * COLS + nt * 8 + 2 * t + e) * MLD;
+        if (g == 0) { dst[HD] = sm.m[nt][e]; dst[HD + 1] = sum; }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float M = m[nt][e];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = e; x < 4; x += 2) M = y[h][nt][x] == -INFINITY ? M : fmaxf(M, s[h][nt][x] * cs[nt][e]);
-#pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-          const float f = ex2(m[nt][e] - M);
-          m[nt][e] = M;
-          l[nt][e] *= f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = e; x < 4; x += 2) y[h][nt][x] = y[h][nt][x] == -INFINITY ? -INFINITY : fmaf(s[h][nt][x], cs[nt][e], -M);
-#pragma unroll
-          for (int u = 0; u < NG; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) { o[u][h][nt][e] *= f; o[u][h][nt][2 + e] *= f; }
-        }
-    }
-    unsigned pf[2][NT][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          s[h][nt][x] = ex2(y[h][nt][x]);
-          l[nt][x & 1] += s[h][nt][x];
-        }
-        pf[h][nt][0] = transposed(pack(s[h][nt][0], s[h][nt][1]));
-        pf[h][nt][1] = transposed(pack(s[h][nt][2], s[h][nt][3]));
+        for (int u = 0; u < NG; ++u)
+          *reinterpret_cast<float4*>(dst + u * 32 + g * 4) =
+              make_float4(sm.o[u][0][nt][e], sm.o[u][0][nt][2 + e], sm.o[u][1][nt][e], sm.o[u][1][nt][2 + e]);
       }
+    __syncthreads();
+    const int slot = 2 * blockIdx.x + (first_list ? 0 : 1);
+    float* acc_out = scratch + (size_t)slot * COLS * HD;
+    float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)2 * gridDim.x * COLS * HD) + (size_t)slot * COLS;
+    if (tid == 0 && u_first == 0) {
+      int2* heads = reinterpret_cast<int2*>(scratch + (size_t)2 * gridDim.x * COLS * (HD + 2));
+      heads[((size_t)at.b * nkv + kvh) * ((max_rows + COLS - 1) / COLS) + row_tile] =
+          make_int2(share_of(unit + c.units - 1, shares, total) - (int)blockIdx.x + 1, slot);
+    }
+    const bool whole_list = u_first == 0 && u_end == c.units;
+    for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
+      const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
+      float M = NOTHING, den = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, merge[(size_t)(w * COLS + r) * MLD + HD]);
 #pragma unroll
-      for (int u = 0; u < NG; ++u) {
-        const unsigned char* vt = pair + h * 2 * TB + TB;
-        const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
-        const uint4 sm = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
-        const __nv_bfloat162 s01 = pair_of(sm.x), s23 = pair_of(sm.y), m01 = pair_of(sm.z), m23 = pair_of(sm.w);
-        unsigned a[4], b[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
-          b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(o[u][0][nt], a[0], a[1], b[0], b[1], pf[h][nt][0], pf[h][nt][1]);
-          mma_bf16(o[u][1][nt], a[2], a[3], b[2], b[3], pf[h][nt][0], pf[h][nt][1]);
-        }
+      for (int w = 0; w < WARPS; ++w) {
+        const float* src = merge + (size_t)(w * COLS + r) * MLD;
+        const float f = exp2f(src[HD] - M);
+        const float4 v = *reinterpret_cast<const float4*>(src + ch);
+        den += f * src[HD + 1];
+        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
       }
-  }
-  cp_async_wait<0>();
-  __syncthreads();               // the rings become the merge area: [warp][row][HD channels, maximum, sum]
-  constexpr int MLD = HD + 4;
-  float* merge = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = l[nt][e];
-#pragma unroll
-      for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      float* dst = merge + (size_t)(warp * COLS + nt * 8 + 2 * t + e) * MLD;
-      if (g == 0) { dst[HD] = m[nt][e]; dst[HD + 1] = sum; }
-#pragma unroll
-      for (int u = 0; u < NG; ++u)
-        *reinterpret_cast<float4*>(dst + u * 32 + g * 4) = make_float4(o[u][0][nt][e], o[u][0][nt][2 + e], o[u][1][nt][e], o[u][1][nt][2 + e]);
+      if (whole_list) {
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const int row = row0 + r;
+        bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD + ch;
+        store4<bf16>(dst, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(acc_out + (size_t)r * HD + ch) = acc;
+        if (ch == 0) ml_out[r] = make_float2(M, den);
+      }
     }
-  __syncthreads();
-  const int slot = 2 * blockIdx.x + (first_list ? 0 : 1);
-  float* acc_out = scratch + (size_t)slot * COLS * HD;
-  float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)2 * gridDim.x * COLS * HD) + (size_t)slot * COLS;
-  const bool whole_list = u_first == 0 && u_end == c.units;
-  for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
-    const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
-    float M = NOTHING, den = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, merge[(size_t)(w * COLS + r) * MLD + HD]);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float* src = merge + (size_t)(w * COLS + r) * MLD;
-      const float f = exp2f(src[HD] - M);
-      const float4 v = *reinterpret_cast<const float4*>(src + ch);
-      den += f * src[HD + 1];
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-    }
-    if (whole_list) {
-      const float inv = den == 0.f ? 0.f : 1.f / den;
-      const int row = row0 + r;
-      bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD + ch;
-      store4<bf16>(dst, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    } else {
-      *reinterpret_cast<float4*>(acc_out + (size_t)r * HD + ch) = acc;
-      if (ch == 0) ml_out[r] = make_float2(M, den);
-    }
-  }
-  unit += u_end - u_first;
-  if (unit >= unit_end) return;
-  __syncthreads();               // the merge area becomes the rings again
-  if (unit - at.first >= c.units * c.row_tiles * nkv)
-    at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, at.b + 1, unit);
+    unit += u_end - u_first;
+    if (unit >= unit_end) return;
+    __syncthreads();                 // the meeting becomes the rings again
+    if (unit - at.first >= c.units * c.row_tiles * nkv)
+      at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, at.b + 1, unit);
   }
 }
 
 // Joins the parts of a list's row: one CTA per (row of a request's kv head, kv head, request), its warps side by side over
-// the parts, four channels per lane, and the warps' sums in order at the end.
-constexpr int CW = 4;
+// the parts, four channels per lane, and the warps' sums in order at the end.  Bound by its chain of dependent reads (the
+// list's note, then references and accumulators at once).
+constexpr int CW = 8;
 __global__ void __launch_bounds__(32 * CW)
-kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q,
-                const int* __restrict__ kv_lens, int B, int nh, int nkv, int cols, int window, int max_rows) {
+kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q, int nh, int nkv,
+                int cols, int max_rows) {
   constexpr int V = (HD + 127) / 128;
   __shared__ float part[CW][HD];
   __shared__ float part_den[CW];
-  __shared__ int found[3];
-  co_pdl_launch_dependents();
   const int r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = nh / nkv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // Safe ahead of the wait: the kernel before starts this one only after its own wait for whatever made the lengths.
-  const Cut c = cut_of(cu_q, kv_lens, b, G, cols, max_rows, window);
-  if (c.row_tiles == 0 || r >= c.q_len * G) return;
-  if (warp == 0) {
-    const int total = all_units(cu_q, kv_lens, B, nkv, G, cols, max_rows, window), shares = min(ctas, total);
-    int before = 0;
-    for (int x = lane; x < b; x += 32) {
-      const Cut d = cut_of(cu_q, kv_lens, x, G, cols, max_rows, window);
-      before += d.units * d.row_tiles * nkv;
-    }
-    const int first = __reduce_add_sync(0xffffffffu, before) + (kvh * c.row_tiles + r / cols) * c.units;
-    if (lane == 0) {
-      const int cta = share_of(first, shares, total);
-      found[0] = cta;
-      found[1] = share_of(first + c.units - 1, shares, total) - cta + 1;
-      found[2] = share_start(cta, shares, total) == first ? 0 : 1;
-    }
-  }
-  __syncthreads();
-  const int parts = found[1], col = r % cols;
-  if (parts == 1) return;
-  // Part 0 is at place 2 cta or 2 cta + 1, part p at 2 (cta + p).
-  const int cta = found[0], odd = found[2];
-  const float2* ml = reinterpret_cast<const float2*>(scratch + (size_t)2 * ctas * cols * HD) + (size_t)2 * cta * cols + col;
-  const float* acc_in = scratch + ((size_t)2 * cta * cols + col) * HD;
-  auto place = [&](int p) { return (size_t)(2 * p + (p == 0 ? odd : 0)) * cols; };
+  const int tok0 = cu_q[b], rows = (cu_q[b + 1] - tok0) * G;
+  if (rows > max_rows || r >= rows) return;
+  const size_t per_part = (size_t)cols * HD;
+  const float2* all_ml = reinterpret_cast<const float2*>(scratch + (size_t)2 * ctas * per_part);
+  const int2* heads = reinterpret_cast<const int2*>(scratch + (size_t)2 * ctas * cols * (HD + 2));
   co_pdl_wait();
-  float M = NOTHING;
-  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[place(p)].x);
-  M = co_warp_max(M);
-  float den = 0.f;
+  const int2 head = heads[((size_t)b * nkv + kvh) * ((max_rows + cols - 1) / cols) + r / cols];
+  const int parts = head.x, col = r % cols;
+  if (parts == 1) return;
+  // Part 0 is at head.y = 2 cta or 2 cta + 1, part p at 2 (cta + p).
+  auto place = [&](int p) { return p == 0 ? head.y : (head.y & ~1) + 2 * p; };
+  auto ml_of = [&](int p) { return all_ml[(size_t)place(p) * cols + col]; };
   float4 acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = NOTHING, den = 0.f;
+  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml_of(p).x);
+  bool known = false;               // M: after the first accumulators are on their way
   for (int p0 = warp * 8; p0 < parts; p0 += CW * 8) {
-    float f = 0.f;
-    if (lane < 8 && p0 + lane < parts) {
-      const float2 x = ml[place(p0 + lane)];
-      f = exp2f(x.x - M);
-      den += f * x.y;
-    }
+    const float2 ml = lane < 8 && p0 + lane < parts ? ml_of(p0 + lane) : make_float2(NOTHING, 0.f);
     float4 in[8][V];
 #pragma unroll
     for (int p = 0; p < 8; ++p)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int ch = v * 128 + lane * 4;
-        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(acc_in + place(p0 + p) * HD + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
+        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(scratch + place(p0 + p) * per_part + (size_t)col * HD + ch)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+    if (!known) M = co_warp_max(M);
+    known = true;
+    const float f = exp2f(ml.x - M);
+    den += f * ml.y;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const float fp = __shfl_sync(0xffffffffu, f, p);
@@ -1033,40 +1062,44 @@ kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ 
   }
   if (lane == 0) part_den[warp] = den;
   __syncthreads();
-  const int ch = threadIdx.x * 4;
+  const int ch = threadIdx.x * 4, used = min(CW, (parts + 7) / 8);
   if (ch < HD) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float d = 0.f;
-#pragma unroll
-    for (int w = 0; w < CW; ++w) {
+    for (int w = 0; w < used; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(&part[w][ch]);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
       d += part_den[w];
     }
     const float inv = d == 0.f ? 0.f : 1.f / d;
-    store4<bf16>(out + (size_t)(c.tok0 + r / G) * out_ld + (size_t)(kvh * G + r % G) * HD + ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    store4<bf16>(out + (size_t)(tok0 + r / G) * out_ld + (size_t)(kvh * G + r % G) * HD + ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
   }
 }
 
 int tiles_of(int max_rows) { return max_rows <= 8 || HD > 128 ? 1 : 2; }
-// CTAs that cut the step's units: those that are resident at a time, or one per unit when there are fewer.
-int ctas_of(int B, int nkv, int max_rows, int max_kv_len) {
+// CTAs that are resident per SM, by their registers.
+constexpr int MOST = HD <= 128 ? 4 : 2, FEWER = HD <= 128 ? 3 : 2;
+// CTAs that cut the step's units: those that are resident at a time, or one per unit when there are fewer units.  One row tile: three CTAs per SM,
+// whose 168 registers let a warp work ahead, beat four of 128 where the shares are long (2 x 131,072 positions: 39.2 against
+// 42 us; 64 x up to 16,384: 138 against 140), four where every unit gets a CTA at once (8 x 4,096: 11.0 against 13.3).
+int ctas_of(int B, int nkv, int max_rows, int max_kv_len, int* per_sm = nullptr) {
   const int nt = tiles_of(max_rows);
-  static int slots = getenv("KV4_SLOTS") ? atoi(getenv("KV4_SLOTS")) : 148 * 4;
   const long long lists = (long long)B * nkv * ((max_rows + 8 * nt - 1) / (8 * nt)), units = lists * (((long long)max_kv_len + 15) / UNIT + 1);
-  return (int)(units < slots ? units : slots);
+  const int resident = nt == 2 ? 2 : units <= 148 * MOST ? MOST : FEWER;
+  if (per_sm) *per_sm = resident;
+  return (int)(units < 148 * resident ? units : 148 * resident);
 }
 
-template <int NT>
+template <int NT, int PER_SM>
 int launch_items(const void* q, long q_ld, void* out, long out_ld, const void* k_cache, const void* v_cache, int num_pages, const int* table,
                  int table_ld, const int* cu_q, const int* kv_lens, int B, int nh, int nkv, int page_size, int window, float scale_log2,
                  int max_rows, int ctas, float* scratch, int* status, cudaStream_t stream) {
   constexpr size_t SMEM = items_smem<NT>();
   if (SMEM > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_items_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    cudaError_t e = cudaFuncSetAttribute(kv4_items_kernel<NT, PER_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
     if (e != cudaSuccess) CO_FAIL("kv4_attention: %zu bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
   }
-  co_launch(kv4_items_kernel<NT>, dim3((unsigned)ctas), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
+  co_launch(kv4_items_kernel<NT, PER_SM>, dim3((unsigned)ctas), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
             (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
             window, scale_log2, max_rows, scratch, status);
   CO_CHECK_LAUNCH("kv4_items");
@@ -1154,7 +1187,8 @@ CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, 
 
 // Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests that it takes.
 CO_EXPORT long coheryn_kv4_scratch_floats(int B, int nkv, int max_rows, int max_kv_len) {
-  return 2L * ctas_of(B, nkv, max_rows, max_kv_len) * 8 * tiles_of(max_rows) * (HD + 2);
+  const int cols = 8 * tiles_of(max_rows);
+  return 2L * ctas_of(B, nkv, max_rows, max_kv_len) * cols * (HD + 2) + 2L * B * nkv * ((max_rows + cols - 1) / cols);
 }
 
 // Attention of the requests with at most `max_rows` query rows per kv head, in bfloat16: q [T, nh * HD] of stride q_ld, out likewise;
@@ -1169,20 +1203,18 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   if ((q_ld & 7) || (out_ld & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15))
     CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
   if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
-  const int nt = tiles_of(max_rows);
-  const int ctas = ctas_of(B, nkv, max_rows, max_kv_len);
+  int per_sm = 0;
+  const int nt = tiles_of(max_rows), ctas = ctas_of(B, nkv, max_rows, max_kv_len, &per_sm);
   if ((long long)B * nkv * ((max_rows + 7) / 8) * ((max_kv_len + 15LL) / UNIT + 1) > 0x7fffffffLL)
     CO_FAIL("kv4_attention: %d requests of %d positions and %d kv heads", B, max_kv_len, nkv);
   if (scratch_floats < coheryn_kv4_scratch_floats(B, nkv, max_rows, max_kv_len) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_attention: the scratch is too small or not 16-byte aligned");
-  const float scale_log2 = scale * 1.4426950408889634f;
-  const int rc = nt == 1 ? launch_items<1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-                                           window, scale_log2, max_rows, ctas, scratch, status, stream)
-                         : launch_items<HD <= 128 ? 2 : 1>(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-                                           window, scale_log2, max_rows, ctas, scratch, status, stream);
+  auto launch = nt == 2 ? launch_items<HD <= 128 ? 2 : 1, 2> : per_sm == MOST ? launch_items<1, MOST> : launch_items<1, FEWER>;
+  const int rc = launch(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size, window,
+                        scale * 1.4426950408889634f, max_rows, ctas, scratch, status, stream);
   if (rc || max_kv_len + 15 <= UNIT) return rc;    // no list is longer than one unit: nothing to join
   co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, ctas,
-            (bf16*)out, out_ld, cu_q, kv_lens, B, nh, nkv, 8 * nt, window, max_rows);
+            (bf16*)out, out_ld, cu_q, nh, nkv, 8 * nt, max_rows);
   CO_CHECK_LAUNCH("kv4_join");
   return 0;
 }
