@@ -999,80 +999,93 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   }
 }
 
-// Joins the parts of a list's row: one CTA per (row of a request's kv head, kv head, request), its warps side by side over
-// the parts, four channels per lane, and the warps' sums in order at the end.  Bound by its chain of dependent reads (the
-// list's note, then references and accumulators at once).
+// Joins the parts of the lists' rows.  A warp takes every `step`-th eight of a row's parts, four channels per lane.  WIDE: one CTA
+// per row, its warps side by side over the parts, their sums added in order at the end; else one CTA per list and a warp per
+// row.  Bound by its chain of dependent reads (the list's note, then references and accumulators at once); with many
+// lists, of few parts each, by the number of CTAs.
 constexpr int CW = 8;
+template <bool WIDE>
 __global__ void __launch_bounds__(32 * CW)
 kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ out, long out_ld, const int* __restrict__ cu_q, int nh, int nkv,
                 int cols, int max_rows) {
   constexpr int V = (HD + 127) / 128;
-  __shared__ float part[CW][HD];
+  __shared__ float part[WIDE ? CW : 1][HD];
   __shared__ float part_den[CW];
-  const int r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = nh / nkv;
+  const int kvh = blockIdx.y, b = blockIdx.z, G = nh / nkv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // Safe ahead of the wait: the kernel before starts this one only after its own wait for whatever made the lengths.
   const int tok0 = cu_q[b], rows = (cu_q[b + 1] - tok0) * G;
-  if (rows > max_rows || r >= rows) return;
+  const int row_tile = WIDE ? (int)blockIdx.x / cols : (int)blockIdx.x;
+  if (rows > max_rows || (WIDE ? (int)blockIdx.x : row_tile * cols) >= rows) return;
   const size_t per_part = (size_t)cols * HD;
   const float2* all_ml = reinterpret_cast<const float2*>(scratch + (size_t)2 * ctas * per_part);
   const int2* heads = reinterpret_cast<const int2*>(scratch + (size_t)2 * ctas * cols * (HD + 2));
   co_pdl_wait();
-  const int2 head = heads[((size_t)b * nkv + kvh) * ((max_rows + cols - 1) / cols) + r / cols];
-  const int parts = head.x, col = r % cols;
+  const int2 head = heads[((size_t)b * nkv + kvh) * ((max_rows + cols - 1) / cols) + row_tile];
+  const int parts = head.x;
   if (parts == 1) return;
   // Part 0 is at head.y = 2 cta or 2 cta + 1, part p at 2 (cta + p).
   auto place = [&](int p) { return p == 0 ? head.y : (head.y & ~1) + 2 * p; };
-  auto ml_of = [&](int p) { return all_ml[(size_t)place(p) * cols + col]; };
-  float4 acc[V];
+  const int col_end = WIDE ? (int)blockIdx.x % cols + 1 : min(cols, rows - row_tile * cols);
+  for (int col = WIDE ? (int)blockIdx.x % cols : warp; col < col_end; col += CW) {
+    auto ml_of = [&](int p) { return all_ml[(size_t)place(p) * cols + col]; };
+    float4 acc[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float M = NOTHING, den = 0.f;
-  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml_of(p).x);
-  bool known = false;               // M: after the first accumulators are on their way
-  for (int p0 = warp * 8; p0 < parts; p0 += CW * 8) {
-    const float2 ml = lane < 8 && p0 + lane < parts ? ml_of(p0 + lane) : make_float2(NOTHING, 0.f);
-    float4 in[8][V];
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = NOTHING, den = 0.f;
+    for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml_of(p).x);
+    bool known = false;               // M: after the first accumulators are on their way
+    for (int p0 = WIDE ? warp * 8 : 0; p0 < parts; p0 += WIDE ? CW * 8 : 8) {
+      const float2 ml = lane < 8 && p0 + lane < parts ? ml_of(p0 + lane) : make_float2(NOTHING, 0.f);
+      float4 in[8][V];
 #pragma unroll
-    for (int p = 0; p < 8; ++p)
+      for (int p = 0; p < 8; ++p)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int ch = v * 128 + lane * 4;
+          in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(scratch + place(p0 + p) * per_part + (size_t)col * HD + ch)
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      if (!known) M = co_warp_max(M);
+      known = true;
+      const float f = exp2f(ml.x - M);
+      den += f * ml.y;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float fp = __shfl_sync(0xffffffffu, f, p);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          acc[v].x += fp * in[p][v].x; acc[v].y += fp * in[p][v].y; acc[v].z += fp * in[p][v].z; acc[v].w += fp * in[p][v].w;
+        }
+      }
+    }
+    den = co_warp_sum(den);
+    if (WIDE) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int ch = v * 128 + lane * 4;
-        in[p][v] = p0 + p < parts && ch < HD ? *reinterpret_cast<const float4*>(scratch + place(p0 + p) * per_part + (size_t)col * HD + ch)
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ch < HD) *reinterpret_cast<float4*>(&part[warp][ch]) = acc[v];
       }
-    if (!known) M = co_warp_max(M);
-    known = true;
-    const float f = exp2f(ml.x - M);
-    den += f * ml.y;
-#pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const float fp = __shfl_sync(0xffffffffu, f, p);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        acc[v].x += fp * in[p][v].x; acc[v].y += fp * in[p][v].y; acc[v].z += fp * in[p][v].z; acc[v].w += fp * in[p][v].w;
+      if (lane == 0) part_den[warp] = den;
+      __syncthreads();
+      if (warp >= V) return;
+      const int used = min(CW, (parts + 7) / 8), ch = threadIdx.x * 4;
+      acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+      den = 0.f;
+      for (int w = 0; w < used && ch < HD; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&part[w][ch]);
+        acc[0].x += x.x; acc[0].y += x.y; acc[0].z += x.z; acc[0].w += x.w;
+        den += part_den[w];
       }
     }
-  }
-  den = co_warp_sum(den);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    const int row = row_tile * cols + col;
+    bf16* dst = out + (size_t)(tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int ch = v * 128 + lane * 4;
-    if (ch < HD) *reinterpret_cast<float4*>(&part[warp][ch]) = acc[v];
-  }
-  if (lane == 0) part_den[warp] = den;
-  __syncthreads();
-  const int ch = threadIdx.x * 4, used = min(CW, (parts + 7) / 8);
-  if (ch < HD) {
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float d = 0.f;
-    for (int w = 0; w < used; ++w) {
-      const float4 x = *reinterpret_cast<const float4*>(&part[w][ch]);
-      sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-      d += part_den[w];
+    for (int v = 0; v < (WIDE ? 1 : V); ++v) {
+      const int ch = (WIDE ? warp : v) * 128 + lane * 4;
+      if (ch < HD) store4<bf16>(dst + ch, acc[v].x * inv, acc[v].y * inv, acc[v].z * inv, acc[v].w * inv);
     }
-    const float inv = d == 0.f ? 0.f : 1.f / d;
-    store4<bf16>(out + (size_t)(tok0 + r / G) * out_ld + (size_t)(kvh * G + r % G) * HD + ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
   }
 }
 
@@ -1213,8 +1226,10 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   const int rc = launch(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size, window,
                         scale * 1.4426950408889634f, max_rows, ctas, scratch, status, stream);
   if (rc || max_kv_len + 15 <= UNIT) return rc;    // no list is longer than one unit: nothing to join
-  co_launch(kv4_join_kernel, dim3((unsigned)max_rows, (unsigned)nkv, (unsigned)B), dim3(32 * CW), 0, stream, (const float*)scratch, ctas,
-            (bf16*)out, out_ld, cu_q, nh, nkv, 8 * nt, max_rows);
+  const int cols = 8 * nt;
+  const bool wide = (long long)B * nkv * max_rows <= 148 * 4;
+  co_launch(wide ? kv4_join_kernel<true> : kv4_join_kernel<false>, dim3((unsigned)(wide ? max_rows : (max_rows + cols - 1) / cols), (unsigned)nkv, (unsigned)B),
+            dim3(32 * CW), 0, stream, (const float*)scratch, ctas, (bf16*)out, out_ld, cu_q, nh, nkv, cols, max_rows);
   CO_CHECK_LAUNCH("kv4_join");
   return 0;
 }
