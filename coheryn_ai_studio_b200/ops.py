@@ -2126,7 +2126,53 @@ def lightning_attention(q, k, v, gate, powers: torch.Tensor, silu: bool, state: 
 
 
 # ------------------------------------------------------------------------------------
-# The step's index arrays made on the device.
+# The step's index arrays made on the device, and a cache that keeps keys and values in 4 bits.  Their calls are a few
+# microseconds of work on the device each, so the host's share counts: argument types are declared once (plain integers then
+# pass as pointers and sizes without a wrapper object each).
+
+
+def _here(*tensors) -> int:
+    """The current device, where all of ``tensors`` (None aside) have to live; the launches go to its current stream."""
+    device = _current_device() if _current_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            if not t.is_cuda:
+                raise KernelError("kernel operands must be CUDA tensors")
+            raise KernelError(f"an operand lives on cuda:{t.get_device()}, but the current device is cuda:{device}")
+    return device
+
+
+def _stream_number(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _words(n: Optional[int], **tensors) -> None:
+    """Contiguous int32 tensors, of ``n`` elements each when that is given."""
+    for name, t in tensors.items():
+        if t is not None:
+            if t.dtype is not torch.int32 or not t.is_contiguous():
+                raise KernelError(f"{name} must be a contiguous int32 tensor")
+            if n is not None and t.numel() != n:
+                raise KernelError(f"{name} has {t.numel()} elements, not {n}")
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+_declared = {}
+
+
+def _entry(lib, name: str, types: str):
+    """The library's function with its argument types: p pointer, i int, l long, f float."""
+    key = (id(lib), name)
+    fn = _declared.get(key)
+    if fn is None:
+        fn = getattr(lib, name)
+        fn.argtypes = [{"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}[c] for c in types]
+        fn.restype = c_int
+        _declared[key] = fn
+    return fn
 
 
 def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tensor, pages: torch.Tensor, page_size: int,
@@ -2147,33 +2193,28 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
 
     An ordinary launch: the arrays are complete before the next kernel in the stream begins, so kernels that look at a
     step's lengths ahead of their wait may follow it directly."""
-    _dev(starts, q_lens, page_cu, pages, block_table, slots, cu_q, kv_lens, positions, token_req, first, status)
-    B, T = starts.numel(), -1
-    for t, name, n in ((starts, "starts", B), (q_lens, "q_lens", B), (page_cu, "page_cu", B + 1), (pages, "pages", None),
-                       (block_table, "block_table", None), (cu_q, "cu_q", B + 1), (kv_lens, "kv_lens", B), (first, "first", B),
-                       (status, "status", 1)):
-        if t is not None:
-            _i32(t, name)
-            if n is not None and t.numel() != n:
-                raise KernelError(f"step_layout: {name} has {t.numel()} elements, not {n}")
-    for t, name in ((positions, "positions"), (token_req, "token_req"), (slots, "slots")):
-        if t is not None:
-            _i32(t, name)
-            if T >= 0 and t.numel() != T:
-                raise KernelError(f"step_layout: {name} has {t.numel()} elements, not {T}")
-            T = t.numel()
+    device = _here(starts, q_lens, page_cu, pages, block_table, slots, cu_q, kv_lens, positions, token_req, first, status)
+    B = starts.numel()
+    _words(B, starts=starts, q_lens=q_lens, kv_lens=kv_lens, first=first)
+    _words(B + 1, page_cu=page_cu, cu_q=cu_q)
+    _words(1, status=status)
+    _words(None, pages=pages, block_table=block_table)
+    per_token = slots if slots is not None else positions if positions is not None else token_req
+    T = per_token.numel() if per_token is not None else 0
+    _words(T, slots=slots, positions=positions, token_req=token_req)
     if block_table.dim() != 2 or block_table.shape[0] != B:
-        raise KernelError(f"step_layout: a block table of shape {tuple(block_table.shape)} for {B} requests")
-    if page_size < 1:
-        raise KernelError("step_layout: page_size must be positive")
+        raise KernelError(f"a block table of shape {tuple(block_table.shape)} for {B} requests")
     if B == 0:
         if cu_q is not None:
             cu_q.zero_()
         return
     lib = core()
-    _check(lib, lib.coheryn_step_layout(_ptr(starts), _ptr(q_lens), _ptr(page_cu), _ptr(pages), c_int(pages.numel()), _ptr(first), c_int(B),
-                                        c_int(max(T, 0)), c_int(page_size), _ptr(cu_q), _ptr(kv_lens), _ptr(positions), _ptr(token_req),
-                                        _ptr(block_table), c_int(block_table.shape[1]), _ptr(slots), _ptr(status), _stream()))
+    rc = _entry(lib, "coheryn_step_layout", "ppppipiiipppppippp")(
+        starts.data_ptr(), q_lens.data_ptr(), page_cu.data_ptr(), pages.data_ptr(), pages.numel(), _at(first), B, T, page_size, _at(cu_q),
+        _at(kv_lens), _at(positions), _at(token_req), block_table.data_ptr(), block_table.shape[1], _at(slots), _at(status),
+        _stream_number(device))
+    if rc:
+        _check(lib, rc)
 
 
 # ------------------------------------------------------------------------------------
@@ -2204,8 +2245,9 @@ def kv4_lib(head_dim: int):
     return lib
 
 
+@functools.lru_cache(maxsize=256)
 def kv4_page_shape(num_kv_heads: int, page_size: int, head_dim: int):
-    """The shape of one page of keys, or of values, in uint8: [kv heads, tiles of 16 positions, bytes of a tile]."""
+    """The shape of one page of keys, or of values, in uint8: (kv heads, tiles of 16 positions, bytes of a tile)."""
     if head_dim % 32 or not 32 <= head_dim <= 256:
         raise KernelError(f"the 4-bit cache takes head sizes 32..256 in steps of 32, not {head_dim}")
     if page_size % 16 or page_size < 16:
@@ -2216,10 +2258,15 @@ def kv4_page_shape(num_kv_heads: int, page_size: int, head_dim: int):
 def _kv4_caches(k_cache, v_cache, num_kv_heads: int, page_size: int, head_dim: int) -> None:
     shape = kv4_page_shape(num_kv_heads, page_size, head_dim)
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype != torch.uint8 or t.dim() != 4 or tuple(t.shape[1:]) != shape or not t.is_contiguous():
+        if t.dtype is not torch.uint8 or t.dim() != 4 or t.shape[1:] != shape or not t.is_contiguous():
             raise KernelError(f"{name} must be contiguous uint8 pages of shape {shape}, not {t.dtype} {tuple(t.shape)}")
     if k_cache.shape[0] != v_cache.shape[0]:
         raise KernelError("the key and the value cache have different numbers of pages")
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_scratch_floats(head_dim: int, B: int, num_kv_heads: int, rows: int, max_kv_len: int) -> int:
+    return int(kv4_lib(head_dim).coheryn_kv4_scratch_floats(c_int(B), c_int(num_kv_heads), c_int(rows), c_int(max_kv_len)))
 
 
 def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], slots: torch.Tensor,
@@ -2231,46 +2278,52 @@ def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin
     ``cos_sin`` may then be None).  Keys are rounded to the compute type before they are quantised.  A group of 32
     channels with a value that is not finite is kept as not-a-number.  Two rows with one slot: one of them is kept, or a
     mixture."""
-    _dev(qkv, positions, cos_sin, slots, k_cache, v_cache)
-    _i32(slots, "slots")
+    device = _here(qkv, positions, cos_sin, slots, k_cache, v_cache)
     T = qkv.shape[0]
+    _words(T, slots=slots)
     _kv4_caches(k_cache, v_cache, num_kv_heads, page_size, head_dim)
     nq = num_heads * head_dim
-    if qkv.dim() != 2 or qkv.shape[1] != nq + 2 * num_kv_heads * head_dim or qkv.stride(1) != 1 or slots.numel() != T:
-        raise KernelError(f"rope_kv4_write: rows of {num_heads} + 2 x {num_kv_heads} heads of {head_dim} and a slot each, not "
-                          f"{tuple(qkv.shape)} with {slots.numel()} slots")
+    if qkv.dim() != 2 or qkv.shape[1] != nq + 2 * num_kv_heads * head_dim or qkv.stride(1) != 1:
+        raise KernelError(f"rope_kv4_write: rows of {num_heads} + 2 x {num_kv_heads} heads of {head_dim}, not {tuple(qkv.shape)}")
+    code = _code(qkv)
     if rotary_dim:
-        if positions is None or cos_sin is None or positions.numel() != T:
+        if positions is None or cos_sin is None:
             raise KernelError("rope_kv4_write: a rotation needs a position for every row and a table")
-        _i32(positions, "positions")
-        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or tuple(cos_sin.shape[1:]) != (rotary_dim // 2, 2):
+        _words(T, positions=positions)
+        if cos_sin.dtype is not torch.float32 or not cos_sin.is_contiguous() or cos_sin.shape[1:] != (rotary_dim // 2, 2):
             raise KernelError(f"rope_kv4_write: cos_sin must be float32 [positions, {rotary_dim // 2}, 2]")
         q = torch.empty((T, nq), dtype=qkv.dtype, device=qkv.device)
     else:
         q = qkv[:, :nq]
     lib = kv4_lib(head_dim)
-    _check(lib, lib.coheryn_kv4_write(
-        _ptr(qkv), c_long(qkv.stride(0)), c_int(_code(qkv)), _ptr(positions), _ptr(cos_sin), c_int(cos_sin.shape[0] if rotary_dim else 0),
-        _ptr(slots), _ptr(k_cache), _ptr(v_cache), c_int(k_cache.shape[0]), _ptr(q if rotary_dim else None), c_int(T), c_int(num_heads),
-        c_int(num_kv_heads), c_int(rotary_dim), c_int(page_size), _ptr(tc_status(qkv.device)), _stream()))
+    rc = _entry(lib, "coheryn_kv4_write", "plippipppipiiiiipp")(
+        qkv.data_ptr(), qkv.stride(0), code, _at(positions), _at(cos_sin), cos_sin.shape[0] if rotary_dim else 0, slots.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], q.data_ptr() if rotary_dim else None, T, num_heads, num_kv_heads, rotary_dim,
+        page_size, tc_status(qkv.device).data_ptr(), _stream_number(device))
+    if rc:
+        _check(lib, rc)
     return q
 
 
 def kv4_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor, head_dim: int, page_size: int, dtype: torch.dtype):
     """Pages of a 4-bit cache as the values they stand for: (keys, values), each [n, kv heads, page_size, head_dim] in
     ``dtype``.  A page number outside the cache reads as zeros."""
-    _dev(k_cache, v_cache, pages)
-    _i32(pages, "pages")
+    device = _here(k_cache, v_cache, pages)
+    _words(None, pages=pages)
     nkv = k_cache.shape[1]
     _kv4_caches(k_cache, v_cache, nkv, page_size, head_dim)
-    if dtype not in _CODES:
+    code = _CODES.get(dtype)
+    if code is None:
         raise KernelError(f"dtype {dtype} is not handled by the kernels")
     n = pages.numel()
     k = torch.empty((n, nkv, page_size, head_dim), dtype=dtype, device=k_cache.device)
     v = torch.empty_like(k)
     lib = kv4_lib(head_dim)
-    _check(lib, lib.coheryn_kv4_pages(_ptr(k_cache), _ptr(v_cache), c_int(k_cache.shape[0]), c_int(nkv), c_int(page_size), _ptr(pages), c_int(n),
-                                      _ptr(k), _ptr(v), c_int(_CODES[dtype]), _ptr(tc_status(k_cache.device)), _stream()))
+    rc = _entry(lib, "coheryn_kv4_pages", "ppiiipippipp")(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], nkv, page_size, pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+        tc_status(k_cache.device).data_ptr(), _stream_number(device))
+    if rc:
+        _check(lib, rc)
     return k, v
 
 
@@ -2290,13 +2343,13 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``KV4_DIRECT_ROWS`` rows per kv
     head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to bfloat16 and
     go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
-    _dev(q, out, k_cache, v_cache, block_tables, token_req, positions, cu_q, kv_lens)
-    _i32(block_tables, "block_tables")
+    device = _here(q, out, k_cache, v_cache, block_tables, token_req, positions, cu_q, kv_lens)
     _kv4_caches(k_cache, v_cache, num_kv_heads, page_size, head_dim)
+    _words(None, block_tables=block_tables)
     if num_heads % num_kv_heads:
         raise KernelError(f"{num_heads} heads do not group over {num_kv_heads} kv heads")
     T, nq = q.shape[0], num_heads * head_dim
-    if q.dim() != 2 or q.shape[1] != nq or tuple(out.shape) != (T, nq) or q.stride(1) != 1 or out.stride(1) != 1 or out.dtype != q.dtype:
+    if q.shape != (T, nq) or out.shape != q.shape or q.stride(1) != 1 or out.stride(1) != 1 or out.dtype is not q.dtype:
         raise KernelError(f"attention_kv4: q and out must be [tokens, {nq}] of one type with contiguous rows")
     if block_tables.dim() != 2:
         raise KernelError("attention_kv4: block_tables must be [requests, entries]")
@@ -2305,34 +2358,36 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     if T == 0:
         return
     lib = kv4_lib(head_dim)
-    fast = (not force_simple and q.dtype == torch.bfloat16 and cu_q is not None and kv_lens is not None and q_lens is not None
-            and max_kv_len is not None and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 4 == 0
-            and out.data_ptr() % 8 == 0)
-    status = tc_status(q.device)
+    q_ld, out_ld, q_at, out_at = q.stride(0), out.stride(0), q.data_ptr(), out.data_ptr()
+    status, stream = tc_status(q.device).data_ptr(), _stream_number(device)
     num_pages, W = k_cache.shape[0], block_tables.shape[1]
-    if not fast:
-        _i32(token_req, "token_req"); _i32(positions, "positions")
-        if token_req.numel() != T or positions.numel() != T:
-            raise KernelError("attention_kv4: every row needs a request and a position")
-        _check(lib, lib.coheryn_kv4_attention_simple(
-            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), c_int(_code(q)), _ptr(k_cache), _ptr(v_cache), c_int(num_pages),
-            _ptr(block_tables), c_int(W), _ptr(token_req), _ptr(positions), c_int(T), c_int(num_heads), c_int(num_kv_heads),
-            c_int(page_size), c_int(window or 0), c_float(scale), _ptr(status), _stream()))
+    if (force_simple or q.dtype is not torch.bfloat16 or cu_q is None or kv_lens is None or q_lens is None or max_kv_len is None
+            or q_ld % 8 or q_at % 16 or out_ld % 4 or out_at % 8):
+        _words(T, token_req=token_req, positions=positions)
+        rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipippiiiiifpp")(
+            q_at, q_ld, out_at, out_ld, _code(q), k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W,
+            token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, status, stream)
+        if rc:
+            _check(lib, rc)
         return
-    _i32(cu_q, "cu_q"); _i32(kv_lens, "kv_lens")
     B, G = len(q_lens), num_heads // num_kv_heads
-    if cu_q.numel() != B + 1 or kv_lens.numel() != B or block_tables.shape[0] != B:
-        raise KernelError(f"attention_kv4: lengths and block tables of {B} requests are needed")
+    _words(B, kv_lens=kv_lens)
+    _words(B + 1, cu_q=cu_q)
+    if block_tables.shape[0] != B or B == 0:
+        raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
     limit = max(KV4_DIRECT_ROWS // G, 1)         # tokens that a request may bring to be read directly
-    direct = max((n for n in q_lens if n <= limit), default=0)
+    longest = max(q_lens)
+    direct = longest if longest <= limit else max((n for n in q_lens if n <= limit), default=0)
     if direct:
-        floats = int(lib.coheryn_kv4_scratch_floats(c_int(B), c_int(num_kv_heads), c_int(direct * G), c_int(max_kv_len)))
+        floats = _kv4_scratch_floats(head_dim, B, num_kv_heads, direct * G, max_kv_len)
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _check(lib, lib.coheryn_kv4_attention(
-            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), _ptr(k_cache), _ptr(v_cache), c_int(num_pages),
-            _ptr(block_tables), c_int(W), _ptr(cu_q), _ptr(kv_lens), c_int(B), c_int(num_heads), c_int(num_kv_heads), c_int(page_size),
-            c_int(window or 0), c_float(scale), c_int(direct * G), c_int(max_kv_len), _ptr(scratch), c_long(floats), _ptr(status), _stream()))
-    if max(q_lens) <= limit:
+        rc = _entry(lib, "coheryn_kv4_attention", "plplppipippiiiiifiiplpp")(
+            q_at, q_ld, out_at, out_ld, k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W, cu_q.data_ptr(),
+            kv_lens.data_ptr(), B, num_heads, num_kv_heads, page_size, window or 0, scale, direct * G, max_kv_len, scratch.data_ptr(), floats,
+            status, stream)
+        if rc:
+            _check(lib, rc)
+    if longest <= limit:
         return
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.
     width = min(W, -(-max_kv_len // page_size))
@@ -2350,14 +2405,15 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         k = torch.empty((n * width, num_kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
         v = torch.empty_like(k)
         table = torch.empty((n, width), dtype=torch.int32, device=q.device)
-        cu, lens = c_void_p(cu_q.data_ptr() + 4 * b), c_void_p(kv_lens.data_ptr() + 4 * b)
-        _check(lib, lib.coheryn_kv4_expand(
-            _ptr(k_cache), _ptr(v_cache), c_int(num_pages), c_int(num_kv_heads), c_int(page_size),
-            c_void_p(block_tables.data_ptr() + 4 * W * b), c_int(W), c_int(width), c_int(n), cu, lens, c_int(window or 0), _ptr(k), _ptr(v),
-            _ptr(table), _ptr(status), _stream()))
+        cu, lens = cu_q.data_ptr() + 4 * b, kv_lens.data_ptr() + 4 * b
+        rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiippippppp")(
+            k_cache.data_ptr(), v_cache.data_ptr(), num_pages, num_kv_heads, page_size, block_tables.data_ptr() + 4 * W * b, W, width, n, cu, lens,
+            window or 0, k.data_ptr(), v.data_ptr(), table.data_ptr(), status, stream)
+        if rc:
+            _check(lib, rc)
         rows = max(q_lens[b:e]) * G
         _check(prompt, prompt.coheryn_attention_bf16(
-            _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), _ptr(k), _ptr(v), _ptr(table), c_int(width), cu, lens, c_int(n),
-            c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
-            c_int(max_kv_len), c_void_p(0), c_long(0), _ptr(status), c_int(T), c_int(n * width), c_int(0), _stream()))
+            c_void_p(q_at), c_long(q_ld), c_void_p(out_at), c_long(out_ld), _ptr(k), _ptr(v), _ptr(table), c_int(width), c_void_p(cu), c_void_p(lens),
+            c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
+            c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * width), c_int(0), c_void_p(stream)))
         b = e
