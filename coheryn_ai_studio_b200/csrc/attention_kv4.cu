@@ -45,14 +45,15 @@ __device__ __forceinline__ size_t tile_at(long long page, int nkv, int kvh, int 
 }
 
 // ------------------------------------------------------------------------------------
-// Rotation and write.  A thread has 8 neighbouring channels of one head of one token; the four threads of a group agree
-// on its minimum and maximum by two shuffles.  Queries are rotated into their own rows; keys are rotated and rounded to
-// the compute type, as a cache in that type would hold them, and then quantised, values quantised as they are.  Every
-// product and sum of the rotation is rounded by itself (no fused multiply-add): the codes are then the same
-// function of the inputs wherever it is computed.
+// Rotation and write.  A thread has 8 neighbouring channels of a head; the four threads of a group agree on its minimum and
+// maximum by two shuffles.  Queries are rotated into their own rows; keys are rotated and rounded to the compute type, as
+// a cache in that type would hold them, and then quantised, values quantised as they are.  Every product and sum of the
+// rotation is rounded by itself (no fused multiply-add): the codes are then the same function of the inputs wherever it is
+// computed.
 //
-// Bound by the bytes of a prompt (2,048 tokens of 28 + 8 heads of 128: 19 MB read, 15 MB written) and by one launch at
-// decoding.
+// A block has one token, so that its position, slot and angles are looked up once for all heads (a thread per 8 channels of
+// any token and head, with its own angles and divisions: 2,048 tokens of 28 + 8 heads of 128 in 22 us).  Bound by the bytes of
+// a prompt (19 MB read, 17 MB written there) and by one launch at decoding.
 // ------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
@@ -84,113 +85,119 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
                  const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
-                 T* __restrict__ q_out, int tokens, int nh, int nkv, int rot, int page_size, int first_head, int* __restrict__ status) {
-  constexpr int TPH = HD / 8;                     // threads of a head
+                 T* __restrict__ q_out, int nh, int nkv, int rot, int page_size, int first_head, int* __restrict__ status) {
+  constexpr int TPH = HD / 8, AT_ONCE = 256 / TPH;      // threads of a head, heads at a time
   co_pdl_launch_dependents();
-  const int heads = nh + 2 * nkv - first_head;    // without a rotation there is nothing to do for the queries
-  const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long row_head = id / TPH;
-  const int piece = (int)(id % TPH);
-  const bool live = row_head < (long long)tokens * heads;
-  const int token = live ? (int)(row_head / heads) : 0;
-  const int head = first_head + (live ? (int)(row_head % heads) : 0);
-  const int c0 = piece * 8;
+  const int token = blockIdx.x, place = threadIdx.x / TPH, piece = threadIdx.x % TPH;
+  const int c0 = piece * 8, half = rot >> 1, heads = nh + 2 * nkv;
+  const int u = piece >> 2, t = piece & 3;
   co_pdl_wait();
-  const T* src = qkv + (size_t)token * ld + (size_t)head * HD;
-  float x[8];
-  load8(src + c0, x);
-  if (rot && head < nh + nkv) {
-    const int half = rot >> 1;
+  const T* row = qkv + (size_t)token * ld;
+  // The token's angles for these channels: x cos -+ partner sin, the partner half a rotation away.
+  float cs[8], sn[8];
+  int partner[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { cs[i] = 1.f; sn[i] = 0.f; partner[i] = c0 + i; }
+  const bool aligned = (half & 7) == 0;                 // the 8 partners are neighbours too
+  bool turned = c0 < rot;
+  if (rot) {
     const int pos = positions[token];
     if (pos < 0 || pos >= n_cos) {
-      if (live && status) *status = BAD_INDEX;
+      turned = false;
+      if (threadIdx.x == 0 && status) *status = BAD_INDEX;
     } else {
-      const float2* cs = cos_sin + (size_t)pos * half;
-      if ((half & 7) == 0) {
-        if (c0 < rot) {
-          const bool upper = c0 >= half;
-          float y[8];
-          load8(src + (upper ? c0 - half : c0 + half), y);
-          const float4* turn = reinterpret_cast<const float4*>(cs + (upper ? c0 - half : c0));
+      const float2* angles = cos_sin + (size_t)pos * half;
+      if (turned && aligned) {
+        const int from = c0 >= half ? c0 - half : c0;
+        const float4* pairs = reinterpret_cast<const float4*>(angles + from);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 t = turn[i];
-            const float a = __fmul_rn(y[2 * i], t.y), b = __fmul_rn(y[2 * i + 1], t.w);
-            const float d = __fmul_rn(x[2 * i], t.x), e = __fmul_rn(x[2 * i + 1], t.z);
-            x[2 * i] = upper ? __fadd_rn(d, a) : __fsub_rn(d, a);
-            x[2 * i + 1] = upper ? __fadd_rn(e, b) : __fsub_rn(e, b);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float4 a = pairs[i];
+          cs[2 * i] = a.x; sn[2 * i] = a.y; cs[2 * i + 1] = a.z; sn[2 * i + 1] = a.w;
         }
-      } else {
+        partner[0] = c0 >= half ? c0 - half : c0 + half;
+      } else if (turned) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int c = c0 + i;
           if (c >= rot) continue;
-          const bool upper = c >= half;
-          const float2 t = cs[upper ? c - half : c];
-          const float y = __fmul_rn(co_to_float<T>(src[upper ? c - half : c + half]), t.y), d = __fmul_rn(x[i], t.x);
-          x[i] = upper ? __fadd_rn(d, y) : __fsub_rn(d, y);
+          partner[i] = c >= half ? c - half : c + half;
+          const float2 a = angles[c >= half ? c - half : c];
+          cs[i] = a.x; sn[i] = a.y;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = co_to_float<T>(co_from_float<T>(x[i]));
     }
   }
-  if (head < nh) {
-    if (live) store8(q_out + (size_t)token * nh * HD + (size_t)head * HD + c0, x);
-  }
-  // The group's range: all four threads take part, whatever their head is.
-  float lo = x[0], hi = x[0];
-  bool finite = true;
+  const int slot = slots[token], page = slot < 0 ? -1 : slot / page_size, in_page = slot - page * page_size, r = in_page & 15;
+  const bool kept = page >= 0 && page < num_pages;      // a negative slot: a row that is not kept
+  if (slot >= 0 && !kept && threadIdx.x == 0 && status) *status = BAD_INDEX;
+
+  for (int h0 = first_head; h0 < heads; h0 += AT_ONCE) {
+    const int head = h0 + place;
+    const bool live = place < AT_ONCE && head < heads;
+    const T* src = row + (size_t)(live ? head : 0) * HD;
+    float x[8];
+    load8(src + c0, x);
+    if (turned && head < nh + nkv) {
+      float y[8];
+      if (aligned) {
+        load8(src + partner[0], y);
+      } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) < INFINITY;
-  }
+        for (int i = 0; i < 8; ++i) y[i] = co_to_float<T>(src[partner[i]]);
+      }
 #pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
-  }
-  if (!live || head < nh) return;
-  const int slot = slots[token];
-  if (slot < 0) return;                           // a row that is not kept
-  const int page = slot / page_size, row = slot - page * page_size;
-  if (page >= num_pages) {
-    if (status) *status = BAD_INDEX;
-    return;
-  }
-  bf16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), m16 = __float2bfloat16_rn(lo);
-  float s = __bfloat162float(s16), m = __bfloat162float(m16);
-  if (!(finite && fabsf(s) < INFINITY && fabsf(m) < INFINITY)) {
-    s16 = m16 = __ushort_as_bfloat16(0x7fff);
-    s = 0.f;
-  }
-  unsigned word = 0;
-  if (s > 0.f) {
+      for (int i = 0; i < 8; ++i) {
+        const float a = __fmul_rn(x[i], cs[i]), b = __fmul_rn(y[i], sn[i]);
+        x[i] = c0 + i < rot ? co_to_float<T>(co_from_float<T>(c0 + i >= half ? __fadd_rn(a, b) : __fsub_rn(a, b))) : x[i];
+      }
+    }
+    if (live && head < nh) store8(q_out + (size_t)token * nh * HD + (size_t)head * HD + c0, x);
+    // The group's range: the four threads of a group take part alike.
+    float lo = x[0], hi = x[0];
+    bool finite = true;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], m), s)), 0.f), 15.f);
-      word |= (unsigned)c << (4 * i);
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+      finite = finite && fabsf(x[i]) < INFINITY;
     }
-  }
-  const int u = piece >> 2, t = piece & 3, r = row & 15;
-  if (head < nh + nkv) {
-    unsigned char* tile = k_cache + tile_at(page, nkv, head - nh, page_size, row);
-    reinterpret_cast<unsigned*>(tile)[r * (4 * NG) + t * NG + u] = word;
-    if (t == 0)
-      reinterpret_cast<unsigned*>(tile + CODES)[r * NG + u] = (unsigned)__bfloat16_as_ushort(s16) | (unsigned)__bfloat16_as_ushort(m16) << 16;
-  } else {
-    unsigned char* tile = v_cache + tile_at(page, nkv, head - nh - nkv, page_size, row);
-    unsigned short* half = reinterpret_cast<unsigned short*>(tile) + ((((u * 8 + 2 * t) * 4 + (r >> 2)) * 2 + ((r >> 1) & 1)) * 2 + (r & 1));
-    half[0] = (unsigned short)word;
-    half[16] = (unsigned short)(word >> 16);      // the next g: four lanes of two words
-    if (t == 0) {
-      bf16* pairs = reinterpret_cast<bf16*>(tile + CODES) + (u * 4 + (r >> 2)) * 8 + (r & 3);
-      pairs[0] = s16;
-      pairs[4] = m16;
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
+    }
+    if (!live || head < nh || !kept) continue;
+    bf16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), m16 = __float2bfloat16_rn(lo);
+    float s = __bfloat162float(s16), m = __bfloat162float(m16);
+    if (!(finite && fabsf(s) < INFINITY && fabsf(m) < INFINITY)) {
+      s16 = m16 = __ushort_as_bfloat16(0x7fff);
+      s = 0.f;
+    }
+    unsigned word = 0;
+    if (s > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], m), s)), 0.f), 15.f);
+        word |= (unsigned)c << (4 * i);
+      }
+    }
+    if (head < nh + nkv) {
+      unsigned char* tile = k_cache + tile_at(page, nkv, head - nh, page_size, in_page);
+      reinterpret_cast<unsigned*>(tile)[r * (4 * NG) + t * NG + u] = word;
+      if (t == 0)
+        reinterpret_cast<unsigned*>(tile + CODES)[r * NG + u] = (unsigned)__bfloat16_as_ushort(s16) | (unsigned)__bfloat16_as_ushort(m16) << 16;
+    } else {
+      unsigned char* tile = v_cache + tile_at(page, nkv, head - nh - nkv, page_size, in_page);
+      unsigned short* dst = reinterpret_cast<unsigned short*>(tile) + ((((u * 8 + 2 * t) * 4 + (r >> 2)) * 2 + ((r >> 1) & 1)) * 2 + (r & 1));
+      dst[0] = (unsigned short)word;
+      dst[16] = (unsigned short)(word >> 16);           // the next g: four lanes of two words
+      if (t == 0) {
+        bf16* pairs = reinterpret_cast<bf16*>(tile + CODES) + (u * 4 + (r >> 2)) * 8 + (r & 3);
+        pairs[0] = s16;
+        pairs[4] = m16;
+      }
     }
   }
 }
@@ -1140,15 +1147,13 @@ CO_EXPORT int coheryn_kv4_write(const void* qkv, long ld, int dtype, const int* 
   if (((uintptr_t)qkv & 15) || ld % align || ((uintptr_t)q_out & 15) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) ||
       ((uintptr_t)cos_sin & 15))
     CO_FAIL("kv4_write: operands must be 16-byte aligned");
-  const int first = rot ? 0 : nh;
-  const long long blocks = ((long long)T * (nh + 2 * nkv - first) * (HD / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) CO_FAIL("kv4_write: %d tokens of %d heads", T, nh + 2 * nkv);
+  const int first = rot ? 0 : nh;        // without a rotation there is nothing to do for the queries
   if (dtype == CO_F32)
-    co_launch(kv4_write_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, (const float*)qkv, ld, positions, (const float2*)cos_sin,
-              n_cos, slots, (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (float*)q_out, T, nh, nkv, rot, page_size, first, status);
+    co_launch(kv4_write_kernel<float>, dim3((unsigned)T), dim3(256), 0, stream, (const float*)qkv, ld, positions, (const float2*)cos_sin, n_cos, slots,
+              (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (float*)q_out, nh, nkv, rot, page_size, first, status);
   else
-    co_launch(kv4_write_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, stream, (const bf16*)qkv, ld, positions, (const float2*)cos_sin,
-              n_cos, slots, (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (bf16*)q_out, T, nh, nkv, rot, page_size, first, status);
+    co_launch(kv4_write_kernel<bf16>, dim3((unsigned)T), dim3(256), 0, stream, (const bf16*)qkv, ld, positions, (const float2*)cos_sin, n_cos, slots,
+              (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (bf16*)q_out, nh, nkv, rot, page_size, first, status);
   CO_CHECK_LAUNCH("kv4_write");
   return 0;
 }

@@ -228,6 +228,53 @@ def host_library() -> ctypes.CDLL:
         return lib
 
 
+def build_calls_module() -> str:
+    """The Python module of calls whose operands are checked in C++ (csrc/host_calls.cpp): compiled against the headers of
+    the interpreter and of torch, whose own libraries it uses."""
+    import torch
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    source = os.path.join(HERE, "host_calls.cpp")
+    h = hashlib.sha256()
+    with open(source, "rb") as fh:
+        h.update(fh.read())
+    h.update(repr((flags, torch.__version__, sys.version_info[:3])).encode())
+    name = f"libcoheryn_b200_calls_{h.hexdigest()[:16]}.so"
+    found = _existing_lib(name)
+    if found:
+        return found
+    out_dir = _lib_dir()
+    target, tmp_target = os.path.join(out_dir, name), os.path.join(out_dir, f".{os.getpid()}_{name}")
+    import sysconfig
+    from torch.utils import cpp_extension
+    includes = list(cpp_extension.include_paths()) + [sysconfig.get_paths()["include"],
+                                                      os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ([host_compiler()] + flags + [x for i in includes for x in ("-isystem", i)] + [source, "-o", tmp_target, f"-L{libs}"]
+           + [f"-l{x}" for x in ("torch_python", "torch_cpu", "c10", "c10_cuda")])
+    print("[coheryn-b200] compiling calls (1 C++ file); this happens once", file=sys.stderr, flush=True)
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise BuildError("the module of checked calls did not compile:\n" + r.stdout)
+    os.replace(tmp_target, target)
+    _drop_stale(out_dir, "libcoheryn_b200_calls_", name)
+    print(f"[coheryn-b200] built {target}", file=sys.stderr, flush=True)
+    return target
+
+
+def calls_module():
+    import importlib.machinery
+    import importlib.util
+    with _lock:
+        module = _loaded.get("calls")
+        if module is None:
+            path = build_calls_module()
+            loader = importlib.machinery.ExtensionFileLoader("coheryn_calls", path)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("coheryn_calls", loader))
+            loader.exec_module(module)
+            _loaded["calls"] = module
+        return module
+
+
 def core_library() -> ctypes.CDLL:
     return load_library("core", CORE_SOURCES)
 
@@ -329,7 +376,7 @@ def maps_attention_library(dk: int, dv: int, maps: int, values_in_keys: bool = F
 
 def build_all(head_dims: Sequence[int] = (16, 32, 64, 128)) -> List[str]:
     """Compile everything ahead of time (no GPU needed)."""
-    paths = [build_host_library(), build_library("core", CORE_SOURCES), build_library("recurrent", RECURRENT_SOURCES),
+    paths = [build_host_library(), build_calls_module(), build_library("core", CORE_SOURCES), build_library("recurrent", RECURRENT_SOURCES),
              build_library("variants", VARIANT_SOURCES), build_library("routed", ROUTED_SOURCES),
              build_library("linear_recurrence", LINEAR_RECURRENCE_SOURCES),
              build_library("linear_attention", LINEAR_ATTENTION_SOURCES), build_library("lightning", LIGHTNING_SOURCES),

@@ -22,7 +22,7 @@
 namespace {
 constexpr int THREADS = 256;
 constexpr int TOKENS_PER_BLOCK = 1024;
-constexpr int TABLE_PER_BLOCK = 4096;   // table entries
+constexpr int TABLE_PER_BLOCK = 2048;   // table entries of one row
 constexpr int MAX_REQUESTS = 12000;     // prefix sums in 48 KB of shared memory
 
 constexpr int BAD_LENGTH = 51;          // status codes
@@ -48,23 +48,20 @@ __device__ __forceinline__ bool list_of(const Lists& l, int b, int& first, int& 
 __global__ void __launch_bounds__(THREADS)
 step_layout_kernel(const int* __restrict__ starts, const int* __restrict__ q_lens, Lists lists, int B, int T, int page_size,
                    int* __restrict__ cu_q, int* __restrict__ kv_lens, int* __restrict__ positions, int* __restrict__ token_req,
-                   int* __restrict__ table, int W, int* __restrict__ slots, int* __restrict__ status, int token_blocks) {
+                   int* __restrict__ table, int W, int* __restrict__ slots, int* __restrict__ status, int token_blocks, int chunks) {
   extern __shared__ int cu[];             // [B + 1], blocks of tokens
   __shared__ int warp_sums[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int bad = 0;
   if ((int)blockIdx.x >= token_blocks) {
-    const long long total = (long long)B * W;
-    const long long e0 = (long long)(blockIdx.x - token_blocks) * TABLE_PER_BLOCK;
-    for (long long e = e0 + tid; e < min(total, e0 + TABLE_PER_BLOCK); e += THREADS) {
-      const int b = (int)(e / W), j = (int)(e - (long long)b * W);
-      int first, from, n;
-      list_of(lists, b, first, from, n);
-      if (j < first) continue;
-      const int i = j - first;
-      if (i < n) table[e] = lists.pages[from + i];
-      else if (!lists.first) table[e] = -1;
-    }
+    // Rows of the table, `chunks` blocks each: the row's list is looked up once.
+    const int x = blockIdx.x - token_blocks, b = x / chunks, j0 = (x - b * chunks) * TABLE_PER_BLOCK;
+    int first, from, n;
+    list_of(lists, b, first, from, n);
+    int* row = table + (long long)b * W;
+    const int end = min(lists.first ? min(W, first + n) : W, j0 + TABLE_PER_BLOCK);
+#pragma unroll 4
+    for (int j = max(j0, first) + tid; j < end; j += THREADS) row[j] = j - first < n ? lists.pages[from + j - first] : -1;
     return;
   }
   // Prefix sums of the lengths: THREADS at a time, a warp scan and the warps' totals before it.
@@ -144,10 +141,11 @@ CO_EXPORT int coheryn_step_layout(const int* starts, const int* q_lens, const in
   if (page_size < 1 || W < 1 || T < 0 || n_pages < 0) CO_FAIL("step_layout: page size %d, table width %d, %d tokens", page_size, W, T);
   const Lists lists{pages, page_cu, first, n_pages};
   const int token_blocks = T > TOKENS_PER_BLOCK ? (T + TOKENS_PER_BLOCK - 1) / TOKENS_PER_BLOCK : 1;
-  const long long table_blocks = ((long long)B * W + TABLE_PER_BLOCK - 1) / TABLE_PER_BLOCK;
+  const int chunks = (W - 1) / TABLE_PER_BLOCK + 1;
+  const long long table_blocks = (long long)B * chunks;
   if (token_blocks + table_blocks > 0x7fffffffLL) CO_FAIL("step_layout: a table of %d x %d entries", B, W);
   step_layout_kernel<<<dim3((unsigned)(token_blocks + table_blocks)), dim3(THREADS), sizeof(int) * (size_t)(B + 1), stream>>>(
-      starts, q_lens, lists, B, T, page_size, cu_q, kv_lens, positions, token_req, table, W, slots, status, token_blocks);
+      starts, q_lens, lists, B, T, page_size, cu_q, kv_lens, positions, token_req, table, W, slots, status, token_blocks, chunks);
   CO_CHECK_LAUNCH("step_layout");
   return 0;
 }

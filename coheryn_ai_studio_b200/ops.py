@@ -2133,11 +2133,10 @@ def lightning_attention(q, k, v, gate, powers: torch.Tensor, silu: bool, state: 
 
 def _here(*tensors) -> int:
     """The current device, where all of ``tensors`` (None aside) have to live; the launches go to its current stream."""
+    _dev(*tensors)
     device = _current_device() if _current_device is not None else torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != device:
-            if not t.is_cuda:
-                raise KernelError("kernel operands must be CUDA tensors")
             raise KernelError(f"an operand lives on cuda:{t.get_device()}, but the current device is cuda:{device}")
     return device
 
@@ -2175,6 +2174,29 @@ def _entry(lib, name: str, types: str):
     return fn
 
 
+_addresses = {}
+
+
+def _address(lib, name: str) -> int:
+    """Where a function of a library begins."""
+    at = _addresses.get((lib, name))
+    if at is None:
+        at = _addresses[(lib, name)] = ctypes.cast(getattr(lib, name), c_void_p).value
+    return at
+
+
+_calls_module = None
+
+
+def _calls():
+    """The module whose functions check the operands in C++ and enter the library; each returns None for a call that is not
+    its ordinary one, which the code below then handles or refuses by name."""
+    global _calls_module
+    if _calls_module is None:
+        _calls_module = build.calls_module()
+    return _calls_module
+
+
 def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tensor, pages: torch.Tensor, page_size: int,
                 block_table: torch.Tensor, slots: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
                 kv_lens: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -2193,6 +2215,14 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
 
     An ordinary launch: the arrays are complete before the next kernel in the stream begins, so kernels that look at a
     step's lengths ahead of their wait may follow it directly."""
+    if starts.is_cuda:
+        lib = core()
+        rc = _calls().layout(_address(lib, "coheryn_step_layout"), starts, q_lens, page_cu, pages, page_size, block_table, slots, cu_q, kv_lens,
+                             positions, token_req, first, status)
+        if rc == 0:
+            return
+        if rc is not None:
+            _check(lib, rc)
     device = _here(starts, q_lens, page_cu, pages, block_table, slots, cu_q, kv_lens, positions, token_req, first, status)
     B = starts.numel()
     _words(B, starts=starts, q_lens=q_lens, kv_lens=kv_lens, first=first)
@@ -2256,12 +2286,11 @@ def kv4_page_shape(num_kv_heads: int, page_size: int, head_dim: int):
 
 
 def _kv4_caches(k_cache, v_cache, num_kv_heads: int, page_size: int, head_dim: int) -> None:
-    shape = kv4_page_shape(num_kv_heads, page_size, head_dim)
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype is not torch.uint8 or t.dim() != 4 or t.shape[1:] != shape or not t.is_contiguous():
-            raise KernelError(f"{name} must be contiguous uint8 pages of shape {shape}, not {t.dtype} {tuple(t.shape)}")
-    if k_cache.shape[0] != v_cache.shape[0]:
-        raise KernelError("the key and the value cache have different numbers of pages")
+    shape, k_shape = kv4_page_shape(num_kv_heads, page_size, head_dim), k_cache.shape
+    if (k_shape != v_cache.shape or k_shape[1:] != shape or k_cache.dtype is not torch.uint8 or v_cache.dtype is not torch.uint8
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise KernelError(f"the caches must be contiguous uint8 pages of shape {shape}, as many of keys as of values, not {k_cache.dtype} "
+                          f"{tuple(k_shape)} and {v_cache.dtype} {tuple(v_cache.shape)}")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2278,6 +2307,14 @@ def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin
     ``cos_sin`` may then be None).  Keys are rounded to the compute type before they are quantised.  A group of 32
     channels with a value that is not finite is kept as not-a-number.  Two rows with one slot: one of them is kept, or a
     mixture."""
+    if qkv.is_cuda:
+        lib = kv4_lib(head_dim)
+        q = _calls().write(_address(lib, "coheryn_kv4_write"), qkv, positions, cos_sin, slots, k_cache, v_cache, num_heads, num_kv_heads, head_dim,
+                           rotary_dim, page_size, tc_status(qkv.device))
+        if q is not None:
+            if type(q) is int:
+                _check(lib, q)
+            return q
     device = _here(qkv, positions, cos_sin, slots, k_cache, v_cache)
     T = qkv.shape[0]
     _words(T, slots=slots)
@@ -2292,7 +2329,7 @@ def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin
         _words(T, positions=positions)
         if cos_sin.dtype is not torch.float32 or not cos_sin.is_contiguous() or cos_sin.shape[1:] != (rotary_dim // 2, 2):
             raise KernelError(f"rope_kv4_write: cos_sin must be float32 [positions, {rotary_dim // 2}, 2]")
-        q = torch.empty((T, nq), dtype=qkv.dtype, device=qkv.device)
+        q = qkv.new_empty((T, nq))
     else:
         q = qkv[:, :nq]
     lib = kv4_lib(head_dim)
@@ -2308,16 +2345,22 @@ def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin
 def kv4_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor, head_dim: int, page_size: int, dtype: torch.dtype):
     """Pages of a 4-bit cache as the values they stand for: (keys, values), each [n, kv heads, page_size, head_dim] in
     ``dtype``.  A page number outside the cache reads as zeros."""
+    code = _CODES.get(dtype)
+    if k_cache.is_cuda and code is not None:
+        lib = kv4_lib(head_dim)
+        both = _calls().pages(_address(lib, "coheryn_kv4_pages"), k_cache, v_cache, pages, head_dim, page_size, code, tc_status(k_cache.device))
+        if both is not None:
+            if type(both) is int:
+                _check(lib, both)
+            return both
     device = _here(k_cache, v_cache, pages)
     _words(None, pages=pages)
     nkv = k_cache.shape[1]
     _kv4_caches(k_cache, v_cache, nkv, page_size, head_dim)
-    code = _CODES.get(dtype)
     if code is None:
         raise KernelError(f"dtype {dtype} is not handled by the kernels")
     n = pages.numel()
-    k = torch.empty((n, nkv, page_size, head_dim), dtype=dtype, device=k_cache.device)
-    v = torch.empty_like(k)
+    k, v = k_cache.new_empty((2, n, nkv, page_size, head_dim), dtype=dtype).unbind(0)
     lib = kv4_lib(head_dim)
     rc = _entry(lib, "coheryn_kv4_pages", "ppiiipippipp")(
         k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], nkv, page_size, pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
@@ -2343,6 +2386,16 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``KV4_DIRECT_ROWS`` rows per kv
     head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to bfloat16 and
     go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
+    if not force_simple and q.is_cuda:
+        lib = kv4_lib(head_dim)
+        rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
+                                _address(lib, "coheryn_kv4_attention_simple"), q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads,
+                                num_kv_heads, head_dim, page_size, window, scale, cu_q, kv_lens, q_lens, max_kv_len, KV4_DIRECT_ROWS,
+                                tc_status(q.device))
+        if rc == 0:
+            return
+        if rc is not None:
+            _check(lib, rc)
     device = _here(q, out, k_cache, v_cache, block_tables, token_req, positions, cu_q, kv_lens)
     _kv4_caches(k_cache, v_cache, num_kv_heads, page_size, head_dim)
     _words(None, block_tables=block_tables)
