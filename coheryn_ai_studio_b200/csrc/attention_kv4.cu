@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tc_common.cuh"
 
 #ifndef CO_HEAD_DIM
@@ -45,15 +47,18 @@ __device__ __forceinline__ size_t tile_at(long long page, int nkv, int kvh, int 
 }
 
 // ------------------------------------------------------------------------------------
-// Rotation and write.  A thread has 8 neighbouring channels of a head; the four threads of a group agree on its minimum and
-// maximum by two shuffles.  Queries are rotated into their own rows; keys are rotated and rounded to the compute type, as
-// a cache in that type would hold them, and then quantised, values quantised as they are.  Every product and sum of the
-// rotation is rounded by itself (no fused multiply-add): the codes are then the same function of the inputs wherever it is
-// computed.
+// Rotation and write.  Queries are rotated into their own rows; keys are rotated and rounded to the compute type, as a cache in
+// that type would hold them, and then quantised, values quantised as they are.  Every product and sum of the rotation is rounded
+// by itself (no fused multiply-add): the codes are then the same function of the inputs wherever it is computed.
+// Quotients are estimated by one reciprocal; only an estimate that lies within 2^-14 of a border between two codes is divided
+// out, so that the code is that of the division.
 //
-// A block has one token, so that its position, slot and angles are looked up once for all heads (a thread per 8 channels of
-// any token and head, with its own angles and divisions: 2,048 tokens of 28 + 8 heads of 128 in 22 us).  Bound by the bytes of
-// a prompt (19 MB read, 17 MB written there) and by one launch at decoding.
+// A thread has 4 neighbouring channels of each half of a head, which turn together: every element is read once, and the
+// angles that a thread reads lie together with its neighbours' (8 neighbouring channels per thread, their partners read a
+// second time and angles 64 bytes apart from lane to lane, took 20 us instead of 8 for 2,048 tokens of 28 + 8 heads of 128:
+// the loads' wavefronts bound it).  The eight threads of a group agree on its minimum and maximum by three shuffles.  Heads
+// that turn another number of channels, or whose halves are not whole groups, go to the kernel after it.  Bound by
+// the bytes of a prompt (19 MB read, 17 MB written there) and by one launch at decoding.
 // ------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
@@ -82,133 +87,17 @@ __device__ __forceinline__ void store8<bf16>(bf16* p, const float (&x)[8]) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
-kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
-                 const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
-                 T* __restrict__ q_out, int nh, int nkv, int rot, int page_size, int first_head, int* __restrict__ status) {
-  constexpr int TPH = HD / 8, AT_ONCE = 256 / TPH;      // threads of a head, heads at a time
-  co_pdl_launch_dependents();
-  const int token = blockIdx.x, place = threadIdx.x / TPH, piece = threadIdx.x % TPH;
-  const int c0 = piece * 8, half = rot >> 1, heads = nh + 2 * nkv;
-  const int u = piece >> 2, t = piece & 3;
-  co_pdl_wait();
-  const T* row = qkv + (size_t)token * ld;
-  // The token's angles for these channels: x cos -+ partner sin, the partner half a rotation away.
-  float cs[8], sn[8];
-  int partner[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { cs[i] = 1.f; sn[i] = 0.f; partner[i] = c0 + i; }
-  const bool aligned = (half & 7) == 0;                 // the 8 partners are neighbours too
-  bool turned = c0 < rot;
-  if (rot) {
-    const int pos = positions[token];
-    if (pos < 0 || pos >= n_cos) {
-      turned = false;
-      if (threadIdx.x == 0 && status) *status = BAD_INDEX;
-    } else {
-      const float2* angles = cos_sin + (size_t)pos * half;
-      if (turned && aligned) {
-        const int from = c0 >= half ? c0 - half : c0;
-        const float4* pairs = reinterpret_cast<const float4*>(angles + from);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 a = pairs[i];
-          cs[2 * i] = a.x; sn[2 * i] = a.y; cs[2 * i + 1] = a.z; sn[2 * i + 1] = a.w;
-        }
-        partner[0] = c0 >= half ? c0 - half : c0 + half;
-      } else if (turned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = c0 + i;
-          if (c >= rot) continue;
-          partner[i] = c >= half ? c - half : c + half;
-          const float2 a = angles[c >= half ? c - half : c];
-          cs[i] = a.x; sn[i] = a.y;
-        }
-      }
-    }
-  }
-  const int slot = slots[token], page = slot < 0 ? -1 : slot / page_size, in_page = slot - page * page_size, r = in_page & 15;
-  const bool kept = page >= 0 && page < num_pages;      // a negative slot: a row that is not kept
-  if (slot >= 0 && !kept && threadIdx.x == 0 && status) *status = BAD_INDEX;
-
-  for (int h0 = first_head; h0 < heads; h0 += AT_ONCE) {
-    const int head = h0 + place;
-    const bool live = place < AT_ONCE && head < heads;
-    const T* src = row + (size_t)(live ? head : 0) * HD;
-    float x[8];
-    load8(src + c0, x);
-    if (turned && head < nh + nkv) {
-      float y[8];
-      if (aligned) {
-        load8(src + partner[0], y);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = co_to_float<T>(src[partner[i]]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = __fmul_rn(x[i], cs[i]), b = __fmul_rn(y[i], sn[i]);
-        x[i] = c0 + i < rot ? co_to_float<T>(co_from_float<T>(c0 + i >= half ? __fadd_rn(a, b) : __fsub_rn(a, b))) : x[i];
-      }
-    }
-    if (live && head < nh) store8(q_out + (size_t)token * nh * HD + (size_t)head * HD + c0, x);
-    // The group's range: the four threads of a group take part alike.
-    float lo = x[0], hi = x[0];
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      finite = finite && fabsf(x[i]) < INFINITY;
-    }
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
-    }
-    if (!live || head < nh || !kept) continue;
-    bf16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), m16 = __float2bfloat16_rn(lo);
-    float s = __bfloat162float(s16), m = __bfloat162float(m16);
-    if (!(finite && fabsf(s) < INFINITY && fabsf(m) < INFINITY)) {
-      s16 = m16 = __ushort_as_bfloat16(0x7fff);
-      s = 0.f;
-    }
-    unsigned word = 0;
-    if (s > 0.f) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], m), s)), 0.f), 15.f);
-        word |= (unsigned)c << (4 * i);
-      }
-    }
-    if (head < nh + nkv) {
-      unsigned char* tile = k_cache + tile_at(page, nkv, head - nh, page_size, in_page);
-      reinterpret_cast<unsigned*>(tile)[r * (4 * NG) + t * NG + u] = word;
-      if (t == 0)
-        reinterpret_cast<unsigned*>(tile + CODES)[r * NG + u] = (unsigned)__bfloat16_as_ushort(s16) | (unsigned)__bfloat16_as_ushort(m16) << 16;
-    } else {
-      unsigned char* tile = v_cache + tile_at(page, nkv, head - nh - nkv, page_size, in_page);
-      unsigned short* dst = reinterpret_cast<unsigned short*>(tile) + ((((u * 8 + 2 * t) * 4 + (r >> 2)) * 2 + ((r >> 1) & 1)) * 2 + (r & 1));
-      dst[0] = (unsigned short)word;
-      dst[16] = (unsigned short)(word >> 16);           // the next g: four lanes of two words
-      if (t == 0) {
-        bf16* pairs = reinterpret_cast<bf16*>(tile + CODES) + (u * 4 + (r >> 2)) * 8 + (r & 3);
-        pairs[0] = s16;
-        pairs[4] = m16;
-      }
-    }
-  }
+__device__ __forceinline__ void load4(const T* p, float (&x)[4]);
+template <>
+__device__ __forceinline__ void load4<float>(const float* p, float (&x)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
 }
-
-// ------------------------------------------------------------------------------------
-// Pages as values: [entry, kv head, page_size, HD] in float32 or bfloat16.  One block per (page, kv head).
-// With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length are
-// zeros, entries that lie wholly behind it or in front of the window of its first new token are left out, and
-// `out_table` gets the entry's place among the output pages, or -1.
-// Bound by the bytes written (16 of 21 bits a value).
-// ------------------------------------------------------------------------------------
+template <>
+__device__ __forceinline__ void load4<bf16>(const bf16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = lo_bf16(v.x); x[1] = hi_bf16(v.x); x[2] = lo_bf16(v.y); x[3] = hi_bf16(v.y);
+}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
 template <>
@@ -219,7 +108,190 @@ template <>
 __device__ __forceinline__ void store4<bf16>(bf16* p, float a, float b, float c, float d) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack(a, b), pack(c, d));
 }
+// N values rounded to the compute type.
+template <int N>
+__device__ __forceinline__ void rounded(float (&)[N], const float*) {}
+template <int N>
+__device__ __forceinline__ void rounded(float (&x)[N], const bf16*) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const unsigned w = pack(x[i], x[i + 1]);
+    x[i] = lo_bf16(w);
+    x[i + 1] = hi_bf16(w);
+  }
+}
+// The pair (scale low half, minimum high half) of a group and the codes of this thread's N values of it, the first lowest.  The group's
+// threads are neighbours, THREADS of them, and come here together.
+template <int THREADS, int N>
+__device__ __forceinline__ uint2 quantised(const float (&x)[N]) {
+  float lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    finite = finite && fabsf(x[i]) < INFINITY;
+  }
+  const unsigned group = ((1u << THREADS) - 1) << (threadIdx.x & 31 & ~(THREADS - 1));
+#pragma unroll
+  for (int o = 1; o < THREADS; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(group, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
+  }
+  finite = __all_sync(group, finite);
+  bf16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), m16 = __float2bfloat16_rn(lo);
+  float s = __bfloat162float(s16), m = __bfloat162float(m16);
+  if (!(finite && fabsf(s) < INFINITY && fabsf(m) < INFINITY)) {
+    s16 = m16 = __ushort_as_bfloat16(0x7fff);
+    s = 0.f;
+  }
+  unsigned codes = 0;
+  if (s > 0.f) {
+    const float inverse = 1.f / s;
+    const bool usual = inverse < 1e37f;                 // (a subnormal scale has no reciprocal)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = __fsub_rn(x[i], m);
+      float c = d * inverse;
+      if (!usual || fabsf(c - floorf(c) - 0.5f) < 6.1e-5f) c = __fdiv_rn(d, s);
+      codes |= (unsigned)fminf(fmaxf(rintf(c), 0.f), 15.f) << (4 * i);
+    }
+  }
+  return make_uint2((unsigned)__bfloat16_as_ushort(s16) | (unsigned)__bfloat16_as_ushort(m16) << 16, codes);
+}
+// Where the codes of channels 32 u + 4 i + 0..3 of row r lie in a key and in a value tile, in 16 bits; and the pairs.
+__device__ __forceinline__ unsigned short* key_codes(unsigned char* tile, int r, int u, int i) {
+  return reinterpret_cast<unsigned short*>(tile) + 2 * (r * (4 * NG) + (i >> 1) * NG + u) + (i & 1);
+}
+__device__ __forceinline__ unsigned short* value_codes(unsigned char* tile, int r, int u, int i) {
+  return reinterpret_cast<unsigned short*>(tile) + 2 * (((u * 8 + i) * 4 + (r >> 2)) * 2 + ((r >> 1) & 1)) + (r & 1);
+}
+__device__ __forceinline__ void put_pair(unsigned char* tile, bool values, int r, int u, unsigned pair) {
+  if (values) {
+    unsigned short* at = reinterpret_cast<unsigned short*>(tile + CODES) + (u * 4 + (r >> 2)) * 8 + (r & 3);
+    at[0] = (unsigned short)pair;
+    at[4] = (unsigned short)(pair >> 16);
+  } else {
+    reinterpret_cast<unsigned*>(tile + CODES)[r * NG + u] = pair;
+  }
+}
 
+// Rotations of whole heads (TURN) and no rotation, heads whose halves are whole groups.
+template <typename T, bool TURN>
+__global__ void __launch_bounds__(256)
+kv4_write_halves_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
+                        const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
+                        T* __restrict__ q_out, int nh, int nkv, int page_size, int first_head, int* __restrict__ status) {
+  constexpr int TPH = HD / 8, AT_ONCE = 256 / TPH, HALF = HD / 2;      // threads of a head, heads of a block
+  co_pdl_launch_dependents();
+  const int place = threadIdx.x / TPH, piece = threadIdx.x % TPH, head = first_head + blockIdx.y * AT_ONCE + place;
+  if (place >= AT_ONCE || head >= nh + 2 * nkv) return;
+  const int token = blockIdx.x, c0 = piece * 4;
+  co_pdl_wait();
+  const T* src = qkv + (size_t)token * ld + (size_t)head * HD + c0;
+  float x[2][4];
+  load4(src, x[0]);
+  load4(src + HALF, x[1]);
+  const bool values = head >= nh + nkv;
+  const int slot = head >= nh ? slots[token] : 0;
+  if (TURN && !values) {
+    const int pos = positions[token];
+    if (pos < 0 || pos >= n_cos) {
+      if (status) *status = BAD_INDEX;
+    } else {
+      const float4* turn = reinterpret_cast<const float4*>(cos_sin + (size_t)pos * HALF + c0);
+      const float4 a = turn[0], b = turn[1];
+      const float cs[4] = {a.x, a.z, b.x, b.z}, sn[4] = {a.y, a.w, b.y, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float l = __fsub_rn(__fmul_rn(x[0][i], cs[i]), __fmul_rn(x[1][i], sn[i]));
+        x[1][i] = __fadd_rn(__fmul_rn(x[1][i], cs[i]), __fmul_rn(x[0][i], sn[i]));
+        x[0][i] = l;
+      }
+    }
+  }
+  if (head < nh) {
+    T* dst = q_out + (size_t)token * nh * HD + (size_t)head * HD + c0;
+    store4(dst, x[0][0], x[0][1], x[0][2], x[0][3]);
+    store4(dst + HALF, x[1][0], x[1][1], x[1][2], x[1][3]);
+    return;
+  }
+  if (slot < 0) return;                                 // a row that is not kept
+  const int page = slot / page_size, row = slot - page * page_size, r = row & 15;
+  if (page >= num_pages) {
+    if (status) *status = BAD_INDEX;
+    return;
+  }
+  unsigned char* tile = (values ? v_cache : k_cache) + tile_at(page, nkv, head - nh - (values ? nkv : 0), page_size, row);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int u = (h * HALF + c0) / 32, i = piece & 7;
+    rounded(x[h], (const T*)nullptr);
+    const uint2 q = quantised<8>(x[h]);
+    *(values ? value_codes(tile, r, u, i) : key_codes(tile, r, u, i)) = (unsigned short)q.y;
+    if (i == 0) put_pair(tile, values, r, u, q.x);
+  }
+}
+
+// Any even number of turned channels, any head: a thread has 8 neighbouring channels.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
+                 const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
+                 T* __restrict__ q_out, int nh, int nkv, int rot, int page_size, int first_head, int* __restrict__ status) {
+  constexpr int TPH = HD / 8, AT_ONCE = 256 / TPH;
+  co_pdl_launch_dependents();
+  const int place = threadIdx.x / TPH, piece = threadIdx.x % TPH, head = first_head + blockIdx.y * AT_ONCE + place;
+  if (place >= AT_ONCE || head >= nh + 2 * nkv) return;
+  const int token = blockIdx.x, c0 = piece * 8, half = rot >> 1;
+  co_pdl_wait();
+  const T* src = qkv + (size_t)token * ld + (size_t)head * HD;
+  float x[8];
+  load8(src + c0, x);
+  const bool values = head >= nh + nkv;
+  if (c0 < rot && !values) {
+    const int pos = positions[token];
+    if (pos < 0 || pos >= n_cos) {
+      if (status) *status = BAD_INDEX;
+    } else {
+      const float2* angles = cos_sin + (size_t)pos * half;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + i;
+        if (c >= rot) continue;
+        const bool upper = c >= half;
+        const float2 a = angles[upper ? c - half : c];
+        x[i] = __fadd_rn(__fmul_rn(x[i], a.x), __fmul_rn(co_to_float<T>(src[upper ? c - half : c + half]), upper ? a.y : -a.y));
+      }
+    }
+  }
+  if (head < nh) {
+    store8(q_out + (size_t)token * nh * HD + (size_t)head * HD + c0, x);
+    return;
+  }
+  const int slot = slots[token];
+  if (slot < 0) return;
+  const int page = slot / page_size, row = slot - page * page_size, r = row & 15, u = piece >> 2, t = piece & 3;
+  if (page >= num_pages) {
+    if (status) *status = BAD_INDEX;
+    return;
+  }
+  unsigned char* tile = (values ? v_cache : k_cache) + tile_at(page, nkv, head - nh - (values ? nkv : 0), page_size, row);
+  rounded(x, (const T*)nullptr);
+  const uint2 q = quantised<4>(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *(values ? value_codes(tile, r, u, 2 * t + i) : key_codes(tile, r, u, 2 * t + i)) = (unsigned short)(q.y >> (16 * i));
+  if (t == 0) put_pair(tile, values, r, u, q.x);
+}
+
+// ------------------------------------------------------------------------------------
+// Pages as values: [entry, kv head, page_size, HD] in float32 or bfloat16.  One block per (page, kv head).
+// With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length are
+// zeros, entries that lie wholly behind it or in front of the window of its first new token are left out, and
+// `out_table` gets the entry's place among the output pages, or -1.
+// Bound by the bytes written (16 of 21 bits a value).
+// ------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(128)
 kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
@@ -1148,12 +1220,22 @@ CO_EXPORT int coheryn_kv4_write(const void* qkv, long ld, int dtype, const int* 
       ((uintptr_t)cos_sin & 15))
     CO_FAIL("kv4_write: operands must be 16-byte aligned");
   const int first = rot ? 0 : nh;        // without a rotation there is nothing to do for the queries
-  if (dtype == CO_F32)
-    co_launch(kv4_write_kernel<float>, dim3((unsigned)T), dim3(256), 0, stream, (const float*)qkv, ld, positions, (const float2*)cos_sin, n_cos, slots,
-              (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (float*)q_out, nh, nkv, rot, page_size, first, status);
-  else
-    co_launch(kv4_write_kernel<bf16>, dim3((unsigned)T), dim3(256), 0, stream, (const bf16*)qkv, ld, positions, (const float2*)cos_sin, n_cos, slots,
-              (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (bf16*)q_out, nh, nkv, rot, page_size, first, status);
+  const int at_once = 256 / (HD / 8), rounds = (nh + 2 * nkv - first + at_once - 1) / at_once;
+  if (rounds > 65535) CO_FAIL("kv4_write: %d heads", nh + 2 * nkv);
+  const dim3 grid((unsigned)T, (unsigned)rounds);
+  auto with = [&](auto* x) {
+    typedef decltype(x) P;
+    typedef std::remove_pointer_t<P> E;
+    if (HD % 64 == 0 && (rot == HD || rot == 0))
+      co_launch(rot ? kv4_write_halves_kernel<E, true> : kv4_write_halves_kernel<E, false>, grid, dim3(256), 0, stream, (P)qkv, ld, positions,
+                (const float2*)cos_sin, n_cos, slots, (unsigned char*)k_cache, (unsigned char*)v_cache, num_pages, (P)q_out, nh, nkv, page_size, first,
+                status);
+    else
+      co_launch(kv4_write_kernel<E>, grid, dim3(256), 0, stream, (P)qkv, ld, positions, (const float2*)cos_sin, n_cos, slots, (unsigned char*)k_cache,
+                (unsigned char*)v_cache, num_pages, (P)q_out, nh, nkv, rot, page_size, first, status);
+  };
+  if (dtype == CO_F32) with((float*)nullptr);
+  else with((bf16*)nullptr);
   CO_CHECK_LAUNCH("kv4_write");
   return 0;
 }
