@@ -178,7 +178,7 @@ __device__ __forceinline__ void put_pair(unsigned char* tile, bool values, int r
 
 // Rotations of whole heads (TURN) and no rotation, heads whose halves are whole groups.
 template <typename T, bool TURN>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 8)
 kv4_write_halves_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ positions, const float2* __restrict__ cos_sin, int n_cos,
                         const int* __restrict__ slots, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, int num_pages,
                         T* __restrict__ q_out, int nh, int nkv, int page_size, int first_head, int* __restrict__ status) {
