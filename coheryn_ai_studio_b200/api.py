@@ -17,7 +17,7 @@ _BIN = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 def run(model: str, prompt: Optional[str] = None, tokens: Optional[Sequence[int]] = None,
         max_tokens: int = 128, context: int = 4096, temperature: float = 0.0, top_k: int = 0,
         top_p: float = 1.0, seed: int = 0, stop_tokens: Sequence[int] = (), dtype: str = "bfloat16",
-        timeout: Optional[float] = None) -> Dict:
+        timeout: Optional[float] = None, kv_bits: Optional[int] = None) -> Dict:
     """Spawn ``coheryn --json run MODEL ...`` and return its result object.  Raises
     RuntimeError carrying the program's JSON error on a non-zero exit."""
     cmd = [sys.executable, _BIN, "--json", "run", model, "--max-tokens", str(max_tokens), "--context",
@@ -27,6 +27,8 @@ def run(model: str, prompt: Optional[str] = None, tokens: Optional[Sequence[int]
         cmd += ["--prompt", prompt]
     if tokens is not None:
         cmd += ["--tokens", ",".join(str(int(t)) for t in tokens)]
+    if kv_bits is not None:
+        cmd += ["--kv-bits", str(kv_bits)]
     for t in stop_tokens:
         cmd += ["--stop-token", str(int(t))]
     p = subprocess.run(cmd, capture_output=True, text=True, timeout=timeout)

@@ -28,6 +28,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .. import ops
 from ..parts.base import FixedState, LayerCache, PagedKV
 from .pages import CacheError, PagePool, SlotPool, host
 
@@ -68,9 +69,16 @@ def _ints(values: Sequence[int]):
 class CacheManager:
     def __init__(self, requirements: Sequence, cache_from: Sequence[Optional[int]], dtype: torch.dtype,
                  device, page_size: int = 16, num_pages: int = 0, max_requests: int = 64,
-                 prefix_reuse: bool = True):
+                 prefix_reuse: bool = True, kv_bits: Optional[int] = None):
+        """``kv_bits`` = 4 keeps keys and values in 4 bits (5 with their scales) in the place of ``dtype``; every mixer has to be
+        able to read such pages (``PagedKV.four_bits``)."""
         if page_size < 1:
             raise ValueError("page_size must be positive")
+        if kv_bits not in (None, 4):
+            raise ValueError(f"a cache keeps keys and values in the compute type or in 4 bits, not in {kv_bits}")
+        if kv_bits == 4 and page_size % 16:
+            raise ValueError(f"a cache in 4 bits takes pages of a multiple of 16 positions, not {page_size}")
+        self.kv_bits = kv_bits
         self.page_size, self.num_pages, self.max_requests = page_size, num_pages, max_requests
         self.dtype, self.device = dtype, device
         self.groups: List[_Group] = []
@@ -89,6 +97,10 @@ class CacheManager:
             self._needs.append((several, len(need) if several else 1))
             for c, one in enumerate(need if several else (need,)):
                 if isinstance(one, PagedKV):
+                    if kv_bits == 4 and not (one.four_bits and one.head_dim % 32 == 0 and 32 <= one.head_dim <= 256
+                                             and one.value_dim == one.head_dim and one.stride == 1 and not one.keep_first):
+                        raise ValueError(f"schedule entry {e}: its attention does not read a cache in 4 bits ({one.head_dim} key and "
+                                         f"{one.value_dim} value channels; built for plain attention with head sizes 32..256 in steps of 32)")
                     for gi, g in enumerate(self.groups):
                         if g.need == one:
                             self._entry_group[(e, c)] = (gi, len(g.entries))
@@ -111,7 +123,13 @@ class CacheManager:
             if n.stride < 1 or (n.stride > 1 and n.window is not None):
                 raise ValueError("rows that stand for blocks of positions need a positive stride and take no window")
             rows_pp = n.rows_per_page(self.page_size)      # rows of a page of this group (the books count positions)
-            if n.v_head_dim == 0:
+            if kv_bits == 4:
+                # codes and scales of zeros: every row stands for zeros
+                g.tensor = torch.zeros((len(g.entries), 2, num_pages + 1) + ops.kv4_page_shape(n.num_kv_heads, page_size, n.head_dim),
+                                       dtype=torch.uint8, device=device)
+                g.k = [g.tensor[i, 0] for i in range(len(g.entries))]
+                g.v = [g.tensor[i, 1] for i in range(len(g.entries))]
+            elif n.v_head_dim == 0:
                 # no value rows: the mixer reads its values out of the key rows
                 g.tensor = torch.zeros((len(g.entries), 1, num_pages + 1, n.num_kv_heads, rows_pp, n.head_dim),
                                        dtype=dtype, device=device)
@@ -163,7 +181,8 @@ class CacheManager:
         if (owner, c) in self._entry_group:
             gi, idx = self._entry_group[(owner, c)]
             g = self.groups[gi]
-            return LayerCache(kind="paged", group=gi, page_size=self.page_size, k=g.k[idx], v=g.v[idx], writes=writes)
+            return LayerCache(kind="paged", group=gi, page_size=self.page_size, k=g.k[idx], v=g.v[idx], writes=writes,
+                              four_bits=self.kv_bits == 4)
         return None
 
     def layer_caches(self) -> List[Optional[LayerCache]]:
@@ -196,6 +215,8 @@ class CacheManager:
         return list(self._state.values())
 
     def bytes_per_token(self) -> int:
+        if self.kv_bits == 4:       # 4 bits a channel, and 32 for the scale and the minimum of 32
+            return sum(len(g.entries) * g.need.num_kv_heads * 2 * g.need.head_dim * 5 // 8 for g in self.groups)
         item = torch.empty((), dtype=self.dtype).element_size()
         return sum(-(-len(g.entries) * g.need.num_kv_heads * (g.need.head_dim + g.need.value_dim) * item // g.need.stride)
                    for g in self.groups)

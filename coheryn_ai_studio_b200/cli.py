@@ -4,7 +4,7 @@
     coheryn run MODEL --prompt TEXT | --tokens 1,2,3 [--max-tokens 128] [--context 4096]
                 [--stream] [--temperature 0] [--top-k 0] [--top-p 1] [--seed 0]
                 [--stop-token ID]... [--repetition-penalty 1] [--frequency-penalty 0]
-                [--presence-penalty 0] [--dtype bfloat16|float32] [--json]
+                [--presence-penalty 0] [--dtype bfloat16|float32] [--kv-bits 4] [--json]
     coheryn trace MODEL --tokens 1,2,3          teacher-forced layer outputs and logits as JSON Lines
     coheryn init DIR|FILE.gguf --config CONFIG.json --seed N [--store bfloat16|float32]
     coheryn models inspect MODEL
@@ -72,6 +72,7 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--presence-penalty", type=float, default=0.0)
     run.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     run.add_argument("--page-size", type=int, default=16)
+    run.add_argument("--kv-bits", type=int, choices=[4], default=None, help="keep keys and values in 4 bits")
     run.add_argument("--max-batched-tokens", type=int, default=2048)
     run.add_argument("--device", default="cuda:0")
 
@@ -121,7 +122,7 @@ def cmd_run(args) -> int:
         params.validate()
         engine = Engine.from_folder(args.model, args.dtype, args.device, context=args.context,
                                     max_num_seqs=1, max_num_batched_tokens=args.max_batched_tokens,
-                                    page_size=args.page_size, kv_cache_tokens=args.context)
+                                    page_size=args.page_size, kv_cache_tokens=args.context, kv_bits=args.kv_bits)
     except (ValueError, RequestRefused) as e:
         raise CliError("invalid_request", str(e), 2) from None
     streamed: List[int] = []

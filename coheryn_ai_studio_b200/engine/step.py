@@ -297,7 +297,66 @@ class StepRunner:
                 return [out[b, :lens[b]] for b in range(B)]
             width = longest
 
+    def _step_arrays(self, starts, q_lens, tables, extra: Sequence[np.ndarray]):
+        """A step's index arrays made on the device (ops.step_layout) from lengths and page lists, which leave the host in one
+        copy together with ``extra``: (StepContext fields, the extra arrays on the device).  ``tables``: per group, per
+        request the page ids."""
+        B, T = len(starts), int(np.sum(q_lens))
+        parts = [starts, q_lens]
+        for lists in tables:
+            counts = [len(l) for l in lists]
+            parts += [np.concatenate(([0], np.cumsum(counts))), np.concatenate(lists) if sum(counts) else np.zeros(0, np.int32)]
+        parts += list(extra)
+        sizes = [len(p) for p in parts]
+        # every array on a boundary of 16 bytes, as an allocation of its own would be
+        at = np.concatenate(([0], np.cumsum([-(-n // 4) * 4 for n in sizes])))
+        packed = np.zeros(int(at[-1]), np.int32)
+        for a, p in zip(at, parts):
+            packed[a:a + len(p)] = p
+        dev = self._to_device(packed)
+        pieces = [dev[a:a + n] for a, n in zip(at.tolist(), sizes)]
+        made = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.device)
+        cu_q, kv_lens, positions, token_req = made(B + 1), made(B), made(T), made(T)
+        block_tables, slots = [], []
+        for g, lists in enumerate(tables):
+            table, slot = made(B, max(1, max(len(l) for l in lists))), made(T)
+            ops.step_layout(pieces[0], pieces[1], pieces[2 + 2 * g], pieces[3 + 2 * g], self.cache.page_size, table, slot,
+                            **(dict(cu_q=cu_q, kv_lens=kv_lens, positions=positions, token_req=token_req) if g == 0 else {}))
+            block_tables.append(table)
+            slots.append(slot)
+        return (dict(cu_q=cu_q, kv_lens=kv_lens, positions=positions, token_req=token_req, block_tables=block_tables, slots=slots),
+                pieces[2 + 2 * len(tables):])
+
+    def _device_context(self, lay: _Layout):
+        """``_host_context`` with the index arrays made on the device."""
+        kv = lay.kv_lens.tolist()
+        R, tail = len(lay.rows), self.tail_shortcut and 2 * len(lay.rows) <= lay.T
+        starts = lay.kv_lens - np.asarray(lay.q_lens, np.int32)
+        fields, (ids, state_slots, rows) = self._step_arrays(starts, lay.q_lens, lay.tables, [lay.ids, lay.state_slots, lay.rows])
+        ctx = StepContext(num_tokens=lay.T, num_requests=lay.B, token_ids=ids, state_slots=state_slots, q_lens=lay.q_lens, kv_lens_host=kv,
+                          max_q_len=max(lay.q_lens), max_kv_len=max(kv), **fields)
+        if tail:
+            # The wanted rows as a step of their own (see ``_host_context``).
+            req, pos = lay.req[lay.rows], lay.pos[lay.rows]
+            if R:
+                fields, (tail_ids, tail_slots) = self._step_arrays(pos, [1] * R, [[lists[b] for b in req] for lists in lay.tables],
+                                                                   [lay.ids[lay.rows], lay.state_slots[req]])
+            else:
+                none = rows[:0]
+                fields = dict(cu_q=torch.zeros(1, dtype=torch.int32, device=self.device), kv_lens=none, positions=none, token_req=none,
+                              block_tables=fields["block_tables"], slots=[none for _ in lay.tables])
+                tail_ids, tail_slots = none, none
+            ctx.tail = StepContext(num_tokens=R, num_requests=R, token_ids=tail_ids, state_slots=tail_slots, q_lens=[1] * R,
+                                   kv_lens_host=(pos + 1).tolist(), max_q_len=1, max_kv_len=int(pos.max()) + 1 if R else 0,
+                                   prior_positions_settled=False, **fields)
+            ctx.tail_rows = rows
+        return ctx, rows
+
     def _context(self, lay: _Layout):
+        # (a model without paged caches has no tables to make)
+        return self._device_context(lay) if self.device.type == "cuda" and lay.tables else self._host_context(lay)
+
+    def _host_context(self, lay: _Layout):
         tables, host_tables = [], []
         for lists in lay.tables:
             width = max(1, max(len(l) for l in lists))

@@ -38,7 +38,7 @@ class Attention(Mixer):
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
 
     def cache_requirement(self):
-        return PagedKV(self.num_kv_heads, self.head_dim, self.window)
+        return PagedKV(self.num_kv_heads, self.head_dim, self.window, four_bits=True)
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         H = self.hidden_size
@@ -72,10 +72,13 @@ class Attention(Mixer):
         [T, heads * head size] (possibly a column slice of a wider buffer).  Three ways to the same
         values: few rows (decoding) rotate and write in the product's own epilogue; a product whose K
         the many-rows kernel splits leaves the addition of its slices to the rotation kernel; otherwise
-        the product, then the rotation kernel."""
+        the product, then the rotation kernel (which quantises as well when the cache keeps 4 bits)."""
         rot = self.position.rotary_dim if self.position is not None else 0
         cos_sin = self.position.cos_sin() if self.position is not None else None
         slots = step.slots[cache.group]
+        if cache.four_bits:
+            return ops.rope_kv4_write(ops.linear(x, self.w_qkv, self.b_qkv), step.positions, cos_sin, slots, cache.k, cache.v, self.num_heads,
+                                      self.num_kv_heads, self.head_dim, rot, cache.page_size)
         if self.position is not None and ops.qkv_rope_ok(x, self.w_qkv, cache.k, rot, self.head_dim):
             return ops.qkv_rope_small(x, self.w_qkv, self.b_qkv, step.positions, cos_sin, slots, cache.k, cache.v,
                                       self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size)
@@ -124,6 +127,11 @@ class Attention(Mixer):
 
     def _attend_q(self, q: torch.Tensor, step: StepContext, cache: LayerCache) -> torch.Tensor:
         """Attention of rotated queries over the cache, then the output projection."""
+        if cache.four_bits:
+            o = torch.empty((q.shape[0], self.q_size), dtype=q.dtype, device=q.device)
+            ops.attention_kv4(q, o, cache.k, cache.v, step, cache.group, self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size,
+                              self.window, self.scale)
+            return ops.linear(o, self.w_o, self.b_o, partial_ok=self.partial_output)
         if self.partial_output and ops.attention_oproj_ok(q, self.w_o, step, self.num_heads, self.num_kv_heads, self.head_dim):
             # a small decode batch: the splits of the attention are merged inside the projection's kernel,
             # and the heads' contributions go to the next norm as partial sums

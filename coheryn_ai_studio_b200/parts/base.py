@@ -53,6 +53,9 @@ class PagedKV:
     keep_first: int = 0                   # with a window: the first positions of a sequence, which stay visible (and cached)
                                           # although the window has passed them
 
+    four_bits: bool = field(default=False, compare=False)     # the mixer also writes and reads pages in 4 bits (ops.rope_kv4_write,
+                                                               # ops.attention_kv4); says nothing about what the cache is
+
     def rows_per_page(self, page_size: int) -> int:
         return -(-page_size // self.stride)
 
@@ -75,7 +78,7 @@ class LayerCache:
     """What a mixer gets for one execution of its layer.
 
     Paged: ``k``/``v`` are ``[pages, kv heads, page_size, head_dim]`` views of the
-    group's pool for this schedule entry; ``group`` indexes ``step.block_tables`` and
+    group's pool for this schedule entry (uint8 ``[pages, kv heads, tiles, bytes]`` in a cache of 4 bits: ``four_bits``); ``group`` indexes ``step.block_tables`` and
     ``step.slots``; ``writes`` is False when the entry reads another entry's cache.
     Fixed state: ``state`` is ``[slots, *shape]``; ``step.state_slots`` gives each
     request's slot."""
@@ -87,6 +90,7 @@ class LayerCache:
     v: Optional[torch.Tensor] = None
     writes: bool = True
     state: Optional[torch.Tensor] = None
+    four_bits: bool = False
     # "several": a mixer that asked for a tuple of requirements gets one cache per element, in order.
     parts: Optional[List["LayerCache"]] = None
 
