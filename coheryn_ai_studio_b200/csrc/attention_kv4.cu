@@ -438,30 +438,32 @@ __device__ __forceinline__ Place find_unit(const int* cu_q, const int* kv_lens, 
 __device__ __forceinline__ float factor(float m, float M) { return m == -INFINITY ? 0.f : exp2f(m - M); }
 
 // ------------------------------------------------------------------------------------
-// Attention in float32 arithmetic: any compute type, any alignment, any rows.  A CTA per (token, kv head) walks the
-// visible tiles with its warps side by side; a lane has two halves of one key row for the scores and four channels of
-// a group for the sums.  HC heads of the group at a time share a tile's codes.
+// Attention in float32 arithmetic: any compute type, any alignment, any rows.  A CTA per (token, kv head, part of the visible tiles)
+// walks its tiles with its warps side by side; a lane has two halves of one key row for the scores and four channels of a group for
+// the sums.  HC heads of the group at a time share a tile's codes.  Bound by the latency of a warp's chain (28 tokens of 14 heads
+// over 2, 256 positions: 16.5 us with 8 warps and 4 heads at a time); so many warps, as many heads as fit the registers, and parts
+// (joined by a kernel after it) while there are fewer CTAs than the GPU holds.
 // ------------------------------------------------------------------------------------
-constexpr int HC = 4;
-constexpr int SW = 8;                        // warps
+constexpr int SW = HD > 128 ? 8 : 16;        // warps
 constexpr int VU = (HD / 4 + 31) / 32;       // units of four channels per lane
 
-template <typename T>
+template <typename T, int HC>
 __global__ void __launch_bounds__(32 * SW)
 kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
                   const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ table, int table_ld,
                   const int* __restrict__ token_req, const int* __restrict__ positions, int nh, int nkv, int page_size, int window,
-                  float scale_log2, int* __restrict__ status) {
-  __shared__ float qs[HC][HD];
+                  float scale_log2, float* __restrict__ scratch, int* __restrict__ status) {
+  __shared__ __align__(16) float qs[HC][HD];
   __shared__ float sp[SW][HC][16];
-  __shared__ float merge[SW][HC][HD + 2];
+  __shared__ float merge[SW / 2][HC][HD + 2];
   co_pdl_launch_dependents();
   co_pdl_wait();
-  const int token = blockIdx.x, kvh = blockIdx.y, G = nh / nkv;
+  const int token = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z, parts = gridDim.z, G = nh / nkv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pos = positions[token];
   const int* pages = table + (size_t)token_req[token] * table_ld;
-  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+  const int lo = window > 0 ? max(0, pos - window + 1) : 0, first = lo >> 4, tiles = pos < 0 ? 0 : (pos >> 4) - first + 1;
+  const int tile_first = first + (int)((long long)tiles * part / parts), tile_end = first + (int)((long long)tiles * (part + 1) / parts);
   for (int h0 = 0; h0 < G; h0 += HC) {
     const int n = min(HC, G - h0);
     __syncthreads();
@@ -480,20 +482,21 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[h][v][c] = 0.f;
     }
-    for (int tile = (lo >> 4) + warp; tile * 16 <= pos; tile += SW) {
+    for (int tile = tile_first + warp; tile < tile_end; tile += SW) {
       const int blk = tile * 16 / page_size;
       const int page = blk < table_ld ? pages[blk] : -1;
       if (page < 0 || page >= num_pages) {
         if (lane == 0 && status) *status = BAD_INDEX;
         continue;
       }
-      const unsigned char* kt = k_cache + tile_at(page, nkv, kvh, page_size, tile * 16 - blk * page_size);
-      const unsigned char* vt = v_cache + tile_at(page, nkv, kvh, page_size, tile * 16 - blk * page_size);
+      const size_t at = tile_at(page, nkv, kvh, page_size, tile * 16 - blk * page_size);
+      const unsigned char *kt = k_cache + at, *vt = v_cache + at;
       // Scores: lane = (row, half); words t = 2 half, 2 half + 1 of every group.
       const int r = lane >> 1, half = lane & 1;
       float s[HC];
 #pragma unroll
       for (int h = 0; h < HC; ++h) s[h] = 0.f;
+#pragma unroll
       for (int u = 0; u < NG; ++u) {
         const unsigned sm = reinterpret_cast<const unsigned*>(kt + CODES)[r * NG + u];
         const float sc = lo_bf16(sm), mn = hi_bf16(sm);
@@ -501,11 +504,14 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
         for (int w = 0; w < 2; ++w) {
           const int t = 2 * half + w;
           const unsigned word = reinterpret_cast<const unsigned*>(kt)[r * (4 * NG) + t * NG + u];
+          float x[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float x = fmaf(sc, (float)((word >> (4 * c)) & 15), mn);
+          for (int c = 0; c < 8; ++c) x[c] = fmaf(sc, (float)((word >> (4 * c)) & 15), mn);
 #pragma unroll
-            for (int h = 0; h < HC; ++h) s[h] = fmaf(qs[h][u * 32 + t * 8 + c], x, s[h]);
+          for (int h = 0; h < HC; ++h) {
+            const float4 a = *reinterpret_cast<const float4*>(&qs[h][u * 32 + t * 8]), b = *reinterpret_cast<const float4*>(&qs[h][u * 32 + t * 8 + 4]);
+            s[h] = fmaf(a.x, x[0], fmaf(a.y, x[1], fmaf(a.z, x[2], fmaf(a.w, x[3], s[h]))));
+            s[h] = fmaf(b.x, x[4], fmaf(b.y, x[5], fmaf(b.z, x[6], fmaf(b.w, x[7], s[h]))));
           }
         }
       }
@@ -555,33 +561,89 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
       __syncwarp();
     }
 #pragma unroll
-    for (int h = 0; h < HC; ++h) {
-      const float sum = co_warp_sum(l[h]);
-      if (lane == 0) { merge[warp][h][HD] = m[h]; merge[warp][h][HD + 1] = sum; }
+    for (int h = 0; h < HC; ++h) l[h] = co_warp_sum(l[h]);
+    // The warps meet: the upper half of them leaves its sums, the lower half adds its own in the same order for every row.
+    auto leave = [&](float (*dst)[HD + 2]) {
 #pragma unroll
-      for (int v = 0; v < VU; ++v) {
-        const int unit = v * 32 + lane;
-        if (unit < HD / 4)
+      for (int h = 0; h < HC; ++h) {
+        if (lane == 0) { dst[h][HD] = m[h]; dst[h][HD + 1] = l[h]; }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) merge[warp][h][unit * 4 + c] = acc[h][v][c];
+        for (int v = 0; v < VU; ++v) {
+          const int unit = v * 32 + lane;
+          if (unit < HD / 4)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) dst[h][unit * 4 + c] = acc[h][v][c];
+        }
       }
+    };
+    if (warp >= SW / 2) leave(merge[warp - SW / 2]);
+    __syncthreads();
+    if (warp < SW / 2) {
+      float (*other)[HD + 2] = merge[warp];
+#pragma unroll
+      for (int h = 0; h < HC; ++h) {
+        const float M = fmaxf(m[h], other[h][HD]), f = factor(m[h], M), g = factor(other[h][HD], M);
+        m[h] = M;
+        l[h] = l[h] * f + other[h][HD + 1] * g;
+#pragma unroll
+        for (int v = 0; v < VU; ++v) {
+          const int unit = v * 32 + lane;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (unit < HD / 4) acc[h][v][c] = acc[h][v][c] * f + other[h][unit * 4 + c] * g;
+        }
+      }
+      __syncwarp();
+      leave(other);
     }
     __syncthreads();
     for (int i = tid; i < n * HD; i += 32 * SW) {
-      const int h = i / HD, c = i % HD;
+      const int h = i / HD, c = i % HD, head = kvh * G + h0 + h;
       float M = -INFINITY, den = 0.f, num = 0.f;
 #pragma unroll
-      for (int w = 0; w < SW; ++w) M = fmaxf(M, merge[w][h][HD]);
+      for (int w = 0; w < SW / 2; ++w) M = fmaxf(M, merge[w][h][HD]);
 #pragma unroll
-      for (int w = 0; w < SW; ++w) {
+      for (int w = 0; w < SW / 2; ++w) {
         const float f = factor(merge[w][h][HD], M);
         den += f * merge[w][h][HD + 1];
         num += f * merge[w][h][c];
       }
-      out[(size_t)token * out_ld + (size_t)(kvh * G + h0 + h) * HD + c] = co_from_float<T>(den == 0.f ? 0.f : num / den);
+      if (parts == 1) {
+        out[(size_t)token * out_ld + (size_t)head * HD + c] = co_from_float<T>(den == 0.f ? 0.f : num / den);
+      } else {
+        float* dst = scratch + (((size_t)token * nh + head) * parts + part) * (HD + 2);
+        dst[c] = num;
+        if (c == 0) { dst[HD] = M; dst[HD + 1] = den; }
+      }
     }
   }
 }
+
+// Joins the parts of a row: a warp per (token, head), in ascending order of the parts.
+template <typename T>
+__global__ void __launch_bounds__(128)
+kv4_simple_join_kernel(const float* __restrict__ scratch, int parts, T* __restrict__ out, long out_ld, int nh, int rows) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  co_pdl_launch_dependents();
+  if (row >= rows) return;
+  co_pdl_wait();
+  const float* src = scratch + (size_t)row * parts * (HD + 2);
+  float M = -INFINITY, den = 0.f, acc[HD / 32];
+  for (int p = lane; p < parts; p += 32) M = fmaxf(M, src[p * (HD + 2) + HD]);
+  M = co_warp_max(M);
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
+  for (int p = 0; p < parts; ++p) {
+    const float f = factor(src[p * (HD + 2) + HD], M);
+    den += f * src[p * (HD + 2) + HD + 1];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) acc[i] += f * src[p * (HD + 2) + i * 32 + lane];
+  }
+  T* dst = out + (size_t)(row / nh) * out_ld + (size_t)(row % nh) * HD;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) dst[i * 32 + lane] = co_from_float<T>(den == 0.f ? 0.f : acc[i] / den);
+}
+
 // ------------------------------------------------------------------------------------
 // Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
 // each with pairs of tiles of its own (pair i of the item goes to warp i mod 4) in a ring of its own that it fills with
@@ -688,9 +750,28 @@ __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) 
 }
 constexpr int MLD = HD + 4;              // a row of the warps' meeting: HD channels, reference, sum
 template <int NT>
-constexpr size_t items_smem() {
-  const size_t ring = (size_t)WARPS * RING, merge = (size_t)WARPS * 8 * NT * MLD * sizeof(float);
+constexpr size_t items_smem() {           // rings, or the warps' meeting and what a cluster's CTAs leave one another
+  const size_t ring = (size_t)WARPS * RING, merge = (size_t)(WARPS + 1) * 8 * NT * MLD * sizeof(float);
   return ring > merge ? ring : merge;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared memory `p` in CTA `rank` of the cluster, and floats from there.
+__device__ __forceinline__ unsigned in_cluster(const void* p, unsigned rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(unsigned at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(unsigned at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
 }
 
 // The query rows of a tile as the products' N side: lane (g, t) has row g of every eight, channels 32 u + 8 t + 0..7.
@@ -822,12 +903,13 @@ __device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[N
   }
 }
 
-template <int NT, int PER_SM>
+// CLUSTER: the CTAs of a cluster cut one list among themselves and join it through their shared memory, without a second kernel.
+template <int NT, int PER_SM, bool CLUSTER>
 __global__ void __launch_bounds__(32 * WARPS, PER_SM)
 kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ block_tables, int table_ld,
                  const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int B, int nh, int nkv, int page_size, int window,
-                 float scale_log2, int max_rows, float* __restrict__ scratch, int* __restrict__ status) {
+                 float scale_log2, int max_rows, int csize, float* __restrict__ scratch, int* __restrict__ status) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int COLS = 8 * NT;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -835,19 +917,40 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   co_pdl_wait();
   co_pdl_launch_dependents();
   const int G = nh / nkv;
-  const int total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window), shares = min((int)gridDim.x, total);
-  if ((int)blockIdx.x >= shares) return;
-  int unit = share_start(blockIdx.x, shares, total);
-  const int unit_end = share_start(blockIdx.x + 1, shares, total);
-  Place at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
+  int total = 0, shares = 0, unit = 0, unit_end = 0;
+  Place at;
+  const int most_tiles = (max_rows + COLS - 1) / COLS, own_list = CLUSTER ? (int)blockIdx.x / csize : 0, rank = CLUSTER ? (int)blockIdx.x % csize : 0;
+  if constexpr (CLUSTER) {
+    at.b = own_list / (nkv * most_tiles);
+    at.cut = cut_of(cu_q, kv_lens, at.b, G, COLS, max_rows, window);
+    if (own_list % most_tiles >= at.cut.row_tiles) return;      // the whole cluster
+  } else {
+    total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window);
+    shares = min((int)gridDim.x, total);
+    if ((int)blockIdx.x >= shares) return;
+    unit = share_start(blockIdx.x, shares, total);
+    unit_end = share_start(blockIdx.x + 1, shares, total);
+    at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
+  }
   unsigned char* ring = smem + (size_t)warp * RING;       // keys, then values
   const unsigned ring_lane = smem_u32(ring) + lane * 16;
   const unsigned char *k_lane = k_cache + lane * 16, *v_lane = v_cache + lane * 16;
 
   for (bool first_list = true; at.b >= 0; first_list = false) {
     const Cut c = at.cut;
-    const int list = (unit - at.first) / c.units, u_first = unit - at.first - list * c.units, u_end = min(c.units, u_first + unit_end - unit);
-    const int row_tile = list % c.row_tiles, kvh = list / c.row_tiles;
+    int row_tile, kvh, u_first, u_end;
+    if constexpr (CLUSTER) {
+      row_tile = own_list % most_tiles;
+      kvh = own_list / most_tiles % nkv;
+      u_first = share_start(rank, csize, c.units);
+      u_end = share_start(rank + 1, csize, c.units);
+    } else {
+      const int list = (unit - at.first) / c.units;
+      u_first = unit - at.first - list * c.units;
+      u_end = min(c.units, u_first + unit_end - unit);
+      row_tile = list % c.row_tiles;
+      kvh = list / c.row_tiles;
+    }
     const int row0 = row_tile * COLS, rows = min(COLS, c.q_len * G - row0);      // query rows of this tile
     const int* table = block_tables + (size_t)at.b * table_ld;
     const int tile_end = min(c.lo16 + u_end * (UNIT / 16), (c.kv_len + 15) >> 4);
@@ -1040,12 +1143,13 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     const int slot = 2 * blockIdx.x + (first_list ? 0 : 1);
     float* acc_out = scratch + (size_t)slot * COLS * HD;
     float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)2 * gridDim.x * COLS * HD) + (size_t)slot * COLS;
-    if (tid == 0 && u_first == 0) {
+    float* left = merge + (size_t)WARPS * COLS * MLD;          // for the cluster: a row's channels, reference and sum
+    if (!CLUSTER && tid == 0 && u_first == 0) {
       int2* heads = reinterpret_cast<int2*>(scratch + (size_t)2 * gridDim.x * COLS * (HD + 2));
-      heads[((size_t)at.b * nkv + kvh) * ((max_rows + COLS - 1) / COLS) + row_tile] =
+      heads[((size_t)at.b * nkv + kvh) * most_tiles + row_tile] =
           make_int2(share_of(unit + c.units - 1, shares, total) - (int)blockIdx.x + 1, slot);
     }
-    const bool whole_list = u_first == 0 && u_end == c.units;
+    const bool whole_list = !CLUSTER && u_first == 0 && u_end == c.units;
     for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
       const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
       float M = NOTHING, den = 0.f;
@@ -1065,10 +1169,38 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         const int row = row0 + r;
         bf16* dst = out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD + ch;
         store4<bf16>(dst, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      } else if (CLUSTER) {
+        *reinterpret_cast<float4*>(left + r * MLD + ch) = acc;
+        if (ch == 0) *reinterpret_cast<float2*>(left + r * MLD + HD) = make_float2(M, den);
       } else {
         *reinterpret_cast<float4*>(acc_out + (size_t)r * HD + ch) = acc;
         if (ch == 0) ml_out[r] = make_float2(M, den);
       }
+    }
+    if constexpr (CLUSTER) {
+      cluster_barrier();
+      // The rows' pieces of four channels, shared among the CTAs; parts in ascending order.
+      for (int x = rank * 32 * WARPS + tid; x < rows * (HD / 4); x += csize * 32 * WARPS) {
+        const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
+        float M = NOTHING, den = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int p = 0; p < csize; ++p) M = fmaxf(M, ld_cluster2(in_cluster(left + r * MLD + HD, p)).x);
+#pragma unroll 8
+        for (int p = 0; p < csize; ++p) {
+          const float2 ml = ld_cluster2(in_cluster(left + r * MLD + HD, p));
+          const float4 v = ld_cluster4(in_cluster(left + r * MLD + ch, p));
+          const float f = exp2f(ml.x - M);
+          den += f * ml.y;
+          acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const int row = row0 + r;
+        store4<bf16>(out + (size_t)(c.tok0 + row / G) * out_ld + (size_t)(kvh * G + row % G) * HD + ch, acc.x * inv, acc.y * inv, acc.z * inv,
+                     acc.w * inv);
+      }
+      cluster_barrier();               // nobody leaves while its part may still be read
+      return;
     }
     unit += u_end - u_first;
     if (unit >= unit_end) return;
@@ -1182,18 +1314,35 @@ int ctas_of(int B, int nkv, int max_rows, int max_kv_len, int* per_sm = nullptr)
   return (int)(units < 148 * resident ? units : 148 * resident);
 }
 
-template <int NT, int PER_SM>
+// CTAs per list when clusters join the lists (0: a kernel after it does): while all of them are resident at once and a CTA gets two
+// units at most, so that the second kernel's start and its chain of reads are what counts (1 x 700 positions: 6.7 us against 8.2; 8 x 4,096,
+// up to three units per CTA of 16: 12.1 against 11.6).
+int cluster_of(int B, int nkv, int max_rows, int max_kv_len) {
+  const int nt = tiles_of(max_rows);
+  const long long lists = (long long)B * nkv * ((max_rows + 8 * nt - 1) / (8 * nt));
+  const int units = (max_kv_len + 15) / UNIT + 1;
+  if (HD > 128 || nt != 1 || units < 2) return 0;
+  for (int c : {16, 8})
+    if (lists * c <= 148 * MOST && units <= 2 * c) return c;
+  return 0;
+}
+
+template <int NT, int PER_SM, bool CLUSTER>
 int launch_items(const void* q, long q_ld, void* out, long out_ld, const void* k_cache, const void* v_cache, int num_pages, const int* table,
                  int table_ld, const int* cu_q, const int* kv_lens, int B, int nh, int nkv, int page_size, int window, float scale_log2,
-                 int max_rows, int ctas, float* scratch, int* status, cudaStream_t stream) {
+                 int max_rows, int ctas, int csize, float* scratch, int* status, cudaStream_t stream) {
   constexpr size_t SMEM = items_smem<NT>();
-  if (SMEM > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_items_kernel<NT, PER_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
-    if (e != cudaSuccess) CO_FAIL("kv4_attention: %zu bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+  auto kernel = kv4_items_kernel<NT, PER_SM, CLUSTER>;
+  cudaError_t e = SMEM > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) : cudaSuccess;
+  if (e == cudaSuccess && csize > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) CO_FAIL("kv4_attention: %zu bytes of shared memory, clusters of %d: %s", SMEM, csize, cudaGetErrorString(e));
+  e = co_launch_cluster(csize, kernel, dim3((unsigned)ctas), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
+                        (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv,
+                        page_size, window, scale_log2, max_rows, csize, scratch, status);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    CO_FAIL("kv4_items: launch failed: %s", cudaGetErrorString(e));
   }
-  co_launch(kv4_items_kernel<NT, PER_SM>, dim3((unsigned)ctas), dim3(32 * WARPS), SMEM, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld,
-            (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size,
-            window, scale_log2, max_rows, scratch, status);
   CO_CHECK_LAUNCH("kv4_items");
   return 0;
 }
@@ -1266,27 +1415,47 @@ CO_EXPORT int coheryn_kv4_pages(const void* k_cache, const void* v_cache, int nu
                       stream);
 }
 
+// Into how many parts the float32 kernel cuts a row's tiles: one tile per warp at least, and no more CTAs than are resident.
+CO_EXPORT int coheryn_kv4_simple_parts(int T, int nkv, int max_kv_len, int window) {
+  if (max_kv_len <= 0 || T <= 0 || nkv <= 0) return 1;
+  const int keys = window > 0 && window < max_kv_len ? window : max_kv_len;
+  const long long by_size = ((long long)keys + 16 * SW - 1) / (16 * SW), by_slots = 148LL * 2 / ((long long)T * nkv);
+  const long long parts = by_size < by_slots ? by_size : by_slots;
+  return parts < 1 ? 1 : (int)parts;
+}
+CO_EXPORT long coheryn_kv4_simple_scratch_floats(int T, int nh, int parts) { return parts > 1 ? (long)T * nh * parts * (HD + 2) : 0; }
+
 CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, long out_ld, int dtype, const void* k_cache, const void* v_cache,
                                            int num_pages, const int* table, int table_ld, const int* token_req, const int* positions, int T,
-                                           int nh, int nkv, int page_size, int window, float scale, int* status, cudaStream_t stream) {
+                                           int nh, int nkv, int page_size, int window, float scale, int parts, float* scratch,
+                                           long scratch_floats, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
   if (check_pages("kv4_attention", nkv, page_size, num_pages)) return 1;
   if (nh < 1 || nh % nkv || nkv > 65535) CO_FAIL("kv4_attention: %d heads do not group over %d kv heads", nh, nkv);
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15)) CO_FAIL("kv4_attention: caches must be 16-byte aligned");
+  if (parts < 1 || parts > 65535 || scratch_floats < coheryn_kv4_simple_scratch_floats(T, nh, parts))
+    CO_FAIL("kv4_attention: %d parts in a scratch of %ld floats", parts, scratch_floats);
   const float scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid((unsigned)T, (unsigned)nkv);
-  if (dtype == CO_F32)
-    co_launch(kv4_simple_kernel<float>, grid, dim3(32 * SW), 0, stream, (const float*)q, q_ld, (float*)out, out_ld, (const unsigned char*)k_cache,
-              (const unsigned char*)v_cache, num_pages, table, table_ld, token_req, positions, nh, nkv, page_size, window, scale_log2, status);
-  else
-    co_launch(kv4_simple_kernel<bf16>, grid, dim3(32 * SW), 0, stream, (const bf16*)q, q_ld, (bf16*)out, out_ld, (const unsigned char*)k_cache,
-              (const unsigned char*)v_cache, num_pages, table, table_ld, token_req, positions, nh, nkv, page_size, window, scale_log2, status);
+  auto with = [&](auto* x) {
+    typedef decltype(x) P;
+    typedef std::remove_pointer_t<P> E;
+    co_launch(nh / nkv <= 4 ? kv4_simple_kernel<E, 4> : kv4_simple_kernel<E, 8>, dim3((unsigned)T, (unsigned)nkv, (unsigned)parts), dim3(32 * SW), 0,
+              stream, (P)q, q_ld, (P)out, out_ld, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, token_req,
+              positions, nh, nkv, page_size, window, scale_log2, scratch, status);
+    co_count_launch();
+    if (parts > 1)
+      co_launch(kv4_simple_join_kernel<E>, dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream, (const float*)scratch, parts, (P)out,
+                out_ld, nh, T * nh);
+  };
+  if (dtype == CO_F32) with((float*)nullptr);
+  else with((bf16*)nullptr);
   CO_CHECK_LAUNCH("kv4_attention_simple");
   return 0;
 }
 
 // Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests that it takes.
 CO_EXPORT long coheryn_kv4_scratch_floats(int B, int nkv, int max_rows, int max_kv_len) {
+  if (cluster_of(B, nkv, max_rows, max_kv_len)) return 0;
   const int cols = 8 * tiles_of(max_rows);
   return 2L * ctas_of(B, nkv, max_rows, max_kv_len) * cols * (HD + 2) + 2L * B * nkv * ((max_rows + cols - 1) / cols);
 }
@@ -1303,16 +1472,18 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   if ((q_ld & 7) || (out_ld & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15))
     CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
   if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
-  int per_sm = 0;
-  const int nt = tiles_of(max_rows), ctas = ctas_of(B, nkv, max_rows, max_kv_len, &per_sm);
   if ((long long)B * nkv * ((max_rows + 7) / 8) * ((max_kv_len + 15LL) / UNIT + 1) > 0x7fffffffLL)
     CO_FAIL("kv4_attention: %d requests of %d positions and %d kv heads", B, max_kv_len, nkv);
+  int per_sm = 0;
+  const int nt = tiles_of(max_rows), csize = cluster_of(B, nkv, max_rows, max_kv_len);
+  const int ctas = csize ? B * nkv * ((max_rows + 7) / 8) * csize : ctas_of(B, nkv, max_rows, max_kv_len, &per_sm);
   if (scratch_floats < coheryn_kv4_scratch_floats(B, nkv, max_rows, max_kv_len) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_attention: the scratch is too small or not 16-byte aligned");
-  auto launch = nt == 2 ? launch_items<HD <= 128 ? 2 : 1, 2> : per_sm == MOST ? launch_items<1, MOST> : launch_items<1, FEWER>;
+  auto launch = csize ? launch_items<1, MOST, true> : nt == 2 ? launch_items<HD <= 128 ? 2 : 1, 2, false>
+                : per_sm == MOST ? launch_items<1, MOST, false> : launch_items<1, FEWER, false>;
   const int rc = launch(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size, window,
-                        scale * 1.4426950408889634f, max_rows, ctas, scratch, status, stream);
-  if (rc || max_kv_len + 15 <= UNIT) return rc;    // no list is longer than one unit: nothing to join
+                        scale * 1.4426950408889634f, max_rows, ctas, csize ? csize : 1, scratch, status, stream);
+  if (rc || csize || max_kv_len + 15 <= UNIT) return rc;    // joined already, or no list is longer than one unit
   const int cols = 8 * nt;
   const bool wide = (long long)B * nkv * max_rows <= 148 * 4;
   co_launch(wide ? kv4_join_kernel<true> : kv4_join_kernel<false>, dim3((unsigned)(wide ? max_rows : (max_rows + cols - 1) / cols), (unsigned)nkv, (unsigned)B),

@@ -169,10 +169,10 @@ PyObject* pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // attention(scratch entry, entry, simple entry, q, out, k_cache, v_cache, block_tables, token_req, positions, heads, kv heads, head_dim, page_size, window,
-//           scale, cu_q, kv_lens, q_lens, max_kv_len, most rows, status): bfloat16 requests of at most `most rows` rows each,
+//           scale, cu_q, kv_lens, q_lens, max_kv_len, most rows, status, parts entry): bfloat16 requests of at most `most rows` rows each,
 // and float32
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 22) return none();
+  if (n != 23) return none();
   return guarded([&]() -> PyObject* {
     Call c;
     const long nh = c.number(a[10]), nkv = c.number(a[11]), hd = c.number(a[12]), page_size = c.number(a[13]);
@@ -190,12 +190,18 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float scale = (float)PyFloat_AS_DOUBLE(a[15]);
     if (code == 0) {
       int *req = c.words(a[8], T), *pos = c.words(a[9], T);
+      const long longest = a[19] == Py_None ? 0 : c.number(a[19]);
       if (!c.ok) return none();
+      typedef int (*Parts)(int, int, int, int);
+      const int parts = ((Parts)address(a[22]))((int)T, (int)nkv, (int)longest, (int)window);
+      const long floats = parts > 1 ? T * nh * parts * (hd + 2) : 0;
+      at::Tensor scratch;
+      if (floats) scratch = at::empty({floats}, q->options().dtype(at::kFloat));
       typedef int (*Fn)(const void*, long, void*, long, int, const void*, const void*, int, const int*, int, const int*, const int*, int, int, int, int, int,
-                        float, int*, void*);
+                        float, int, float*, long, int*, void*);
       return PyLong_FromLong(((Fn)address(a[2]))(q->data_ptr(), (long)q->stride(0), out->data_ptr(), (long)out->stride(0), code, k, v, (int)pages, table,
-                                                 (int)tt.size(1), req, pos, (int)T, (int)nh, (int)nkv, (int)page_size, (int)window, scale, status,
-                                                 c.stream()));
+                                                 (int)tt.size(1), req, pos, (int)T, (int)nh, (int)nkv, (int)page_size, (int)window, scale, parts,
+                                                 floats ? (float*)scratch.data_ptr() : nullptr, floats, status, c.stream()));
     }
     if (!PyList_Check(a[18]) || a[16] == Py_None || a[17] == Py_None || a[19] == Py_None) return none();
     const long B = (long)PyList_GET_SIZE(a[18]), G = nh / nkv, longest_kv = c.number(a[19]);

@@ -2391,7 +2391,7 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
                                 _address(lib, "coheryn_kv4_attention_simple"), q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads,
                                 num_kv_heads, head_dim, page_size, window, scale, cu_q, kv_lens, q_lens, max_kv_len, KV4_DIRECT_ROWS,
-                                tc_status(q.device))
+                                tc_status(q.device), _address(lib, "coheryn_kv4_simple_parts"))
         if rc == 0:
             return
         if rc is not None:
@@ -2417,9 +2417,13 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     if (force_simple or q.dtype is not torch.bfloat16 or cu_q is None or kv_lens is None or q_lens is None or max_kv_len is None
             or q_ld % 8 or q_at % 16 or out_ld % 4 or out_at % 8):
         _words(T, token_req=token_req, positions=positions)
-        rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipippiiiiifpp")(
+        parts = int(lib.coheryn_kv4_simple_parts(c_int(T), c_int(num_kv_heads), c_int(max_kv_len or 0), c_int(window or 0)))
+        floats = T * num_heads * parts * (head_dim + 2) if parts > 1 else 0
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipippiiiiifiplpp")(
             q_at, q_ld, out_at, out_ld, _code(q), k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W,
-            token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, status, stream)
+            token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, parts, _at(scratch), floats,
+            status, stream)
         if rc:
             _check(lib, rc)
         return
