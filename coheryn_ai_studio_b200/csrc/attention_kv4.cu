@@ -881,7 +881,7 @@ __device__ __forceinline__ void tile_scores(float (&s)[NT][4], const Queries<NT>
 
 // Adds a tile's values, weighted: pf[nt] holds the probabilities of the 16 positions for row g of every eight.
 template <int NT>
-__device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[NT][2], const unsigned char* vt) {
+__device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[NT][4], const unsigned char* vt) {
   const int lane = threadIdx.x & 31, t = lane & 3;
   const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
 #pragma unroll
@@ -899,6 +899,8 @@ __device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[N
     for (int nt = 0; nt < NT; ++nt) {
       mma_bf16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
       mma_bf16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
+      mma_bf16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][2], pf[nt][3]);
+      mma_bf16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][2], pf[nt][3]);
     }
   }
 }
@@ -1012,7 +1014,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
 
     float s[2][NT][4];
-    unsigned pf[2][NT][2];
+    unsigned pf[2][NT][4];
     // From the scores s of pair i, whose values are at `values`, to its probabilities pf.
     auto probabilities = [&](int i, unsigned char* values) {
       const int key0 = (tile0 + i * 2 * WARPS) * 16;
@@ -1085,8 +1087,13 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
             y[h][nt][x] = ex2(y[h][nt][x]);
             sm.l[nt][x & 1] += y[h][nt][x];
           }
-          pf[h][nt][0] = transposed(pack(y[h][nt][0], y[h][nt][1]));
-          pf[h][nt][1] = transposed(pack(y[h][nt][2], y[h][nt][3]));
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float a = y[h][nt][2 * x], b = y[h][nt][2 * x + 1];
+            const unsigned w = pack(a, b);
+            pf[h][nt][x] = transposed(w);
+            pf[h][nt][2 + x] = transposed(pack(a - lo_bf16(w), b - hi_bf16(w)));
+          }
         }
     };
 
