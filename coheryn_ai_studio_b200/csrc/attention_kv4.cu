@@ -40,6 +40,10 @@ __device__ __forceinline__ float hi_bf16(unsigned w) { return __uint_as_float(w 
 __device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
 __device__ __forceinline__ __nv_bfloat162 pair_of(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
 __device__ __forceinline__ unsigned pack(float a, float b) { return bits(__floats2bfloat162_rn(a, b)); }
+__device__ __forceinline__ unsigned pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
 
 // The start of the tile that holds row `row` of a page.
 __device__ __forceinline__ size_t tile_at(long long page, int nkv, int kvh, int page_size, int row) {
@@ -286,27 +290,105 @@ kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ pos
 }
 
 // ------------------------------------------------------------------------------------
-// Pages as values: [entry, kv head, page_size, HD] in float32 or bfloat16.  One block per (page, kv head).
+// Pages as values: [entry, kv head, page_size, HD] in float32, bfloat16, or scaled float16 (for attention_kv4_prompt.cu).  One block per (page, kv head).
 // With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length are
 // zeros, entries that lie wholly behind it or in front of the window of its first new token are left out, and
 // `out_table` gets the entry's place among the output pages, or -1.
 // Bound by the bytes written (16 of 21 bits a value).
 // ------------------------------------------------------------------------------------
+template <>
+__device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+}
+template <>
+__device__ __forceinline__ void store4<__half>(__half* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_f16(a, b), pack_f16(c, d));
+}
+// How many rows of entry j of request b's block table hold something that its new tokens see (0: the entry is not needed).
+__device__ __forceinline__ int rows_needed(const int* cu_q, const int* lens, int b, int j, int page_size, int window) {
+  const int len = lens[b], first_new = len - (cu_q[b + 1] - cu_q[b]);
+  const int first_key = window > 0 ? max(0, first_new - window + 1) : 0;
+  return (j + 1) * page_size <= first_key ? 0 : max(0, min(page_size, len - j * page_size));
+}
+
+// The largest magnitude among the keys, and among the values, that the requests' new tokens see, from the pairs alone (a group's
+// values lie between m and m + 15 s): RANGE_BLOCKS partial answers.  A fifth of the pages' bytes.
+constexpr int RANGE_BLOCKS = 128;
+__global__ void __launch_bounds__(256)
+kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
+                 const int* __restrict__ table, int table_ld, int width, int n, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
+                 float2* __restrict__ partial) {
+  __shared__ float2 part[8];
+  co_pdl_launch_dependents();
+  co_pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_page = page_size >> 4;
+  float k_most = 0.f, v_most = 0.f;
+  // A warp takes a (request, entry, kv head) at a time.
+  const long long items = (long long)n * width * nkv;
+  for (long long x = (long long)blockIdx.x * 8 + warp; x < items; x += RANGE_BLOCKS * 8) {
+    const int kvh = (int)(x % nkv), j = (int)(x / nkv % width), b = (int)(x / nkv / width);
+    const int rows = rows_needed(cu_q, lens, b, j, page_size, window), page = rows ? table[(size_t)b * table_ld + j] : -1;
+    if (page < 0 || page >= num_pages) continue;
+    for (int tile = 0; tile < per_page && tile * 16 < rows; ++tile) {
+      const size_t at = tile_at(page, nkv, kvh, page_size, tile * 16) + CODES;
+      for (int i = lane; i < 16 * NG; i += 32) {         // keys: row i / NG
+        const unsigned w = reinterpret_cast<const unsigned*>(k_cache + at)[i];
+        const float m = hi_bf16(w);
+        if (tile * 16 + i / NG < rows) k_most = fmaxf(k_most, fmaxf(fabsf(m), fabsf(fmaf(15.f, lo_bf16(w), m))));
+      }
+      for (int i = lane; i < 4 * NG; i += 32) {          // values: rows 4 (i % 4)..
+        const uint4 w = reinterpret_cast<const uint4*>(v_cache + at)[i];
+        const float sc[4] = {lo_bf16(w.x), hi_bf16(w.x), lo_bf16(w.y), hi_bf16(w.y)}, mn[4] = {lo_bf16(w.z), hi_bf16(w.z), lo_bf16(w.w), hi_bf16(w.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tile * 16 + (i & 3) * 4 + e < rows) v_most = fmaxf(v_most, fmaxf(fabsf(mn[e]), fabsf(fmaf(15.f, sc[e], mn[e]))));
+      }
+    }
+  }
+  k_most = co_warp_max(k_most);
+  v_most = co_warp_max(v_most);
+  if (lane == 0) part[warp] = make_float2(k_most, v_most);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) { k_most = fmaxf(k_most, part[w].x); v_most = fmaxf(v_most, part[w].y); }
+    partial[blockIdx.x] = make_float2(k_most, v_most);
+  }
+}
+// The power of two that brings a largest magnitude to 2^13..2^14, and its inverse.
+__device__ __forceinline__ float2 to_float16_range(float most) {
+  const int e = min(max((int)(__float_as_uint(most) >> 23), 14), 240);
+  return make_float2(__uint_as_float((unsigned)(267 - e) << 23), __uint_as_float((unsigned)(e - 13) << 23));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(128)
 kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
                  const int* __restrict__ table, int table_ld, int width, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
-                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, int* __restrict__ status) {
+                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, const float2* __restrict__ range,
+                 float* __restrict__ factors, int* __restrict__ status) {
+  constexpr bool HALF = sizeof(T) == 2 && !std::is_same<T, bf16>::value;
+  __shared__ float2 most[4];
   co_pdl_launch_dependents();
   co_pdl_wait();
   const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
   const long long entry = (long long)b * width + j;
+  float k_by = 1.f, v_by = 1.f;
+  if constexpr (HALF) {             // float16: times the powers of two that the largest values ask for
+    static_assert(RANGE_BLOCKS == 128, "a thread per partial answer");
+    const float2 x = range[threadIdx.x];
+    const float kx = co_warp_max(x.x), vx = co_warp_max(x.y);
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = make_float2(kx, vx);
+    __syncthreads();
+    const float2 k2 = to_float16_range(fmaxf(fmaxf(most[0].x, most[1].x), fmaxf(most[2].x, most[3].x)));
+    const float2 v2 = to_float16_range(fmaxf(fmaxf(most[0].y, most[1].y), fmaxf(most[2].y, most[3].y)));
+    k_by = k2.x;
+    v_by = v2.x;
+    if (j == 0 && kvh == 0 && b == 0 && threadIdx.x == 0) { factors[0] = k2.y; factors[1] = v2.y; }
+  }
   int valid = page_size;                           // rows of the page that hold something
   if (lens) {
-    const int len = lens[b], first_new = len - (cu_q[b + 1] - cu_q[b]);
-    const int first_key = window > 0 ? max(0, first_new - window + 1) : 0;
-    valid = min(page_size, len - j * page_size);
-    if (valid <= 0 || (j + 1) * page_size <= first_key) {
+    valid = rows_needed(cu_q, lens, b, j, page_size, window);
+    if (!valid) {
       if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
       return;
     }
@@ -330,7 +412,10 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
       const unsigned word = reinterpret_cast<const unsigned*>(kt)[r * (4 * NG) + t * NG + u];
       const unsigned sm = reinterpret_cast<const unsigned*>(kt + CODES)[r * NG + u];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) x[c] = keep ? fmaf(lo_bf16(sm), (float)((word >> (4 * c)) & 15), hi_bf16(sm)) : 0.f;
+      for (int c = 0; c < 8; ++c) {
+        const float y = fmaf(lo_bf16(sm), (float)((word >> (4 * c)) & 15), hi_bf16(sm));
+        x[c] = keep ? (HALF ? y * k_by : y) : 0.f;
+      }
       store8(ko + (size_t)(tile * 16 + r) * HD + u * 32 + t * 8, x);
     }
     for (int i = threadIdx.x; i < 32 * NG; i += 128) {
@@ -345,7 +430,10 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
         const unsigned h = (e < 2 ? words.x : words.y) >> (16 * (e & 1));
         float x[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = r < valid ? fmaf(sc[e], (float)((h >> (4 * c)) & 15), mn[e]) : 0.f;
+        for (int c = 0; c < 4; ++c) {
+          const float y = fmaf(sc[e], (float)((h >> (4 * c)) & 15), mn[e]);
+          x[c] = r < valid ? (HALF ? y * v_by : y) : 0.f;
+        }
         store4(vo + (size_t)r * HD + u * 32 + g * 4, x[0], x[1], x[2], x[3]);
       }
     }
@@ -725,10 +813,6 @@ __device__ __forceinline__ unsigned masked(unsigned word, unsigned mask, unsigne
 // Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair c 2^-24 (j even) or 16 c 2^-24 (j odd).
 __device__ __forceinline__ unsigned codes128(unsigned word, int j) { return masked(word >> (4 * j), 0x000f000fu, 0x43004300u); }
 __device__ __forceinline__ unsigned codes16(unsigned word, int j) { return (j < 2 ? word : word >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
-__device__ __forceinline__ unsigned pack_f16(float a, float b) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const unsigned*>(&v);
-}
 template <int N>
 __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) {
   if constexpr (N % 4 == 0) {
@@ -1396,17 +1480,21 @@ CO_EXPORT int coheryn_kv4_write(const void* qkv, long ld, int dtype, const int* 
   return 0;
 }
 
+constexpr int PAGES_F16 = 2;      // beside the dtype codes
+
 static int launch_pages(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
                         int width, int n, const int* cu_q, const int* lens, int window, void* k_out, void* v_out, int dtype, int* out_table,
-                        int* status, cudaStream_t stream) {
+                        const float2* range, float* factors, int* status, cudaStream_t stream) {
   if (nkv > 65535 || n > 65535) CO_FAIL("kv4_pages: %d requests, %d kv heads", n, nkv);
   const dim3 grid((unsigned)width, (unsigned)nkv, (unsigned)n);
-  if (dtype == CO_F32)
-    co_launch(kv4_pages_kernel<float>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
-              page_size, table, table_ld, width, cu_q, lens, window, (float*)k_out, (float*)v_out, out_table, status);
-  else
-    co_launch(kv4_pages_kernel<bf16>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
-              page_size, table, table_ld, width, cu_q, lens, window, (bf16*)k_out, (bf16*)v_out, out_table, status);
+  auto with = [&](auto* x) {
+    typedef decltype(x) P;
+    co_launch(kv4_pages_kernel<std::remove_pointer_t<P>>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
+              num_pages, nkv, page_size, table, table_ld, width, cu_q, lens, window, (P)k_out, (P)v_out, out_table, range, factors, status);
+  };
+  if (dtype == CO_F32) with((float*)nullptr);
+  else if (dtype == PAGES_F16) with((__half*)nullptr);
+  else with((bf16*)nullptr);
   CO_CHECK_LAUNCH("kv4_pages");
   return 0;
 }
@@ -1418,8 +1506,8 @@ CO_EXPORT int coheryn_kv4_pages(const void* k_cache, const void* v_cache, int nu
   if (check_pages("kv4_pages", nkv, page_size, num_pages)) return 1;
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
     CO_FAIL("kv4_pages: operands must be 16-byte aligned");
-  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, status,
-                      stream);
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, nullptr,
+                      nullptr, status, stream);
 }
 
 // Into how many parts the float32 kernel cuts a row's tiles: one tile per warp at least, and no more CTAs than are resident.
@@ -1499,16 +1587,23 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   return 0;
 }
 
-// The pages of requests b = 0..n-1 of a block table in bfloat16, dense: entry (b, j) becomes page b * width + j of k_out and v_out
-// [n * width, nkv, page_size, HD] and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length are zeros.
+// The pages of requests b = 0..n-1 of a block table, dense: entry (b, j) becomes page b * width + j of k_out and v_out [n * width, nkv, page_size, HD]
+// and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length are zeros.  In bfloat16, or, with `factors` (float32
+// [2 + 2 * 128], of which the first two are what keys and values have to be multiplied by), in scaled float16.
 CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
                                  int width, int n, const int* cu_q, const int* kv_lens, int window, void* k_out, void* v_out, int* out_table,
-                                 int* status, cudaStream_t stream) {
+                                 float* factors, int* status, cudaStream_t stream) {
   if (n <= 0 || width <= 0) return 0;
   if (check_pages("kv4_expand", nkv, page_size, num_pages)) return 1;
-  if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
+  if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || ((uintptr_t)factors & 7))
     CO_FAIL("kv4_expand: operands must be 16-byte aligned");
   if (width > table_ld) CO_FAIL("kv4_expand: %d entries of rows of %d", width, table_ld);
-  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, n, cu_q, kv_lens, window, k_out, v_out, CO_BF16,
-                      out_table, status, stream);
+  float2* range = factors ? reinterpret_cast<float2*>(factors + 2) : nullptr;
+  if (factors) {
+    co_launch(kv4_range_kernel, dim3(RANGE_BLOCKS), dim3(256), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
+              page_size, table, table_ld, width, n, cu_q, kv_lens, window, range);
+    CO_CHECK_LAUNCH("kv4_range");
+  }
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, n, cu_q, kv_lens, window, k_out, v_out,
+                      factors ? PAGES_F16 : CO_BF16, out_table, (const float2*)range, factors, status, stream);
 }

@@ -38,6 +38,7 @@ LINEAR_RECURRENCE_SOURCES = ["linear_recurrence.cu", "runtime.cu"]
 LINEAR_ATTENTION_SOURCES = ["linear_attention.cu", "runtime.cu"]
 LIGHTNING_SOURCES = ["lightning_attention.cu", "runtime.cu"]
 POOLED_ATTENTION_SOURCES = ["attention_pooled.cu", "runtime.cu"]
+KV4_SOURCES = ["attention_kv4.cu", "attention_kv4_prompt.cu", "runtime.cu"]
 HEADERS = ["common.cuh"]
 
 
@@ -301,7 +302,7 @@ def kv4_library(head_dim: int) -> ctypes.CDLL:
     one head size when a cache of that kind is first used."""
     if head_dim % 32 != 0 or not 32 <= head_dim <= 256:
         raise BuildError(f"the 4-bit cache takes head sizes 32..256 in steps of 32, not {head_dim}")
-    return load_library(f"kv4_hd{head_dim}", ["attention_kv4.cu", "runtime.cu"], {"CO_HEAD_DIM": head_dim})
+    return load_library(f"kv4_hd{head_dim}", KV4_SOURCES, {"CO_HEAD_DIM": head_dim})
 
 
 def recurrent_library() -> ctypes.CDLL:
@@ -389,7 +390,7 @@ def build_all(head_dims: Sequence[int] = (16, 32, 64, 128)) -> List[str]:
         paths.append(build_library(f"maps_{dk}_{dv}_{maps}", ["attention_maps_tc.cu", "runtime.cu"],
                                    {"CO_MAPS_DK": dk, "CO_MAPS_DV": dv, "CO_MAPS_N": maps}))
     for hd in (64, 128):
-        paths.append(build_library(f"kv4_hd{hd}", ["attention_kv4.cu", "runtime.cu"], {"CO_HEAD_DIM": hd}))
+        paths.append(build_library(f"kv4_hd{hd}", KV4_SOURCES, {"CO_HEAD_DIM": hd}))
     for hd in head_dims:
         paths.append(build_library(f"attn_hd{hd}", ["attention_bf16.cu", "attention_tc.cu", "runtime.cu"],
                                    {"CO_HEAD_DIM": hd}))

@@ -2269,6 +2269,7 @@ def kv4_lib(head_dim: int):
         lib.coheryn_last_error.restype = ctypes.c_char_p
         lib.coheryn_launch_count.restype = ctypes.c_ulonglong
         lib.coheryn_kv4_scratch_floats.restype = c_long
+        lib.coheryn_kv4_prompt_scratch_floats.restype = c_long
         if lib.coheryn_kv4_head_dim() != head_dim:
             raise KernelError(f"the library of the 4-bit cache was built for head size {lib.coheryn_kv4_head_dim()}, not {head_dim}")
         _kv4_libs[head_dim] = lib
@@ -2446,10 +2447,11 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             _check(lib, rc)
     if longest <= limit:
         return
-    # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.
+    # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
+    # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages.
     width = min(W, -(-max_kv_len // page_size))
     most = max(1, min(65535, KV4_EXPAND_BYTES // max(1, width * num_kv_heads * page_size * head_dim * 4)))
-    prompt = attention_lib(head_dim)
+    half = bool(lib.coheryn_kv4_prompt_takes(c_int(num_heads), c_int(num_kv_heads), c_int(page_size))) and scale > 0
     b = 0
     while b < B:
         e = b
@@ -2458,19 +2460,30 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         if e == b:
             b += 1
             continue
-        n = e - b
-        k = torch.empty((n * width, num_kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
-        v = torch.empty_like(k)
-        table = torch.empty((n, width), dtype=torch.int32, device=q.device)
+        n, rows = e - b, max(q_lens[b:e]) * G
+        k, v = q.new_empty((2, n * width, num_kv_heads, page_size, head_dim)).unbind(0)       # (16 bits a value, whichever kind)
+        table = block_tables.new_empty((n, width))
+        factors = torch.empty(2 + 2 * 128, dtype=torch.float32, device=q.device) if half else None
         cu, lens = cu_q.data_ptr() + 4 * b, kv_lens.data_ptr() + 4 * b
-        rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiippippppp")(
+        rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiippipppppp")(
             k_cache.data_ptr(), v_cache.data_ptr(), num_pages, num_kv_heads, page_size, block_tables.data_ptr() + 4 * W * b, W, width, n, cu, lens,
-            window or 0, k.data_ptr(), v.data_ptr(), table.data_ptr(), status, stream)
+            window or 0, k.data_ptr(), v.data_ptr(), table.data_ptr(), _at(factors), status, stream)
         if rc:
             _check(lib, rc)
-        rows = max(q_lens[b:e]) * G
-        _check(prompt, prompt.coheryn_attention_bf16(
-            c_void_p(q_at), c_long(q_ld), c_void_p(out_at), c_long(out_ld), _ptr(k), _ptr(v), _ptr(table), c_int(width), c_void_p(cu), c_void_p(lens),
-            c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
-            c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * width), c_int(0), c_void_p(stream)))
+        if half:
+            parts = int(lib.coheryn_kv4_prompt_parts(c_int(num_heads), c_int(num_kv_heads), c_int(n), c_int(sum(q_lens[b:e])), c_int(rows),
+                                                     c_int(max_kv_len), c_int(window or 0)))
+            floats = int(lib.coheryn_kv4_prompt_scratch_floats(c_int(num_heads), c_int(num_kv_heads), c_int(n), c_int(rows), c_int(parts)))
+            scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+            rc = _entry(lib, "coheryn_kv4_prompt", "pliplppipippiiiiifipiplpp")(
+                q_at, q_ld, T, out_at, out_ld, k.data_ptr(), v.data_ptr(), n * width, table.data_ptr(), width, cu, lens, n, num_heads, num_kv_heads,
+                page_size, window or 0, scale, rows, factors.data_ptr(), parts, _at(scratch), floats, status, stream)
+            if rc:
+                _check(lib, rc)
+        else:
+            prompt = attention_lib(head_dim)
+            _check(prompt, prompt.coheryn_attention_bf16(
+                c_void_p(q_at), c_long(q_ld), c_void_p(out_at), c_long(out_ld), _ptr(k), _ptr(v), _ptr(table), c_int(width), c_void_p(cu), c_void_p(lens),
+                c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
+                c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * width), c_int(0), c_void_p(stream)))
         b = e
