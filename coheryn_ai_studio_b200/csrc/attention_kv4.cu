@@ -327,8 +327,8 @@ kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   const long long items = (long long)n * width * nkv;
   for (long long x = (long long)blockIdx.x * 8 + warp; x < items; x += RANGE_BLOCKS * 8) {
     const int kvh = (int)(x % nkv), j = (int)(x / nkv % width), b = (int)(x / nkv / width);
-    const int rows = rows_needed(cu_q, lens, b, j, page_size, window), page = rows ? table[(size_t)b * table_ld + j] : -1;
-    if (page < 0 || page >= num_pages) continue;
+    const int page = table[(size_t)b * table_ld + j], rows = rows_needed(cu_q, lens, b, j, page_size, window);    // (asked for at once)
+    if (rows == 0 || page < 0 || page >= num_pages) continue;
     for (int tile = 0; tile < per_page && tile * 16 < rows; ++tile) {
       const size_t at = tile_at(page, nkv, kvh, page_size, tile * 16) + CODES;
       for (int i = lane; i < 16 * NG; i += 32) {         // keys: row i / NG
@@ -372,6 +372,9 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   co_pdl_wait();
   const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
   const long long entry = (long long)b * width + j;
+  // The loads that depend on nothing first: a block lives for little more than its chain of them.
+  const int page = table[(size_t)b * table_ld + j];
+  int valid = lens ? rows_needed(cu_q, lens, b, j, page_size, window) : page_size;      // rows of the page that hold something
   float k_by = 1.f, v_by = 1.f;
   if constexpr (HALF) {             // float16: times the powers of two that the largest values ask for
     static_assert(RANGE_BLOCKS == 128, "a thread per partial answer");
@@ -385,20 +388,15 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     v_by = v2.x;
     if (j == 0 && kvh == 0 && b == 0 && threadIdx.x == 0) { factors[0] = k2.y; factors[1] = v2.y; }
   }
-  int valid = page_size;                           // rows of the page that hold something
-  if (lens) {
-    valid = rows_needed(cu_q, lens, b, j, page_size, window);
-    if (!valid) {
-      if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
-      return;
-    }
+  if (!valid) {
+    if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
+    return;
   }
-  const int page = table[(size_t)b * table_ld + j];
   const bool known = page >= 0 && page < num_pages;
   if (!known) valid = 0;
   if (kvh == 0 && threadIdx.x == 0) {
     if (out_table) out_table[entry] = known ? (int)entry : -1;
-    if (!known && status) *status = BAD_INDEX;
+    if (status && (!known || (lens && lens[b] > width * page_size))) *status = BAD_INDEX;      // (or the table ends before the request)
   }
   T* ko = k_out + ((size_t)entry * nkv + kvh) * page_size * HD;
   T* vo = v_out + ((size_t)entry * nkv + kvh) * page_size * HD;

@@ -234,7 +234,8 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const unsigned col_s = 128 * t, col_o = 256 + 128 * t;
     if (n_tiles > 0 && active) {
       // The row of Q to float16, its largest element brought to 1..2; the rows beyond the tile's whole tokens, which were not
-      // fetched, to zeros, so that their scores are 0 and their threads walk the same path as the others.
+      // fetched, to zeros, so that their scores are 0 and their threads walk the same path as the others.  Pieces in an order of
+      // the row's own, so that the lanes do not meet in the same banks.
       if (!mbar_wait(q_full, 0)) { if (lane == 0) atomicExch(status, 37); ok = false; }
       unsigned char* q_row = q_s + t * TILE_BYTES + row * 128;
       float most = 0.f;
@@ -242,7 +243,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       for (int c = 0; c < KCH; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(q_row + c * CHUNK_BYTES + i * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4));
           const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
@@ -254,7 +255,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       for (int c = 0; c < KCH; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint4* at = reinterpret_cast<uint4*>(q_row + c * CHUNK_BYTES + i * 16);
+          uint4* at = reinterpret_cast<uint4*>(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4));
           const uint4 v = row < RT ? *at : make_uint4(0, 0, 0, 0);
           unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -399,10 +400,10 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
 }
 
-// Joins the parts of every row, a warp per row, parts in ascending order.
+// Joins the parts of every row, a warp per row, parts in ascending order.  Bound by what the parts left (3 parts of 10,752 rows: 17 MB).
 __global__ void __launch_bounds__(256)
 kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out, long out_stride, const int* __restrict__ cu_q, Shape sh) {
-  constexpr int C = SUPPORTED ? HD / 32 : 1;         // columns per lane
+  constexpr int C = SUPPORTED ? HD / 32 : 2;         // neighbouring columns per lane: 2 or 4
   co_pdl_launch_dependents();
   const int rr = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z, G = sh.nh / sh.nkv, RT = 128 / G * G;
   co_pdl_wait();
@@ -414,21 +415,35 @@ kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out
   float M = -INFINITY, den = 0.f, acc[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  for (int p = lane; p < sh.parts; p += 32) M = fmaxf(M, base[(size_t)p * PART_FLOATS + 256 * HD + row * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  // The reference may still move: what has been added up is scaled when it does.
+#pragma unroll 4
   for (int p = 0; p < sh.parts; ++p) {
     const float* src = base + (size_t)p * PART_FLOATS;
     const float2 ml = *reinterpret_cast<const float2*>(src + 256 * HD + row * 2);
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    den += f * ml.y;
+    float x[C];
+    if constexpr (C == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src + row * HD + lane * 4);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(src + row * HD + lane * 2);
+      x[0] = v.x; x[1] = v.y;
+    }
+    const float N = fmaxf(M, ml.x), f = M == -INFINITY ? 0.f : exp2f(M - N), g = ml.x == -INFINITY ? 0.f : exp2f(ml.x - N);
+    M = N;
+    den = den * f + ml.y * g;
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] += f * src[row * HD + c * 32 + lane];
+    for (int c = 0; c < C; ++c) acc[c] = acc[c] * f + x[c] * g;
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  bf16* dst = out + (size_t)(tok0 + rr / G) * out_stride + (size_t)(kvh * G + rr % G) * HD;
+  bf16* dst = out + (size_t)(tok0 + rr / G) * out_stride + (size_t)(kvh * G + rr % G) * HD + lane * C;
+  unsigned w[C / 2];
 #pragma unroll
-  for (int c = 0; c < C; ++c) dst[c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
+  for (int c = 0; c < C / 2; ++c) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    w[c] = *reinterpret_cast<const unsigned*>(&v);
+  }
+  if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<unsigned*>(dst) = w[0];
 }
 
 int pairs_of(int nh, int nkv, int max_rows) {

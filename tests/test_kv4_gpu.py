@@ -257,6 +257,59 @@ def test_portions_in_pieces_and_direct_agree(rows, monkeypatch):
     check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, rounded_keys=(0, 1, 2))
 
 
+@pytest.mark.parametrize("heads,nkv,hd,window", [(8, 2, 64, None), (5, 1, 128, None), (14, 2, 64, 1500), (2, 2, 128, 700), (8, 2, 64, 2300)])
+def test_portions_late_in_long_prompts(heads, nkv, hd, window):
+    """Few row tiles and many keys: the key tiles are cut into parts for a CTA each; pairs of row tiles whose first sees a key tile less."""
+    q_lens, lens = [75, 1, 150], [3000, 40, 2049]
+    cache = Cache(12, lens, nkv, hd)
+    q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, window, 4, pad=1)
+    parts = ops().kv4_lib(hd).coheryn_kv4_prompt_parts(heads, nkv, 1, 150, 150 * heads // nkv, 3000, window or 0)
+    assert (parts > 1) == (window is None or window > 2000)          # eight key tiles per part at least
+    check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
+
+
+@pytest.mark.parametrize("scale", [1e-9, 3e-3, 1e6, 1e20])
+def test_keys_and_values_of_any_magnitude(scale):
+    """The tensor cores see powers of two times keys, values and queries: exact, whatever their magnitude."""
+    heads, nkv, hd, q_lens, lens = 4, 2, 64, [70, 1, 9], [200, 300, 30]
+    cache = Cache(13, lens, nkv, hd)
+    for t, values in ((cache.k_cache, False), (cache.v_cache, True)):
+        rows = kc.cache_rows(t.cpu().numpy(), values)
+        with np.errstate(invalid="ignore"):
+            tiles = (rows * scale).astype(np.float32).reshape(t.shape[0], nkv, 1, 16, hd)
+        t.copy_(torch.from_numpy(kc.pack(tiles, values)))
+    held = [kc.cache_rows(t.cpu().numpy(), v) for t, v in ((cache.k_cache, False), (cache.v_cache, True))]
+    for b, n in enumerate(lens):
+        pages = [p for p in cache.table[b] if p >= 0]
+        cache.k64[b], cache.v64[b] = (h[pages].transpose(0, 2, 1, 3).reshape(-1, nkv, hd)[:n] for h in held)
+    q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, q_spread=1.5 / scale)
+    check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16)
+
+
+def test_many_requests_of_all_lengths_share_the_cuts():
+    """More lists than clusters would hold: the units of all of them in equal shares, lists that begin and end inside a share."""
+    rng = np.random.default_rng(7)
+    lens = [int(x) for x in rng.integers(1, 900, 60)] + [2500, 0, 1]
+    q_lens = [1] * 60 + [1, 0, 1]
+    for heads, nkv, hd, window in ((4, 2, 64, None), (16, 8, 128, 300), (2, 1, 256, None)):
+        cache = Cache(20, lens, nkv, hd)
+        q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, window)
+        check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
+
+
+def test_rows_of_wider_buffers():
+    heads, nkv, hd, lens, q_lens = 4, 2, 64, [300, 90], [1, 70]
+    cache = Cache(2, lens, nkv, hd)
+    wide = torch.randn(71, heads * hd + 64, device=DEV).to(torch.bfloat16)
+    q, room = wide[:, 32:32 + heads * hd], torch.full((71, heads * hd + 16), 7.0, device=DEV, dtype=torch.bfloat16)
+    out = room[:, 8:8 + heads * hd]
+    cu = np.array([0, 1, 71])
+    ops().attention_kv4_rows(q, out, cache.k_cache, cache.v_cache, i32(cache.table), i32([0] + [1] * 70), i32([299] + list(range(20, 90))), heads, nkv, hd,
+                             16, None, hd ** -0.5, cu_q=i32(cu), kv_lens=i32(lens), q_lens=q_lens, max_kv_len=300)
+    check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16)
+    assert (room[:, :8] == 7).all() and (room[:, 8 + heads * hd:] == 7).all()
+
+
 def test_sharp_scores_and_a_long_context():
     """Scores in the hundreds (one key takes nearly all), over a context that is cut into many items."""
     lens, heads, nkv, hd = [9000, 5], 2, 1, 64
@@ -307,7 +360,8 @@ def test_a_row_without_keys_gives_zeros():
     assert (other[0] == 0).all()
 
 
-def test_captured_and_replayed_with_other_lengths_and_on_another_stream():
+@pytest.mark.parametrize("longest", [1024, 8192])        # parts joined in clusters, and by a kernel of their own
+def test_captured_and_replayed_with_other_lengths_and_on_another_stream(longest):
     o = ops()
     heads, nkv, hd, lens = 12, 2, 128, [900, 33, 400]
     cache = Cache(3, lens, nkv, hd)
@@ -317,7 +371,7 @@ def test_captured_and_replayed_with_other_lengths_and_on_another_stream():
 
     def call(to):
         o.attention_kv4_rows(q, to, cache.k_cache, cache.v_cache, table, req, pos, heads, nkv, hd, 16, None, hd ** -0.5, cu_q=cu, kv_lens=kv,
-                             q_lens=[1, 1, 1], max_kv_len=1024)
+                             q_lens=[1, 1, 1], max_kv_len=longest)
     call(out)
     torch.cuda.synchronize()
     graphs, outs = [], [torch.zeros_like(q) for _ in range(2)]
