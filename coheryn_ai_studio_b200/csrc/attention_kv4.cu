@@ -526,9 +526,10 @@ __device__ __forceinline__ float factor(float m, float M) { return m == -INFINIT
 // ------------------------------------------------------------------------------------
 // Attention in float32 arithmetic: any compute type, any alignment, any rows.  A CTA per (token, kv head, part of the visible tiles)
 // walks its tiles with its warps side by side; a lane has two halves of one key row for the scores and four channels of a group for
-// the sums.  HC heads of the group at a time share a tile's codes.  Bound by the latency of a warp's chain (28 tokens of 14 heads
-// over 2, 256 positions: 16.5 us with 8 warps and 4 heads at a time); so many warps, as many heads as fit the registers, and parts
-// (joined by a kernel after it) while there are fewer CTAs than the GPU holds.
+// the sums.  HC heads of the group at a time share a tile's codes.  Bound by the latency of a warp's chain; so many warps, as many
+// heads at a time as fit the registers (28 tokens of 14 heads over 2, 256 positions: 12.1 us by 8 heads, 14.2 by 4; 12 tokens of 32
+// over 8, 300 positions: 19.6 by 8, of which half idle, 14.7 by 4), and parts (joined by a kernel after it) while there are
+// fewer CTAs than the GPU holds.
 // ------------------------------------------------------------------------------------
 constexpr int SW = HD > 128 ? 8 : 16;        // warps
 constexpr int VU = (HD / 4 + 31) / 32;       // units of four channels per lane
@@ -731,8 +732,8 @@ kv4_simple_join_kernel(const float* __restrict__ scratch, int parts, T* __restri
 }
 
 // ------------------------------------------------------------------------------------
-// Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per item, four warps,
-// each with pairs of tiles of its own (pair i of the item goes to warp i mod 4) in a ring of its own that it fills with
+// Attention of few query rows per kv head (decoding, short runs) on mma.sync.m16n8k16: one CTA per share of the units, four warps,
+// each with pairs of tiles of its own (pair i of a list's share goes to warp i mod 4) in a ring of its own that it fills with
 // cp.async, so that warps never wait for one another before the end (bulk copies of whole tiles by one lane took more
 // instructions: their operands go through uniform registers).  Decoding is
 // bound by the cache's bytes, and with 5 bits a value nearly as much by the instructions that turn codes into operands,
@@ -747,7 +748,8 @@ kv4_simple_join_kernel(const float* __restrict__ scratch, int parts, T* __restri
 //    exact, but for elements under 2^-24 of it;
 //  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs).  The scale
 //    put on the probability instead takes fewer instructions but rounds p s, whose error meets s c and not s c + m;
-//  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory;
+//  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory, each as the sum
+//    of two bfloat16 terms: rounded to one they were the largest error of all (64 x 16,384 positions, 138 us instead of 147);
 //  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
 //    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
 //  * the values' product of a pair and the scores of the next stand in one run of code without a branch, so that a warp
@@ -1302,7 +1304,8 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 // Joins the parts of the lists' rows.  A warp takes every `step`-th eight of a row's parts, four channels per lane.  WIDE: one CTA
 // per row, its warps side by side over the parts, their sums added in order at the end; else one CTA per list and a warp per
 // row.  Bound by its chain of dependent reads (the list's note, then references and accumulators at once); with many
-// lists, of few parts each, by the number of CTAs.
+// lists, of few parts each, by the number of CTAs.  So WIDE where the lists have more parts than a warp reads at once (both kernels, us: 14
+// parts each, 224 rows, 16.0 wide, 17.1 by list; 9 parts, 512 rows, 29.9, 34.1; 7 parts, 448 rows, 23.0, 22.4; 2 parts, 1,792 rows, 29.0, 22.7).
 constexpr int CW = 8;
 template <bool WIDE>
 __global__ void __launch_bounds__(32 * CW)
@@ -1392,28 +1395,43 @@ kv4_join_kernel(const float* __restrict__ scratch, int ctas, bf16* __restrict__ 
 int tiles_of(int max_rows) { return max_rows <= 8 || HD > 128 ? 1 : 2; }
 // CTAs that are resident per SM, by their registers.
 constexpr int MOST = HD <= 128 ? 4 : 2, FEWER = HD <= 128 ? 3 : 2;
-// CTAs that cut the step's units: those that are resident at a time, or one per unit when there are fewer units.  One row tile: three CTAs per SM,
-// whose 168 registers let a warp work ahead, beat four of 128 where the shares are long (2 x 131,072 positions: 39.2 against
-// 42 us; 64 x up to 16,384: 138 against 140), four where every unit gets a CTA at once (8 x 4,096: 11.0 against 13.3).
-int ctas_of(int B, int nkv, int max_rows, int max_kv_len, int* per_sm = nullptr) {
-  const int nt = tiles_of(max_rows);
-  const long long lists = (long long)B * nkv * ((max_rows + 8 * nt - 1) / (8 * nt)), units = lists * (((long long)max_kv_len + 15) / UNIT + 1);
-  const int resident = nt == 2 ? 2 : units <= 148 * MOST ? MOST : FEWER;
-  if (per_sm) *per_sm = resident;
-  return (int)(units < 148 * resident ? units : 148 * resident);
-}
 
-// CTAs per list when clusters join the lists (0: a kernel after it does): while all of them are resident at once and a CTA gets two
-// units at most, so that the second kernel's start and its chain of reads are what counts (1 x 700 positions: 6.7 us against 8.2; 8 x 4,096,
-// up to three units per CTA of 16: 12.1 against 11.6).
-int cluster_of(int B, int nkv, int max_rows, int max_kv_len) {
+// How a step's units get their CTAs.
+//  * A cluster per list, while every cluster is resident at once and a CTA gets four units at most: one kernel, and no chain of reads through
+//    memory after it.  Against equal shares, heads 32 over 8, one token each (us): 1 x 900 positions 6.2 (7.9), 4 x 1,900 9.0 (11.3),
+//    8 x 1,900 11.9 (16.5), 24 x 900 13.3 (18.3); four tokens each of heads 28 over 4, 4 x 1,900 12.1 (24.0).  A list has its CTAs to itself, so
+//    one long list beside short ones may lose: 8 requests of 100 positions but one of 1,900, 10.0 (9.2).
+//    Clusters as large as are resident, and no larger than gives every CTA a unit (1 x 200: 5.8 with two CTAs, 6.7 with four).  A cluster lies
+//    in one GPC, whose last SMs it may not fill: 64 clusters of 4 run at once at two CTAs per SM, 72 do not (11.9 against 19.3 us at
+//    1,900 positions), 104 do at three per SM, 112 do not.  Sixteen pay for four lists and more than eight units (1,900: 6.8 against 7.5),
+//    no more (8 lists: 8.1 against 7.6).  More than two units per CTA only where the equal shares would give an SM several too
+//    (8 lists of 3,900: 9.3 against 9.1; 32 lists: 11.5 against 15.4).
+//  * Equal shares otherwise, one per resident CTA.  Three CTAs per SM, whose 168 registers let a warp work ahead, beat four of 128 (2 x 131,072,
+//    28 heads over 4: 45.4 against 48.5; 64 x 8,192: 78 against 85), but where four give every unit a CTA at once (24 x 700: 12.6 against 14.6).
+struct Split {
+  int csize;       // CTAs of the cluster that has a list to itself; 0: all units in equal shares, joined by a kernel after it
+  int per_sm;      // resident CTAs per SM, for which the kernel is built
+  int ctas;
+};
+Split split_of(int B, int nkv, int max_rows, int max_kv_len) {
   const int nt = tiles_of(max_rows);
   const long long lists = (long long)B * nkv * ((max_rows + 8 * nt - 1) / (8 * nt));
-  const int units = (max_kv_len + 15) / UNIT + 1;
-  if (HD > 128 || nt != 1 || units < 2) return 0;
-  for (int c : {16, 8})
-    if (lists * c <= 148 * MOST && units <= 2 * c) return c;
-  return 0;
+  const int units = max(1, (int)((max_kv_len + UNIT - 1LL) / UNIT));         // of a list, at most
+  if (units > 1) {
+    int c = 0, per_sm = 2;
+    if (HD <= 128 && lists <= 4 && units > 8) c = 16;
+    for (int x : {8, 4, 2})
+      if (c == 0 && lists * x <= 256) c = x;
+    for (int x : {8, 4, 2})
+      if (FEWER == 3 && nt == 1 && c < 8 && x > c && lists * x <= 416) { c = x; per_sm = 3; break; }
+    if (c) {
+      while (c > 2 && units <= c / 2) c /= 2;
+      if (units <= 4 * c && (units <= 2 * c || lists * units > 148 * 2)) return {c, per_sm, (int)(lists * c)};
+    }
+  }
+  const long long all = lists * units;
+  const int per_sm = nt == 2 ? 2 : all > 148 * FEWER && all <= 148 * MOST ? MOST : FEWER;
+  return {0, per_sm, (int)(all < 148 * per_sm ? all : 148 * per_sm)};
 }
 
 template <int NT, int PER_SM, bool CLUSTER>
@@ -1546,11 +1564,13 @@ CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, 
   return 0;
 }
 
-// Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests that it takes.
+// Floats of scratch that coheryn_kv4_attention needs; max_rows: the largest q_len * heads / kv_heads among the requests
+// that it takes, max_kv_len: the most positions that one's rows see, from a multiple of 16 on.
 CO_EXPORT long coheryn_kv4_scratch_floats(int B, int nkv, int max_rows, int max_kv_len) {
-  if (cluster_of(B, nkv, max_rows, max_kv_len)) return 0;
+  const Split split = split_of(B, nkv, max_rows, max_kv_len);
+  if (split.csize) return 0;
   const int cols = 8 * tiles_of(max_rows);
-  return 2L * ctas_of(B, nkv, max_rows, max_kv_len) * cols * (HD + 2) + 2L * B * nkv * ((max_rows + cols - 1) / cols);
+  return 2L * split.ctas * cols * (HD + 2) + 2L * B * nkv * ((max_rows + cols - 1) / cols);
 }
 
 // Attention of the requests with at most `max_rows` query rows per kv head, in bfloat16: q [T, nh * HD] of stride q_ld, out likewise;
@@ -1565,20 +1585,21 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   if ((q_ld & 7) || (out_ld & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15))
     CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
   if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
-  if ((long long)B * nkv * ((max_rows + 7) / 8) * ((max_kv_len + 15LL) / UNIT + 1) > 0x7fffffffLL)
+  if ((long long)B * nkv * ((max_rows + 7) / 8) * (max_kv_len / UNIT + 1LL) > 0x7fffffffLL)
     CO_FAIL("kv4_attention: %d requests of %d positions and %d kv heads", B, max_kv_len, nkv);
-  int per_sm = 0;
-  const int nt = tiles_of(max_rows), csize = cluster_of(B, nkv, max_rows, max_kv_len);
-  const int ctas = csize ? B * nkv * ((max_rows + 7) / 8) * csize : ctas_of(B, nkv, max_rows, max_kv_len, &per_sm);
+  const Split split = split_of(B, nkv, max_rows, max_kv_len);
+  const int nt = tiles_of(max_rows), ctas = split.ctas, csize = split.csize;
   if (scratch_floats < coheryn_kv4_scratch_floats(B, nkv, max_rows, max_kv_len) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_attention: the scratch is too small or not 16-byte aligned");
-  auto launch = csize ? launch_items<1, MOST, true> : nt == 2 ? launch_items<HD <= 128 ? 2 : 1, 2, false>
-                : per_sm == MOST ? launch_items<1, MOST, false> : launch_items<1, FEWER, false>;
+  constexpr int NT = HD <= 128 ? 2 : 1;
+  auto launch = nt == 2 ? (csize ? launch_items<NT, 2, true> : launch_items<NT, 2, false>)
+                : csize ? (split.per_sm == 2 ? launch_items<1, 2, true> : launch_items<1, FEWER, true>)
+                : split.per_sm == MOST ? launch_items<1, MOST, false> : launch_items<1, FEWER, false>;
   const int rc = launch(q, q_ld, out, out_ld, k_cache, v_cache, num_pages, table, table_ld, cu_q, kv_lens, B, nh, nkv, page_size, window,
                         scale * 1.4426950408889634f, max_rows, ctas, csize ? csize : 1, scratch, status, stream);
-  if (rc || csize || max_kv_len + 15 <= UNIT) return rc;    // joined already, or no list is longer than one unit
+  if (rc || csize || max_kv_len <= UNIT) return rc;    // joined already, or no list is longer than one unit
   const int cols = 8 * nt;
-  const bool wide = (long long)B * nkv * max_rows <= 148 * 4;
+  const bool wide = ctas > 8LL * B * nkv * ((max_rows + cols - 1) / cols);
   co_launch(wide ? kv4_join_kernel<true> : kv4_join_kernel<false>, dim3((unsigned)(wide ? max_rows : (max_rows + cols - 1) / cols), (unsigned)nkv, (unsigned)B),
             dim3(32 * CW), 0, stream, (const float*)scratch, ctas, (bf16*)out, out_ld, cu_q, nh, nkv, cols, max_rows);
   CO_CHECK_LAUNCH("kv4_join");

@@ -213,14 +213,16 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int *cu_q = c.words(a[16], B + 1), *kv_lens = c.words(a[17], B);
     if (!c.ok || B < 1 || B > 65535 || tt.size(0) != B || longest < 1 || longest * G > most || longest_kv < 0) return none();
     if (q->stride(0) % 8 || (uintptr_t)q->data_ptr() % 16 || out->stride(0) % 4 || (uintptr_t)out->data_ptr() % 8) return none();
+    // The positions that a request's rows see, from a multiple of 16 on: by these the kernel's units are counted.
+    const long seen = window > 0 ? std::min(longest_kv, window + longest + 14) : longest_kv;
     typedef long (*Scratch)(int, int, int, int);
-    const long floats = ((Scratch)address(a[0]))((int)B, (int)nkv, (int)(longest * G), (int)longest_kv);
+    const long floats = ((Scratch)address(a[0]))((int)B, (int)nkv, (int)(longest * G), (int)seen);
     at::Tensor scratch = at::empty({floats}, q->options().dtype(at::kFloat));
     typedef int (*Fn)(const void*, long, void*, long, const void*, const void*, int, const int*, int, const int*, const int*, int, int, int, int, int, float,
                       int, int, float*, long, int*, void*);
     return PyLong_FromLong(((Fn)address(a[1]))(q->data_ptr(), (long)q->stride(0), out->data_ptr(), (long)out->stride(0), k, v, (int)pages, table,
                                                (int)tt.size(1), cu_q, kv_lens, (int)B, (int)nh, (int)nkv, (int)page_size, (int)window, scale,
-                                               (int)(longest * G), (int)longest_kv, (float*)scratch.data_ptr(), floats, status, c.stream()));
+                                               (int)(longest * G), (int)seen, (float*)scratch.data_ptr(), floats, status, c.stream()));
   });
 }
 

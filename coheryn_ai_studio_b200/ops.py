@@ -642,11 +642,11 @@ def describe_status(code: int) -> str:
     """What a non-zero device status word means."""
     if code in STATUS_MESSAGES:
         return STATUS_MESSAGES[code]
-    if 11 <= code <= 40:
+    if 11 <= code <= 39:
         return (f"a kernel gave up a bounded wait and left its output unfinished (code {code}: 11-14 tensor-core product: "
                 "producer, MMA issuer, epilogue, split of float32 operands; 12 and 13 also the matrix memory in chunks: MMA issuer, the "
                 "others; 19 self-test; 31-39 prompt attention: 31 producer, 32-36 MMA issuer, "
-                "37-39 softmax; 40 attention over a 4-bit cache)")
+                "37-39 softmax)")
     return f"device status {code}"
 
 
@@ -2252,8 +2252,10 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
 _kv4_libs = {}
 
 # Requests with at most this many query rows (tokens times heads of a group) read the 4-bit pages directly; longer portions
-# have their pages expanded to bfloat16 once and go through the prompt kernels.
-KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "64"))
+# have their pages expanded to 16 bits a value once and go through the prompt kernels.  Directly against expanded, in us: 112 rows
+# of 7 heads over each of 4, 1 x 1,024 positions 10 and 28, 8 x 8,192 103 and 120; 128 rows, 4 over each of 8, 1 x 65,536 210 and 221,
+# 8 x 1,024 52 and 43; 256 rows, 1 x 65,536 399 and 248.
+KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "128"))
 
 # The expanded pages of a call take at most about this many bytes at a time (one request always goes in one piece).
 KV4_EXPAND_BYTES = 1 << 30
@@ -2385,8 +2387,8 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros.
     bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
     ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``KV4_DIRECT_ROWS`` rows per kv
-    head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to bfloat16 and
-    go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
+    head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
+    value and go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
     if not force_simple and q.is_cuda:
         lib = kv4_lib(head_dim)
         rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
@@ -2437,11 +2439,12 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     longest = max(q_lens)
     direct = longest if longest <= limit else max((n for n in q_lens if n <= limit), default=0)
     if direct:
-        floats = _kv4_scratch_floats(head_dim, B, num_kv_heads, direct * G, max_kv_len)
+        seen = min(max_kv_len, window + direct + 14) if window else max_kv_len        # positions, from a multiple of 16 on
+        floats = _kv4_scratch_floats(head_dim, B, num_kv_heads, direct * G, seen)
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         rc = _entry(lib, "coheryn_kv4_attention", "plplppipippiiiiifiiplpp")(
             q_at, q_ld, out_at, out_ld, k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W, cu_q.data_ptr(),
-            kv_lens.data_ptr(), B, num_heads, num_kv_heads, page_size, window or 0, scale, direct * G, max_kv_len, scratch.data_ptr(), floats,
+            kv_lens.data_ptr(), B, num_heads, num_kv_heads, page_size, window or 0, scale, direct * G, seen, scratch.data_ptr(), floats,
             status, stream)
         if rc:
             _check(lib, rc)

@@ -526,6 +526,23 @@ def test_steps_of_layout_write_and_attention(dtype):
             assert (err <= tol).all(), (q_lens, b, float((err / tol).max()))
 
 
+# How lists get their CTAs: clusters of 16, 8, 4 and 2 (also of three CTAs per SM), two row tiles, lists that end early, long ones beside short.
+@pytest.mark.parametrize("requests,heads,nkv,hd,tokens,longest", [
+    (1, 4, 2, 64, 1, 1500), (1, 14, 2, 128, 3, 1100), (3, 2, 1, 32, 1, 2048), (9, 8, 2, 64, 1, 900), (16, 8, 2, 128, 1, 700), (20, 8, 2, 32, 1, 1000),
+    (24, 16, 4, 96, 1, 450), (26, 8, 4, 128, 1, 500), (40, 8, 4, 64, 1, 250), (70, 2, 2, 128, 1, 600), (3, 6, 2, 256, 2, 1000), (30, 4, 2, 160, 1, 500),
+    (5, 12, 2, 64, 5, 700), (16, 7, 1, 128, 9, 300)])
+@pytest.mark.parametrize("window", [None, 130])
+def test_lists_of_clusters(requests, heads, nkv, hd, tokens, longest, window):
+    rng = np.random.default_rng(requests * longest)
+    q_lens = [int(x) for x in rng.integers(0, tokens + 1, requests)]
+    q_lens[0] = tokens
+    lens = [int(n + rng.integers(0, longest - n + 1)) for n in q_lens]
+    lens[0], lens[-1] = longest, max(q_lens[-1], 1)
+    cache = Cache(31, lens, nkv, hd)
+    q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, window, 5, pad=1)
+    check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
+
+
 # ------------------------------------------------------------------------------------ refusals
 def test_refusals():
     o = ops()
