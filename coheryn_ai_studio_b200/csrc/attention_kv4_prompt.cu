@@ -7,13 +7,20 @@
 // (found on the device), a query row by its own that brings its largest to 1..2.  That is exact but for what lies under 2^-24 of the
 // largest.  The factors meet again in the exponent's factor and in the last division.
 //
-// The arrangement is that of the framework's two-tile prompt kernel: a CTA owns two consecutive tiles of TOK = 128 / G tokens times
-// the G heads of a group (rows r = token * G + head) and fetches every tile of 128 keys once for both.  Warp 0 fetches (two K
-// stages, one V stage), one thread of warp 1 issues the MMAs (S_A, S_B, O_A, O_B fill the 512 columns of tensor memory),
-// warps 2..5 and 6..9 are the softmax of a tile, one thread per row; a row's probabilities go to shared memory as operand A of P V.
-// What is its own: the conversion of Q in place, and PARTS: where a step has few pairs of tiles and each sees many keys (a portion late in
-// a long prompt), the key tiles of a pair are cut into parts for a CTA each, which leave (reference, sum, accumulator) in the
-// scratch for a kernel that joins them.  384 tokens after 8,191 beside 15 decoding requests, 28 heads over 4: 44 pairs on 148 SMs.
+// The arrangement is near that of the framework's two-tile prompt kernel: a CTA owns two consecutive tiles of TOK = 128 / G tokens times
+// the G heads of a group (rows r = token * G + head) and fetches every tile of 128 keys once for both.  Warp 0 fetches Q and
+// the keys (two stages), warp 11 the values (one), a thread of warp 1 and one of warp 10 issue the MMAs of a tile each (S_A, S_B, O_A, O_B
+// fill the 512 columns of tensor memory), warps 2..5 and 6..9 are the softmax of a tile, one thread per row; a row's
+// probabilities go to shared memory as operand A of P V.  Its own are:
+//  * the conversion of Q in place;
+//  * turns: the tiles' exponentials alternate, so that one tile's run while the other's scores are fetched and its products
+//    made (2,048 tokens of 28 heads over 4, the whole call: 60 us, 62 without; 384 after 8,191: 102, 109);
+//  * two multiply-adds, or sums, an instruction (61 against 65 us);
+//  * PARTS: where a step has few pairs of tiles and each sees many keys (a portion late in a long prompt), the key tiles of a pair
+//    are cut into parts for a CTA each, which leave (reference, sum, accumulator) in the scratch for a kernel that joins them.
+//    384 tokens after 8,191 beside 15 decoding requests, 28 heads over 4: 44 pairs on 148 SMs.
+// Bound by a warp's chain: of the 4,100 cycles that a pair of key tiles takes, 2 x 1,480 are exponentials (2 x 1,024 the unit's own
+// time), the products 2,048; before the first and after the last tile a CTA takes 5,400 and 6,000.
 // Every wait is bounded: on expiry the kernel records a code in `status` and winds down.
 #include <cuda_fp16.h>
 
@@ -48,12 +55,45 @@ __device__ __forceinline__ unsigned pack_half(float a, float b) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
+// Shared memory by its own address: through a pointer, whose alignment by hand hides where it points, these become generic accesses.
+__device__ __forceinline__ uint4 ld_shared(unsigned at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two at a time: a b + c, a + b.
+__device__ __forceinline__ unsigned long long pair_f32(unsigned lo, unsigned hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2 of_pair(unsigned long long v) {
+  unsigned lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+
 struct Shape {
-  int nh, nkv, page_size, cache_rows, window, rows_per_box, n_req, pairs, parts, table_ld;
+  int G, TOK, nkv, page_size, cache_rows, window, rows_per_box, n_req, pairs, parts, table_ld;
   float scale_log2;
 };
 
-__global__ void __launch_bounds__(320, 1)
+constexpr int THREADS = 384;
+__global__ void __launch_bounds__(THREADS, 1)
 kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   bf16* __restrict__ out, long out_stride, const int* __restrict__ block_tables, const int* __restrict__ cu_q,
                   const int* __restrict__ kv_lens, const float* __restrict__ factors, Shape sh, float* __restrict__ scratch,
@@ -75,15 +115,17 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   unsigned long long* s_free = s_full + 2;          // [tile] softmax -> MMA: S is in registers (one arrival per warp)
   unsigned long long* p_full = s_free + 2;          // [tile] softmax -> MMA: P written, O rescaled (one arrival per warp)
   unsigned long long* pv_done = p_full + 2;         // [tile] MMA -> softmax: O += P V is complete
-  unsigned* tmem_slot = (unsigned*)(pv_done + 2);
-  static_assert((5 + 2 * K_STAGES + 8) * 8 + 4 <= 256, "barriers fit their slot");
+  unsigned long long* turn = pv_done + 2;           // [tile][quarter] the other tile's warp is through with its exponentials
+  unsigned* tmem_slot = (unsigned*)(turn + 8);
+  static_assert((5 + 2 * K_STAGES + 16) * 8 + 4 <= 256, "barriers fit their slot");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1); mbar_init(v_full, 1); mbar_init(v_empty, 1);
-    for (int s = 0; s < K_STAGES; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    mbar_init(q_full, 1); mbar_init(v_full, 1); mbar_init(v_empty, 2);
+    for (int s = 0; s < K_STAGES; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 2); }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_ready[t], 4); mbar_init(&s_full[t], 1); mbar_init(&s_free[t], 4); mbar_init(&p_full[t], 4); mbar_init(&pv_done[t], 1);
+      for (int x = 0; x < 4; ++x) mbar_init(&turn[4 * t + x], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -99,26 +141,27 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   co_pdl_wait();
 
   // Late rows see the most keys: their pairs of tiles are started first, for all (request, kv head) before any earlier pair.
-  const int part = (int)(blockIdx.x % sh.parts), unit = (int)(blockIdx.x / sh.parts), heads_reqs = sh.nkv * sh.n_req;
-  const int kvh = unit % sh.nkv, pair = sh.pairs - 1 - unit / heads_reqs, b = (unit % heads_reqs) / sh.nkv;
-  const int G = sh.nh / sh.nkv, TOK = 128 / G, RT = TOK * G;
+  const unsigned unit = blockIdx.x / (unsigned)sh.parts, request = unit / (unsigned)sh.nkv, late = request / (unsigned)sh.n_req;
+  const int part = (int)(blockIdx.x - unit * sh.parts), kvh = (int)(unit - request * sh.nkv), b = (int)(request - late * sh.n_req);
+  const int pair = sh.pairs - 1 - (int)late, G = sh.G, TOK = sh.TOK, RT = TOK * G;
   const int tok0 = cu_q[b], q_len = cu_q[b + 1] - tok0, kv_len = kv_lens[b];
   const int rows = q_len * G;
   const bool active_a = 2 * pair * RT < rows, active_b = (2 * pair + 1) * RT < rows;
   const int base_pos = kv_len - q_len;
   const int first_a = 2 * pair * RT, first_b = first_a + RT;
-  const int last_a = min(rows, first_a + RT) - 1, last_b = min(rows, first_b + RT) - 1;
-  const int key_first = sh.window > 0 ? max(0, base_pos + first_a / G - sh.window + 1) : 0, tile_first = key_first / BN;
-  const int pos_hi_a = base_pos + last_a / G, pos_hi_b = base_pos + last_b / G;      // (a request shorter than its rows: negative ones see nothing)
+  const int token_a = 2 * pair * TOK, token_b = token_a + TOK;
+  const int key_first = sh.window > 0 ? max(0, base_pos + token_a - sh.window + 1) : 0, tile_first = key_first / BN;
+  const int pos_hi_a = base_pos + min(q_len, token_a + TOK) - 1, pos_hi_b = base_pos + min(q_len, token_b + TOK) - 1;      // (a request shorter than its rows: negative ones see nothing)
   const int all_a = active_a && pos_hi_a >= 0 ? pos_hi_a / BN - tile_first + 1 : 0;  // key tiles of tile A, of tile B
   const int all_b = active_b && pos_hi_b >= 0 ? pos_hi_b / BN - tile_first + 1 : 0;
   const int all = all_a > all_b ? all_a : all_b;
   const int j0 = (int)((long long)all * part / sh.parts), j1 = (int)((long long)all * (part + 1) / sh.parts);      // of this part
   const int n_a = max(0, min(all_a, j1) - j0), n_b = max(0, min(all_b, j1) - j0), n_tiles = n_b > n_a ? n_b : n_a;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 11) {
+    // Warp 0 fetches Q and the keys, warp 11 the values.
     if (n_tiles > 0) {
-      if (lane == 0) {
+      if (warp == 0 && lane == 0) {
         mbar_expect_tx(q_full, (unsigned)(KCH * RT * 128 * (active_b ? 2 : 1)));
         for (int t = 0; t < (active_b ? 2 : 1); ++t)
           for (int c = 0; c < KCH; ++c)
@@ -145,31 +188,24 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (lane == 0 && !mbar_wait(bar, parity)) { atomicExch(status, 31); ok = 0; }
         return __shfl_sync(0xffffffffu, ok, 0) != 0;
       };
-      // K runs one tile ahead of V: K(0), then K(i + 1) and V(i).
-      int row_v = box_row(0), row_k = box_row(1);
-      fetch(&map_k, k_s, row_v, &k_full[0]);
-      bool ok = true;
-      for (int i = 0; i < n_tiles && ok; ++i) {
-        const int row_next = box_row(i + 2);
-        if (i + 1 < n_tiles) {
-          const int s = (i + 1) % K_STAGES;
-          if (i + 1 >= K_STAGES) ok = wait_for(&k_empty[s], (unsigned)(((i + 1) / K_STAGES) - 1) & 1);
-          if (!ok) break;
-          fetch(&map_k, k_s + (size_t)s * TILE_BYTES, row_k, &k_full[s]);
-        }
-        if (i >= 1) ok = wait_for(v_empty, (unsigned)(i - 1) & 1);
-        if (!ok) break;
-        fetch(&map_v, v_s, row_v, v_full);
-        row_v = row_k; row_k = row_next;
+      const bool keys = warp == 0;
+      const int stages = keys ? K_STAGES : 1;
+      int row = box_row(0);
+      for (int i = 0; i < n_tiles; ++i) {
+        const int row_next = box_row(i + 1), stage = i % stages;
+        if (i >= stages && !wait_for(keys ? &k_empty[stage] : v_empty, (unsigned)(i / stages - 1) & 1)) break;
+        if (keys) fetch(&map_k, k_s + (size_t)stage * TILE_BYTES, row, &k_full[stage]);
+        else fetch(&map_v, v_s, row, v_full);
+        row = row_next;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 10) {
+    // The MMAs of tile A, of tile B: neither waits for the other's softmax.
     if (lane == 0 && n_tiles > 0) {
+      const int t = warp == 1 ? 0 : 1, mine = t ? n_b : n_a;
       constexpr unsigned idesc_qk = umma_idesc(128, BN) & FLOAT16;
       constexpr unsigned idesc_pv = umma_idesc_b_mn(128, HD) & FLOAT16;
-      bool ok = mbar_wait(&q_ready[0], 0) && (!active_b || mbar_wait(&q_ready[1], 0));
-      if (!ok) atomicExch(status, 32);
-      auto issue_qk = [&](int t, int j) {        // S_t = Q_t K(j)^T; K(j) has landed and S_t is free
+      auto issue_qk = [&](int j) {        // S = Q K(j)^T; K(j) has landed and S is free
         const unsigned char* k_src = k_s + (size_t)(j % K_STAGES) * TILE_BYTES;
 #pragma unroll
         for (int c = 0; c < KCH; ++c) {
@@ -179,7 +215,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         umma_commit(&s_full[t]);
       };
-      auto issue_pv = [&](int t, int j) {        // O_t += P_t V(j); P and V(j) have been waited for
+      auto issue_pv = [&](int j) {        // O += P V(j); P and V(j) have been waited for
         const unsigned long long dv = umma_desc_offsets(v_s, CHUNK_BYTES, 1024);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk) {   // 16 positions: 32 bytes along a row of P (64 per chunk), 16 rows of V further
@@ -188,34 +224,32 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         umma_commit(&pv_done[t]);
       };
+      // Both issuers go through every stage, so that each of its barriers' phases has two arrivals, also where one has no more tiles.
+      bool ok = mine == 0 || mbar_wait(&q_ready[t], 0);
+      if (!ok) atomicExch(status, 32);
       if (ok && !mbar_wait(&k_full[0], 0)) { atomicExch(status, 33); ok = false; }
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (n_a > 0) issue_qk(0, 0);
-        if (n_b > 0) issue_qk(1, 0);
+        if (mine > 0) issue_qk(0);
         umma_commit(&k_empty[0]);
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
         // The next scores first: they wait only for the softmax threads to hold S(j) in registers.
         if (j + 1 < n_tiles) {
           if (!mbar_wait(&k_full[(j + 1) % K_STAGES], (unsigned)((j + 1) / K_STAGES) & 1)) { atomicExch(status, 33); ok = false; break; }
-          for (int t = 0; t < 2 && ok; ++t)
-            if (j + 1 < (t ? n_b : n_a)) {
-              if (!mbar_wait(&s_free[t], (unsigned)j & 1)) { atomicExch(status, 34); ok = false; break; }
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              issue_qk(t, j + 1);
-            }
-          if (!ok) break;
+          if (j + 1 < mine) {
+            if (!mbar_wait(&s_free[t], (unsigned)j & 1)) { atomicExch(status, 34); ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            issue_qk(j + 1);
+          }
           umma_commit(&k_empty[(j + 1) % K_STAGES]);
         }
-        for (int t = 0; t < 2 && ok; ++t)
-          if (j < (t ? n_b : n_a)) {
-            if (!mbar_wait(&p_full[t], (unsigned)j & 1)) { atomicExch(status, 35); ok = false; break; }
-            if (!mbar_wait(v_full, (unsigned)j & 1)) { atomicExch(status, 36); ok = false; break; }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            issue_pv(t, j);
-          }
-        if (!ok) break;
+        if (j < mine && !mbar_wait(&p_full[t], (unsigned)j & 1)) { atomicExch(status, 35); ok = false; break; }
+        if (!mbar_wait(v_full, (unsigned)j & 1)) { atomicExch(status, 36); ok = false; break; }
+        if (j < mine) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          issue_pv(j);
+        }
         umma_commit(v_empty);
       }
     }
@@ -237,40 +271,41 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // fetched, to zeros, so that their scores are 0 and their threads walk the same path as the others.  Pieces in an order of
       // the row's own, so that the lanes do not meet in the same banks.
       if (!mbar_wait(q_full, 0)) { if (lane == 0) atomicExch(status, 37); ok = false; }
-      unsigned char* q_row = q_s + t * TILE_BYTES + row * 128;
+      const unsigned q_row = smem_u32(q_s + t * TILE_BYTES + row * 128);
+      uint4 v[KCH][8];
       float most = 0.f;
 #pragma unroll
       for (int c = 0; c < KCH; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4));
-          const unsigned w[4] = {v.x, v.y, v.z, v.w};
+          v[c][i] = ld_shared(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4));
+          const unsigned w[4] = {v[c][i].x, v[c][i].y, v[c][i].z, v[c][i].w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
         }
       const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);          // 2^(e - 127) <= most
-      const float down = row < RT ? __uint_as_float((unsigned)(254 - e) << 23) : 0.f;
+      const float down = __uint_as_float((unsigned)(254 - e) << 23);
       row_scale = sh.scale_log2 * factors[0] * __uint_as_float((unsigned)e << 23);
 #pragma unroll
       for (int c = 0; c < KCH; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint4* at = reinterpret_cast<uint4*>(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4));
-          const uint4 v = row < RT ? *at : make_uint4(0, 0, 0, 0);
-          unsigned w[4] = {v.x, v.y, v.z, v.w};
+          unsigned w[4] = {v[c][i].x, v[c][i].y, v[c][i].z, v[c][i].w};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = pack_half(__uint_as_float(w[x] << 16) * down, __uint_as_float(w[x] & 0xffff0000u) * down);
-          *at = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int x = 0; x < 4; ++x)
+            w[x] = row < RT ? pack_half(__uint_as_float(w[x] << 16) * down, __uint_as_float(w[x] & 0xffff0000u) * down) : 0u;
+          st_shared(q_row + c * CHUNK_BYTES + ((i ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
         }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[t]);
     }
     if (my_tiles > 0) {
-      unsigned char* p_row = p_s + t * P_BYTES + row * 128;
+      const unsigned p_row = smem_u32(p_s + t * P_BYTES + row * 128);
+      // Rows that are not kept see everything, so that they take no part in the choice of the path below.
       const int pos = base_pos + (row_first + row) / G;
-      const int hi = valid ? pos : -1;
-      const int lo = sh.window > 0 ? max(0, pos - sh.window + 1) : 0;
+      const int hi = valid ? pos : 0x7fffffff;
+      const int lo = valid && sh.window > 0 ? max(0, pos - sh.window + 1) : 0;
       for (int j = 0; j < my_tiles && ok; ++j) {
         if (!mbar_wait(&s_full[t], (unsigned)j & 1)) { if (lane == 0) atomicExch(status, 37); ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -283,21 +318,25 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (lane == 0) mbar_arrive(&s_free[t]);
         const int key0 = (tile_first + j0 + j) * BN;
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (!valid || (key0 + BN - 1 <= hi && key0 >= lo)) {
+        const int hi_col = hi - key0, lo_col = lo - key0;        // columns lo_col..hi_col are seen
+        if (!__all_sync(0xffffffffu, hi_col >= BN - 1 && lo_col <= 0)) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[i][c]));
-        } else {
+            for (int c = 0; c < 32; ++c)
+              if (i * 32 + c > hi_col) sr[i][c] = __float_as_uint(-INFINITY);
+          if (sh.window > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int key = key0 + i * 32 + c;
-              if (key > hi || key < lo) sr[i][c] = __float_as_uint(-INFINITY);
-              mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[i][c]));
-            }
+              for (int c = 0; c < 32; ++c)
+                if (i * 32 + c < lo_col) sr[i][c] = __float_as_uint(-INFINITY);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[i][c]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         // The reference m follows the running maximum lazily (p stays below 2^8, far inside float16's range), and the warp
         // decides together, because rescaling O is a warp-wide access to tensor memory.
@@ -323,27 +362,35 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_wait_st();
           }
         }
+        // The tiles' warps of an SM's quarter take turns at the exponentials, A(j) B(j) A(j + 1) ..: together they would wait together, too.
+        const int before = t ? j : j - 1;            // the other tile's step whose exponentials come before these
+        if (before >= 0 && before < (t ? n_a : n_b) && !mbar_wait(&turn[4 * t + quarter], (unsigned)before & 1)) {
+          if (lane == 0) atomicExch(status, 38);
+          ok = false;
+          break;
+        }
         // Exponentials, 32 columns at a time, each group packed and stored at once: row `row` of chunk i / 2 of the P tile,
         // 16-byte piece c at c ^ (row % 8).
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        const unsigned scale_bits = __float_as_uint(row_scale), use_bits = __float_as_uint(-m_use);
+        const unsigned long long scale2 = pair_f32(scale_bits, scale_bits), use2 = pair_f32(use_bits, use_bits);
+        unsigned long long sum2[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           unsigned pr[16];
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            sr[i][c] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(sr[i][c]), row_scale, -m_use)));
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float p0 = __uint_as_float(sr[i][c]), p1 = __uint_as_float(sr[i][c + 1]);
-            sum4[(c >> 1) & 3] += p0 + p1;
-            pr[c >> 1] = pack_half(p0, p1);
+          for (int c = 0; c < 16; ++c) {
+            const float2 x = of_pair(fma2(pair_f32(sr[i][2 * c], sr[i][2 * c + 1]), scale2, use2));
+            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+            sum2[c & 3] = add2(sum2[c & 3], pair_f32(__float_as_uint(p0), __float_as_uint(p1)));
+            pr[c] = pack_half(p0, p1);
           }
-          unsigned char* dst = p_row + (i >> 1) * CHUNK_BYTES;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(dst + ((((i & 1) * 4 + c) ^ (row & 7)) << 4)) = make_uint4(pr[4 * c], pr[4 * c + 1], pr[4 * c + 2], pr[4 * c + 3]);
+            st_shared(p_row + (i >> 1) * CHUNK_BYTES + ((((i & 1) * 4 + c) ^ (row & 7)) << 4), pr[4 * c], pr[4 * c + 1], pr[4 * c + 2], pr[4 * c + 3]);
         }
-        l = l * corr + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        if (lane == 0) mbar_arrive(&turn[4 * (1 - t) + quarter]);
+        const float2 all = of_pair(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])));
+        l = l * corr + (all.x + all.y);
         m = m_new;
         fence_proxy_async();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -356,38 +403,60 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
     if (active && ok) {
-      const int rr = row_first + row;
+      // Rows leave by way of the tile's probabilities' place, 64 columns at a time: written by a thread a row each, every store to memory
+      // would meet 32 rows (9,500 cycles a CTA instead of 6,000).
       const float v_factor = factors[1];
       const float mul = sh.parts > 1 ? v_factor : l == 0.f ? 0.f : v_factor / l;
-      float* part_row = scratch + (size_t)blockIdx.x * PART_FLOATS + (t * 128 + row) * HD;
       if (sh.parts > 1 && valid)
         *reinterpret_cast<float2*>(scratch + (size_t)blockIdx.x * PART_FLOATS + 256 * HD + (t * 128 + row) * 2) = make_float2(m, l);
-      bf16* orow = out + (size_t)(tok0 + rr / G) * out_stride + (size_t)(kvh * G + rr % G) * HD;
+      const int token = (row_first + row) / G;
+      const long long place = !valid ? -1
+                              : sh.parts > 1 ? (long long)blockIdx.x * PART_FLOATS + (t * 128 + row) * HD
+                                             : (long long)(tok0 + token) * out_stride + (kvh * G + row_first + row - token * G) * HD;
+      const unsigned stage = smem_u32(p_s + t * P_BYTES);
 #pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += 32) {
-        unsigned o[32];
-        if (my_tiles > 0) {
-          tmem_ld32(lane_addr + col_o + c0, o);     // warp-collective: invalid rows read too, and skip the store
-        } else {
+      for (int c0 = 0; c0 < HD; c0 += 64) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = 0;
+        for (int h = 0; h < 2; ++h) {
+          unsigned o[32];
+          if (my_tiles > 0) {
+            tmem_ld32(lane_addr + col_o + c0 + 32 * h, o);     // warp-collective
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = 0;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * mul);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            st_shared(stage + row * 256 + (((h * 8 + c) ^ (row & 7)) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
         }
-        if (valid && sh.parts > 1) {
+        __syncwarp();
+        const int piece = lane & 15;
+        uint4 v[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<float4*>(part_row + c0 + c) = make_float4(__uint_as_float(o[c]) * mul, __uint_as_float(o[c + 1]) * mul,
-                                                                        __uint_as_float(o[c + 2]) * mul, __uint_as_float(o[c + 3]) * mul);
-        } else if (valid) {
+        for (int i = 0; i < 16; ++i) {
+          const int r = quarter * 32 + 2 * i + (lane >> 4);
+          v[i] = ld_shared(stage + r * 256 + ((piece ^ (r & 7)) << 4));
+        }
+        if (sh.parts > 1) {
+          float* to = scratch + c0 + piece * 4;
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(o[c]) * mul, __uint_as_float(o[c + 1]) * mul);
-            __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[c + 2]) * mul, __uint_as_float(o[c + 3]) * mul);
-            uint2 raw;
-            raw.x = *reinterpret_cast<unsigned*>(&x);
-            raw.y = *reinterpret_cast<unsigned*>(&y);
-            *reinterpret_cast<uint2*>(orow + c0 + c) = raw;
+          for (int i = 0; i < 16; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, place, 2 * i + (lane >> 4));
+            if (at >= 0) *reinterpret_cast<uint4*>(to + at) = v[i];
+          }
+        } else {
+          bf16* to = out + c0 + piece * 4;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, place, 2 * i + (lane >> 4));
+            const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[i].x), __uint_as_float(v[i].y));
+            const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(v[i].z), __uint_as_float(v[i].w));
+            if (at >= 0) *reinterpret_cast<uint2*>(to + at) = make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
           }
         }
+        __syncwarp();
       }
     }
   }
@@ -405,7 +474,7 @@ __global__ void __launch_bounds__(256)
 kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out, long out_stride, const int* __restrict__ cu_q, Shape sh) {
   constexpr int C = SUPPORTED ? HD / 32 : 2;         // neighbouring columns per lane: 2 or 4
   co_pdl_launch_dependents();
-  const int rr = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z, G = sh.nh / sh.nkv, RT = 128 / G * G;
+  const int rr = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z, G = sh.G, RT = sh.TOK * G;
   co_pdl_wait();
   const int tok0 = cu_q[b], rows = (cu_q[b + 1] - tok0) * G;
   if (rr >= rows) return;
@@ -486,7 +555,7 @@ CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens,
   if (parts < 1 || scratch_floats < coheryn_kv4_prompt_scratch_floats(nh, nkv, n, max_rows, parts) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_prompt: %d parts in a scratch of %ld floats", parts, scratch_floats);
   const int G = nh / nkv, TOK = 128 / G;
-  const Shape sh{nh, nkv, page_size, (int)cache_rows, window, page_size >= BN ? BN : page_size, n, pairs_of(nh, nkv, max_rows), parts, table_ld,
+  const Shape sh{G, TOK, nkv, page_size, (int)cache_rows, window, page_size >= BN ? BN : page_size, n, pairs_of(nh, nkv, max_rows), parts, table_ld,
                  scale * 1.4426950408889634f};
   CUtensorMap mq, mk, mv;
   {
@@ -503,7 +572,7 @@ CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens,
   }
   cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) CO_FAIL("kv4_prompt: %d bytes of shared memory: %s", SMEM_BYTES, cudaGetErrorString(e));
-  co_launch(kv4_prompt_kernel, dim3((unsigned)ctas), dim3(320), (size_t)SMEM_BYTES, stream, mq, mk, mv, (bf16*)out, out_stride, block_tables, cu_q, kv_lens,
+  co_launch(kv4_prompt_kernel, dim3((unsigned)ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, mq, mk, mv, (bf16*)out, out_stride, block_tables, cu_q, kv_lens,
             factors, sh, scratch, status);
   CO_CHECK_LAUNCH("kv4_prompt");
   if (parts > 1) {
