@@ -446,15 +446,19 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 // list and go on with the next; what a CTA has of a list that it does not hold whole goes to the scratch, at place
 // 2 * CTA for the list that its share begins in and 2 * CTA + 1 for the one that it begins inside the share.  Whoever has a
 // list's first unit notes its number of parts and the place of the first for the kernel that joins them.
+// A list costs its CTAs about EXTRA units more than its positions (its queries, the first tiles' way, the warps' meeting), and counts as
+// longer by so much, in front of its first unit: else the shares that hold many short lists finish last (64 requests of 40 heads over 8
+// and every length up to 16,384: 135 us, 149 without; of 28 over 4, up to 8,000: 47.5, 69).  Not where there is a CTA for every unit.
 // ------------------------------------------------------------------------------------
-constexpr int UNIT = 128;
+constexpr int UNIT = 128, EXTRA = 2;
 
 struct Cut {                       // of one request
   int tok0, q_len, kv_len;
   int lo16, units;                 // first tile of 16 positions; units from there on, at least one if there are rows
+  int span;                        // units and what a list costs besides
   int row_tiles;                   // 0: the request is not for this kernel
 };
-__device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b, int G, int rows_per_tile, int max_rows, int window) {
+__device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b, int G, int rows_per_tile, int max_rows, int window, int extra) {
   Cut c;
   c.tok0 = cu_q[b];
   c.q_len = cu_q[b + 1] - c.tok0;
@@ -464,16 +468,21 @@ __device__ __forceinline__ Cut cut_of(const int* cu_q, const int* kv_lens, int b
   c.lo16 = first >> 4;
   c.row_tiles = rows > 0 && rows <= max_rows ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
   c.units = c.row_tiles ? max(1, (c.kv_len - c.lo16 * 16 + UNIT - 1) / UNIT) : 0;
+  c.span = c.row_tiles ? c.units + extra : 0;
   return c;
 }
-// All units of the step.  One warp; all lanes get the answer.
-__device__ __forceinline__ int all_units(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows, int window) {
-  int total = 0;
+// The length of all lists together, and in `extra` what every one counts beside its units.  One warp; all lanes get the answer.
+__device__ __forceinline__ int all_units(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows, int window,
+                                         int& extra) {
+  int units = 0, lists = 0;
   for (int b = threadIdx.x & 31; b < B; b += 32) {
-    const Cut c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
-    total += c.units * c.row_tiles * nkv;
+    const Cut c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window, 0);
+    units += c.units * c.row_tiles * nkv;
+    lists += c.row_tiles * nkv;
   }
-  return __reduce_add_sync(0xffffffffu, total);
+  units = __reduce_add_sync(0xffffffffu, units);
+  extra = units <= (int)gridDim.x ? 0 : EXTRA;
+  return units + extra * __reduce_add_sync(0xffffffffu, lists);
 }
 // The shares: share i of `shares` is units [share_start(i), share_start(i + 1)).
 __device__ __forceinline__ int share_start(int i, int shares, int total) { return (int)((long long)total * i / shares); }
@@ -486,16 +495,16 @@ struct Place {                     // a unit's request, and the request's first 
 };
 // One warp; all lanes get the answer.
 __device__ __forceinline__ Place find_unit(const int* cu_q, const int* kv_lens, int B, int nkv, int G, int rows_per_tile, int max_rows,
-                                           int window, int unit, int b_from, int first) {
+                                           int window, int extra, int unit, int b_from, int first) {
   const int lane = threadIdx.x & 31;
   Place p;
   p.b = -1;
   int before = first;
   for (int b0 = b_from; b0 < B && p.b < 0; b0 += 32) {
     const int b = b0 + lane;
-    Cut c = {0, 0, 0, 0, 0, 0};
-    if (b < B) c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window);
-    const int mine = c.units * c.row_tiles * nkv;
+    Cut c = {0, 0, 0, 0, 0, 0, 0};
+    if (b < B) c = cut_of(cu_q, kv_lens, b, G, rows_per_tile, max_rows, window, extra);
+    const int mine = c.span * c.row_tiles * nkv;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -514,6 +523,7 @@ __device__ __forceinline__ Place find_unit(const int* cu_q, const int* kv_lens, 
       p.cut.lo16 = __shfl_sync(0xffffffffu, c.lo16, src);
       p.cut.units = __shfl_sync(0xffffffffu, c.units, src);
       p.cut.row_tiles = __shfl_sync(0xffffffffu, c.row_tiles, src);
+      p.cut.span = p.cut.units + extra;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
@@ -1003,20 +1013,20 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
   co_pdl_wait();
   co_pdl_launch_dependents();
   const int G = nh / nkv;
-  int total = 0, shares = 0, unit = 0, unit_end = 0;
+  int total = 0, shares = 0, unit = 0, unit_end = 0, extra = 0;
   Place at;
   const int most_tiles = (max_rows + COLS - 1) / COLS, own_list = CLUSTER ? (int)blockIdx.x / csize : 0, rank = CLUSTER ? (int)blockIdx.x % csize : 0;
   if constexpr (CLUSTER) {
     at.b = own_list / (nkv * most_tiles);
-    at.cut = cut_of(cu_q, kv_lens, at.b, G, COLS, max_rows, window);
+    at.cut = cut_of(cu_q, kv_lens, at.b, G, COLS, max_rows, window, 0);
     if (own_list % most_tiles >= at.cut.row_tiles) return;      // the whole cluster
   } else {
-    total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window);
+    total = all_units(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, extra);
     shares = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= shares) return;
     unit = share_start(blockIdx.x, shares, total);
     unit_end = share_start(blockIdx.x + 1, shares, total);
-    at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, 0, 0);
+    at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, extra, unit, 0, 0);
   }
   unsigned char* ring = smem + (size_t)warp * RING;       // keys, then values
   const unsigned ring_lane = smem_u32(ring) + lane * 16;
@@ -1024,16 +1034,18 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 
   for (bool first_list = true; at.b >= 0; first_list = false) {
     const Cut c = at.cut;
-    int row_tile, kvh, u_first, u_end;
+    int row_tile, kvh, u_first, u_end, s_first = 0, s_end = 0;
     if constexpr (CLUSTER) {
       row_tile = own_list % most_tiles;
       kvh = own_list / most_tiles % nkv;
       u_first = share_start(rank, csize, c.units);
       u_end = share_start(rank + 1, csize, c.units);
     } else {
-      const int list = (unit - at.first) / c.units;
-      u_first = unit - at.first - list * c.units;
-      u_end = min(c.units, u_first + unit_end - unit);
+      const int list = (unit - at.first) / c.span;
+      s_first = unit - at.first - list * c.span;
+      s_end = min(c.span, s_first + unit_end - unit);
+      u_first = max(0, s_first - extra);
+      u_end = max(0, s_end - extra);
       row_tile = list % c.row_tiles;
       kvh = list / c.row_tiles;
     }
@@ -1235,12 +1247,12 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     float* acc_out = scratch + (size_t)slot * COLS * HD;
     float2* ml_out = reinterpret_cast<float2*>(scratch + (size_t)2 * gridDim.x * COLS * HD) + (size_t)slot * COLS;
     float* left = merge + (size_t)WARPS * COLS * MLD;          // for the cluster: a row's channels, reference and sum
-    if (!CLUSTER && tid == 0 && u_first == 0) {
+    if (!CLUSTER && tid == 0 && s_first == 0) {
       int2* heads = reinterpret_cast<int2*>(scratch + (size_t)2 * gridDim.x * COLS * (HD + 2));
       heads[((size_t)at.b * nkv + kvh) * most_tiles + row_tile] =
-          make_int2(share_of(unit + c.units - 1, shares, total) - (int)blockIdx.x + 1, slot);
+          make_int2(share_of(unit + c.span - 1, shares, total) - (int)blockIdx.x + 1, slot);
     }
-    const bool whole_list = !CLUSTER && u_first == 0 && u_end == c.units;
+    const bool whole_list = !CLUSTER && s_first == 0 && s_end == c.span;
     for (int x = tid; x < rows * (HD / 4); x += 32 * WARPS) {
       const int r = x / (HD / 4), ch = x % (HD / 4) * 4;
       float M = NOTHING, den = 0.f;
@@ -1293,11 +1305,11 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
       cluster_barrier();               // nobody leaves while its part may still be read
       return;
     }
-    unit += u_end - u_first;
+    unit += s_end - s_first;
     if (unit >= unit_end) return;
     __syncthreads();                 // the meeting becomes the rings again
-    if (unit - at.first >= c.units * c.row_tiles * nkv)
-      at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, unit, at.b + 1, unit);
+    if (unit - at.first >= c.span * c.row_tiles * nkv)
+      at = find_unit(cu_q, kv_lens, B, nkv, G, COLS, max_rows, window, extra, unit, at.b + 1, unit);
   }
 }
 
@@ -1585,7 +1597,7 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   if ((q_ld & 7) || (out_ld & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15))
     CO_FAIL("kv4_attention: q and the caches must be 16-byte aligned, out 8-byte");
   if (max_kv_len < 0 || B > 65535) CO_FAIL("kv4_attention: %d requests of at most %d positions", B, max_kv_len);
-  if ((long long)B * nkv * ((max_rows + 7) / 8) * (max_kv_len / UNIT + 1LL) > 0x7fffffffLL)
+  if ((long long)B * nkv * ((max_rows + 7) / 8) * (max_kv_len / UNIT + 1LL + EXTRA) > 0x7fffffffLL)
     CO_FAIL("kv4_attention: %d requests of %d positions and %d kv heads", B, max_kv_len, nkv);
   const Split split = split_of(B, nkv, max_rows, max_kv_len);
   const int nt = tiles_of(max_rows), ctas = split.ctas, csize = split.csize;

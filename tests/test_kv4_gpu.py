@@ -543,6 +543,21 @@ def test_lists_of_clusters(requests, heads, nkv, hd, tokens, longest, window):
     check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
 
 
+# More units of 128 positions than CTAs: shares that begin and end inside lists, in front of their first unit too, and hold many short ones.
+@pytest.mark.parametrize("requests,heads,nkv,hd,tokens,longest", [
+    (200, 8, 4, 64, 1, 300), (150, 4, 4, 128, 1, 700), (10, 8, 8, 32, 2, 9000), (60, 10, 5, 96, 2, 1200), (90, 3, 3, 256, 1, 600), (40, 14, 2, 64, 4, 2500)])
+@pytest.mark.parametrize("window", [None, 200])
+def test_shares_across_lists(requests, heads, nkv, hd, tokens, longest, window):
+    rng = np.random.default_rng(requests + longest)
+    q_lens = [int(x) for x in rng.integers(0, tokens + 1, requests)]
+    q_lens[-1] = tokens
+    lens = [int(n + (longest - n) * rng.random() ** 3) for n in q_lens]
+    lens[requests // 2] = longest
+    cache = Cache(37, lens, nkv, hd)
+    q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, window, 7, pad=1)
+    check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
+
+
 # ------------------------------------------------------------------------------------ refusals
 def test_refusals():
     o = ops()
