@@ -448,7 +448,8 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 // list's first unit notes its number of parts and the place of the first for the kernel that joins them.
 // A list costs its CTAs about EXTRA units more than its positions (its queries, the first tiles' way, the warps' meeting), and counts as
 // longer by so much, in front of its first unit: else the shares that hold many short lists finish last (64 requests of 40 heads over 8
-// and every length up to 16,384: 135 us, 149 without; of 28 over 4, up to 8,000: 47.5, 69).  Not where there is a CTA for every unit.
+// and every length up to 16,384: 135 us, 149 without; of 28 over 4, up to 8,000: 47.5, 69).  Not where there is a CTA for every unit, nor
+// where every list is one unit.
 // ------------------------------------------------------------------------------------
 constexpr int UNIT = 128, EXTRA = 2;
 
@@ -481,8 +482,9 @@ __device__ __forceinline__ int all_units(const int* cu_q, const int* kv_lens, in
     lists += c.row_tiles * nkv;
   }
   units = __reduce_add_sync(0xffffffffu, units);
-  extra = units <= (int)gridDim.x ? 0 : EXTRA;
-  return units + extra * __reduce_add_sync(0xffffffffu, lists);
+  lists = __reduce_add_sync(0xffffffffu, lists);
+  extra = units <= (int)gridDim.x || units == lists ? 0 : EXTRA;      // (lists of one unit each are not cut)
+  return units + extra * lists;
 }
 // The shares: share i of `shares` is units [share_start(i), share_start(i + 1)).
 __device__ __forceinline__ int share_start(int i, int shares, int total) { return (int)((long long)total * i / shares); }
@@ -547,7 +549,7 @@ constexpr int VU = (HD / 4 + 31) / 32;       // units of four channels per lane
 template <typename T, int HC>
 __global__ void __launch_bounds__(32 * SW)
 kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long out_ld, const unsigned char* __restrict__ k_cache,
-                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ table, int table_ld,
+                  const unsigned char* __restrict__ v_cache, int num_pages, const int* __restrict__ table, int table_ld, int n_req,
                   const int* __restrict__ token_req, const int* __restrict__ positions, int nh, int nkv, int page_size, int window,
                   float scale_log2, float* __restrict__ scratch, int* __restrict__ status) {
   __shared__ __align__(16) float qs[HC][HD];
@@ -557,8 +559,13 @@ kv4_simple_kernel(const T* __restrict__ q, long q_ld, T* __restrict__ out, long 
   co_pdl_wait();
   const int token = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z, parts = gridDim.z, G = nh / nkv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int pos = positions[token];
-  const int* pages = table + (size_t)token_req[token] * table_ld;
+  int pos = positions[token];
+  const int req = token_req[token];
+  if (req < 0 || req >= n_req) {
+    if (tid == 0 && status) *status = BAD_INDEX;
+    pos = -1;                          // sees nothing
+  }
+  const int* pages = table + (size_t)(pos < 0 ? 0 : req) * table_ld;
   const int lo = window > 0 ? max(0, pos - window + 1) : 0, first = lo >> 4, tiles = pos < 0 ? 0 : (pos >> 4) - first + 1;
   const int tile_first = first + (int)((long long)tiles * part / parts), tile_end = first + (int)((long long)tiles * (part + 1) / parts);
   for (int h0 = 0; h0 < G; h0 += HC) {
@@ -1549,7 +1556,7 @@ CO_EXPORT int coheryn_kv4_simple_parts(int T, int nkv, int max_kv_len, int windo
 CO_EXPORT long coheryn_kv4_simple_scratch_floats(int T, int nh, int parts) { return parts > 1 ? (long)T * nh * parts * (HD + 2) : 0; }
 
 CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, long out_ld, int dtype, const void* k_cache, const void* v_cache,
-                                           int num_pages, const int* table, int table_ld, const int* token_req, const int* positions, int T,
+                                           int num_pages, const int* table, int table_ld, int n_req, const int* token_req, const int* positions, int T,
                                            int nh, int nkv, int page_size, int window, float scale, int parts, float* scratch,
                                            long scratch_floats, int* status, cudaStream_t stream) {
   if (T <= 0) return 0;
@@ -1563,7 +1570,7 @@ CO_EXPORT int coheryn_kv4_attention_simple(const void* q, long q_ld, void* out, 
     typedef decltype(x) P;
     typedef std::remove_pointer_t<P> E;
     co_launch(nh / nkv <= 4 ? kv4_simple_kernel<E, 4> : kv4_simple_kernel<E, 8>, dim3((unsigned)T, (unsigned)nkv, (unsigned)parts), dim3(32 * SW), 0,
-              stream, (P)q, q_ld, (P)out, out_ld, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, token_req,
+              stream, (P)q, q_ld, (P)out, out_ld, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, table, table_ld, n_req, token_req,
               positions, nh, nkv, page_size, window, scale_log2, scratch, status);
     co_count_launch();
     if (parts > 1)

@@ -186,7 +186,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!c.ok || code != out_code || q->size(0) != out->size(0) || q->size(0) < 1) return none();
     const long T = (long)q->size(0);
     const at::Tensor& tt = THPVariable_Unpack(a[7]);
-    if (tt.dim() != 2 || tt.size(1) > 0x7fffffffL) return none();
+    if (tt.dim() != 2 || tt.size(0) > 0x7fffffffL || tt.size(1) > 0x7fffffffL) return none();
     const float scale = (float)PyFloat_AS_DOUBLE(a[15]);
     if (code == 0) {
       int *req = c.words(a[8], T), *pos = c.words(a[9], T);
@@ -197,10 +197,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const long floats = parts > 1 ? T * nh * parts * (hd + 2) : 0;
       at::Tensor scratch;
       if (floats) scratch = at::empty({floats}, q->options().dtype(at::kFloat));
-      typedef int (*Fn)(const void*, long, void*, long, int, const void*, const void*, int, const int*, int, const int*, const int*, int, int, int, int, int,
+      typedef int (*Fn)(const void*, long, void*, long, int, const void*, const void*, int, const int*, int, int, const int*, const int*, int, int, int, int, int,
                         float, int, float*, long, int*, void*);
       return PyLong_FromLong(((Fn)address(a[2]))(q->data_ptr(), (long)q->stride(0), out->data_ptr(), (long)out->stride(0), code, k, v, (int)pages, table,
-                                                 (int)tt.size(1), req, pos, (int)T, (int)nh, (int)nkv, (int)page_size, (int)window, scale, parts,
+                                                 (int)tt.size(1), (int)tt.size(0), req, pos, (int)T, (int)nh, (int)nkv, (int)page_size, (int)window, scale, parts,
                                                  floats ? (float*)scratch.data_ptr() : nullptr, floats, status, c.stream()));
     }
     if (!PyList_Check(a[18]) || a[16] == Py_None || a[17] == Py_None || a[19] == Py_None) return none();

@@ -98,10 +98,10 @@ step_layout_kernel(const int* __restrict__ starts, const int* __restrict__ q_len
       if (kv_lens) kv_lens[b] = s + q;
       int first, from, n;
       const bool ok = list_of(lists, b, first, from, n);
-      if (s < 0 || (long long)s + q > 0x7fffffffLL) bad = BAD_LENGTH;
+      if (s < 0 || (long long)s + q > 0x7fffffffLL || cu[b + 1] < cu[b]) bad = BAD_LENGTH;      // (the last: offsets beyond 32 bits)
       else if (!ok || (n && (long long)first + n > W)) bad = BAD_PAGES;
     }
-    if (tid == 0 && cu[B] > T) bad = BAD_LENGTH;
+    if (tid == 0 && (slots || positions || token_req) && cu[B] > T) bad = BAD_LENGTH;
   }
   const int tokens = min(cu[B], T);
   const int t0 = blockIdx.x * TOKENS_PER_BLOCK;

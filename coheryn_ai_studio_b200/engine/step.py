@@ -353,8 +353,10 @@ class StepRunner:
         return ctx, rows
 
     def _context(self, lay: _Layout):
-        # (a model without paged caches has no tables to make)
-        return self._device_context(lay) if self.device.type == "cuda" and lay.tables else self._host_context(lay)
+        # (a model without paged caches has no tables to make; wanted rows are requests of a step of their own)
+        if self.device.type == "cuda" and lay.tables and max(lay.B, len(lay.rows)) <= ops.STEP_LAYOUT_REQUESTS:
+            return self._device_context(lay)
+        return self._host_context(lay)
 
     def _host_context(self, lay: _Layout):
         tables, host_tables = [], []

@@ -2197,6 +2197,9 @@ def _calls():
     return _calls_module
 
 
+STEP_LAYOUT_REQUESTS = 11999      # that one call of step_layout takes at most (csrc/step_layout.cu keeps their offsets in 48 KB)
+
+
 def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tensor, pages: torch.Tensor, page_size: int,
                 block_table: torch.Tensor, slots: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
                 kv_lens: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -2423,9 +2426,9 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         parts = int(lib.coheryn_kv4_simple_parts(c_int(T), c_int(num_kv_heads), c_int(max_kv_len or 0), c_int(window or 0)))
         floats = T * num_heads * parts * (head_dim + 2) if parts > 1 else 0
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipippiiiiifiplpp")(
+        rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipiippiiiiifiplpp")(
             q_at, q_ld, out_at, out_ld, _code(q), k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W,
-            token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, parts, _at(scratch), floats,
+            block_tables.shape[0], token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, parts, _at(scratch), floats,
             status, stream)
         if rc:
             _check(lib, rc)

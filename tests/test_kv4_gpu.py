@@ -477,6 +477,11 @@ def test_step_layout_of_lengths_that_do_not_fit():
     assert code == 52 and table == [[1, 2, 3, 4]]
     code, (slots, _, _), _ = call([0], [1], [0, 1], [2 ** 31 - 1], 1)                     # a slot beyond 32 bits
     assert code == 52 and slots == [-1]
+    assert call([0, 0], [2 ** 31 - 1] * 2, [0, 1, 2], [5, 6], 2)[0] == 51                # offsets beyond 32 bits
+    table, status = torch.full((2, 3), 77, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    cu_q = torch.full((3,), 77, dtype=torch.int32, device=DEV)
+    o.step_layout(i32([0, 3]), i32([2, 4]), i32([0, 1, 2]), i32([5, 6]), 16, table, cu_q=cu_q, status=status)      # no array of tokens
+    assert int(status) == 0 and cu_q.tolist() == [0, 2, 6] and table.tolist() == [[5, -1, -1], [6, -1, -1]]
     with pytest.raises(o.KernelError, match="requests"):
         call([0] * 12000, [0] * 12000, [0] * 12001, [0], 0)
 
@@ -545,7 +550,8 @@ def test_lists_of_clusters(requests, heads, nkv, hd, tokens, longest, window):
 
 # More units of 128 positions than CTAs: shares that begin and end inside lists, in front of their first unit too, and hold many short ones.
 @pytest.mark.parametrize("requests,heads,nkv,hd,tokens,longest", [
-    (200, 8, 4, 64, 1, 300), (150, 4, 4, 128, 1, 700), (10, 8, 8, 32, 2, 9000), (60, 10, 5, 96, 2, 1200), (90, 3, 3, 256, 1, 600), (40, 14, 2, 64, 4, 2500)])
+    (200, 8, 4, 64, 1, 300), (150, 4, 4, 128, 1, 700), (10, 8, 8, 32, 2, 9000), (60, 10, 5, 96, 2, 1200), (90, 3, 3, 256, 1, 600), (40, 14, 2, 64, 4, 2500),
+    (300, 8, 4, 64, 1, 120), (180, 12, 2, 128, 5, 128)])
 @pytest.mark.parametrize("window", [None, 200])
 def test_shares_across_lists(requests, heads, nkv, hd, tokens, longest, window):
     rng = np.random.default_rng(requests + longest)
@@ -556,6 +562,19 @@ def test_shares_across_lists(requests, heads, nkv, hd, tokens, longest, window):
     cache = Cache(37, lens, nkv, hd)
     q, out, cu = run_attention(cache, q_lens, lens, heads, torch.bfloat16, window, 7, pad=1)
     check_attention(cache, q, out, cu, q_lens, lens, heads, torch.bfloat16, window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_requests_that_are_not_there(dtype):
+    o = ops()
+    heads, nkv, hd = 4, 2, 64
+    cache = Cache(3, [40, 70], nkv, hd)
+    q = torch.randn(4, heads * hd, device=DEV).to(dtype)
+    both = [torch.full_like(q, 7.0) for _ in range(2)]
+    for out, req in zip(both, ([0, 0, 1, 1], [0, -1, 1, 2])):
+        o.attention_kv4_rows(q, out, cache.k_cache, cache.v_cache, i32(cache.table), i32(req), i32([39, 20, 69, 5]), heads, nkv, hd, 16, None, hd ** -0.5, force_simple=True)
+    expect_status(41)
+    assert (both[1][[1, 3]] == 0).all() and torch.equal(both[0][[0, 2]], both[1][[0, 2]])
 
 
 # ------------------------------------------------------------------------------------ refusals
