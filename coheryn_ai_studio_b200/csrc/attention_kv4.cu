@@ -59,10 +59,10 @@ __device__ __forceinline__ size_t tile_at(long long page, int nkv, int kvh, int 
 //
 // A thread has 4 neighbouring channels of each half of a head, which turn together: every element is read once, and the
 // angles that a thread reads lie together with its neighbours' (8 neighbouring channels per thread, their partners read a
-// second time and angles 64 bytes apart from lane to lane, took 20 us instead of 8 for 2,048 tokens of 28 + 8 heads of 128:
-// the loads' wavefronts bound it).  The eight threads of a group agree on its minimum and maximum by three shuffles.  Heads
+// second time and angles 64 bytes apart from lane to lane, took 23 us instead of 17 for 2,048 tokens of 28 + 8 heads of 128 and
+// their pages read back: the loads' wavefronts bound it).  The eight threads of a group agree on its minimum and maximum by three shuffles.  Heads
 // that turn another number of channels, or whose halves are not whole groups, go to the kernel after it.  Bound by
-// the bytes of a prompt (19 MB read, 17 MB written there) and by one launch at decoding.
+// the latency of its few loads and of the shuffles (half of the issue slots; 19 MB read and 17 MB written there), at decoding by one launch.
 // ------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
@@ -448,7 +448,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 // list's first unit notes its number of parts and the place of the first for the kernel that joins them.
 // A list costs its CTAs about EXTRA units more than its positions (its queries, the first tiles' way, the warps' meeting), and counts as
 // longer by so much, in front of its first unit: else the shares that hold many short lists finish last (64 requests of 40 heads over 8
-// and every length up to 16,384: 135 us, 149 without; of 28 over 4, up to 8,000: 47.5, 69).  Not where there is a CTA for every unit, nor
+// and every length up to 16,384: 135 us, 149 without, in short runs, after which the power limit holds both to 149; of 28 over 4, up to 8,000: 47.5, 69).  Not where there is a CTA for every unit, nor
 // where every list is one unit.
 // ------------------------------------------------------------------------------------
 constexpr int UNIT = 128, EXTRA = 2;
@@ -766,7 +766,7 @@ kv4_simple_join_kernel(const float* __restrict__ scratch, int parts, T* __restri
 //  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs).  The scale
 //    put on the probability instead takes fewer instructions but rounds p s, whose error meets s c and not s c + m;
 //  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory, each as the sum
-//    of two bfloat16 terms: rounded to one they were the largest error of all (64 x 16,384 positions, 138 us instead of 147);
+//    of two bfloat16 terms: rounded to one they were the largest error of all (2.7e-3 against 64 bits, 2.3e-3 with two, for 6 % of the time);
 //  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
 //    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
 //  * the values' product of a pair and the scores of the next stand in one run of code without a branch, so that a warp
