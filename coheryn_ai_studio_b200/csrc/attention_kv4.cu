@@ -312,20 +312,21 @@ __device__ __forceinline__ int rows_needed(const int* cu_q, const int* lens, int
 }
 
 // The largest magnitude among the keys, and among the values, that the requests' new tokens see, from the pairs alone (a group's
-// values lie between m and m + 15 s): RANGE_BLOCKS partial answers.  A fifth of the pages' bytes.
-constexpr int RANGE_BLOCKS = 128;
-__global__ void __launch_bounds__(256)
+// values lie between m and m + 15 s): RANGE_BLOCKS partial answers.  A fifth of the pages' bytes; bound by a warp's chain of reads, an item after
+// the other, so as many warps as an SM holds (384 tokens after 8,191 beside 15 requests, the whole call: 99 us, 102 with 8 warps a block).
+constexpr int RANGE_BLOCKS = 128, RANGE_WARPS = 32;
+__global__ void __launch_bounds__(32 * RANGE_WARPS)
 kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
                  const int* __restrict__ table, int table_ld, int width, int n, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
                  float2* __restrict__ partial) {
-  __shared__ float2 part[8];
+  __shared__ float2 part[RANGE_WARPS];
   co_pdl_launch_dependents();
   co_pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_page = page_size >> 4;
   float k_most = 0.f, v_most = 0.f;
   // A warp takes a (request, entry, kv head) at a time.
   const long long items = (long long)n * width * nkv;
-  for (long long x = (long long)blockIdx.x * 8 + warp; x < items; x += RANGE_BLOCKS * 8) {
+  for (long long x = (long long)blockIdx.x * RANGE_WARPS + warp; x < items; x += RANGE_BLOCKS * RANGE_WARPS) {
     const int kvh = (int)(x % nkv), j = (int)(x / nkv % width), b = (int)(x / nkv / width);
     const int page = table[(size_t)b * table_ld + j], rows = rows_needed(cu_q, lens, b, j, page_size, window);    // (asked for at once)
     if (rows == 0 || page < 0 || page >= num_pages) continue;
@@ -350,7 +351,7 @@ kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   if (lane == 0) part[warp] = make_float2(k_most, v_most);
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) { k_most = fmaxf(k_most, part[w].x); v_most = fmaxf(v_most, part[w].y); }
+    for (int w = 1; w < RANGE_WARPS; ++w) { k_most = fmaxf(k_most, part[w].x); v_most = fmaxf(v_most, part[w].y); }
     partial[blockIdx.x] = make_float2(k_most, v_most);
   }
 }
@@ -1638,7 +1639,7 @@ CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int n
   if (width > table_ld) CO_FAIL("kv4_expand: %d entries of rows of %d", width, table_ld);
   float2* range = factors ? reinterpret_cast<float2*>(factors + 2) : nullptr;
   if (factors) {
-    co_launch(kv4_range_kernel, dim3(RANGE_BLOCKS), dim3(256), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
+    co_launch(kv4_range_kernel, dim3(RANGE_BLOCKS), dim3(32 * RANGE_WARPS), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
               page_size, table, table_ld, width, n, cu_q, kv_lens, window, range);
     CO_CHECK_LAUNCH("kv4_range");
   }
