@@ -2257,8 +2257,15 @@ _kv4_libs = {}
 # Requests with at most this many query rows (tokens times heads of a group) read the 4-bit pages directly; longer portions
 # have their pages expanded to 16 bits a value once and go through the prompt kernels.  Directly against expanded, in us: 112 rows
 # of 7 heads over each of 4, 1 x 1,024 positions 10 and 28, 8 x 8,192 103 and 120; 128 rows, 4 over each of 8, 1 x 65,536 210 and 221,
-# 8 x 1,024 52 and 43; 256 rows, 1 x 65,536 399 and 248.
+# 8 x 1,024 52 and 43; 256 rows, 1 x 65,536 399 and 248.  Half as many at head sizes 192 and 256, which the direct kernel takes in tiles of
+# 8 rows instead of 16 and whose prompts have a tcgen05 kernel (256, 8 x 8,192: 64 rows 134 and 165, 128 rows 254 and 167); not at those between
+# (160, 8 x 8,192: 128 rows 183 and 415).
 KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "128"))
+
+
+def kv4_direct_rows(head_dim: int) -> int:
+    return KV4_DIRECT_ROWS // 2 if head_dim in (192, 256) else KV4_DIRECT_ROWS
+
 
 # The expanded pages of a call take at most about this many bytes at a time (one request always goes in one piece).
 KV4_EXPAND_BYTES = 1 << 30
@@ -2389,14 +2396,14 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     """Attention of rows (request token_req[i] at position positions[i]) over the 4-bit pages of a cache, causal, with an
     optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros.
     bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
-    ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``KV4_DIRECT_ROWS`` rows per kv
-    head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
+    ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``kv4_direct_rows(head_dim)`` rows
+    per kv head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
     value and go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
     if not force_simple and q.is_cuda:
         lib = kv4_lib(head_dim)
         rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
                                 _address(lib, "coheryn_kv4_attention_simple"), q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads,
-                                num_kv_heads, head_dim, page_size, window, scale, cu_q, kv_lens, q_lens, max_kv_len, KV4_DIRECT_ROWS,
+                                num_kv_heads, head_dim, page_size, window, scale, cu_q, kv_lens, q_lens, max_kv_len, kv4_direct_rows(head_dim),
                                 tc_status(q.device), _address(lib, "coheryn_kv4_simple_parts"))
         if rc == 0:
             return
@@ -2438,7 +2445,7 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     _words(B + 1, cu_q=cu_q)
     if block_tables.shape[0] != B or B == 0:
         raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
-    limit = max(KV4_DIRECT_ROWS // G, 1)         # tokens that a request may bring to be read directly
+    limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly
     longest = max(q_lens)
     direct = longest if longest <= limit else max((n for n in q_lens if n <= limit), default=0)
     if direct:
