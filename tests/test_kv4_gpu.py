@@ -393,6 +393,42 @@ def test_captured_and_replayed_with_other_lengths_and_on_another_stream(longest)
         check_attention(Clipped(cache, now), q, out, [0, 1, 2, 3], [1, 1, 1], now, heads, torch.bfloat16)
 
 
+@pytest.mark.parametrize("heads,nkv,hd", [(4, 2, 64), (7, 1, 128), (2, 1, 96)])
+def test_portions_captured_and_replayed_over_other_pages(heads, nkv, hd):
+    """Two captured calls of portions beside a single token, replayed at once over a cache that has changed in between."""
+    o = ops()
+    q_lens, lens = [150, 1, 200], [400, 77, 200]
+    caches = [Cache(seed, lens, nkv, hd) for seed in (51, 51, 52)]
+    kept = caches[0]
+    q = torch.randn(351, heads * hd, device=DEV).to(torch.bfloat16)
+    cu, kv = i32([0, 150, 151, 351]), i32(lens)
+    req = i32(np.repeat([0, 1, 2], q_lens))
+    pos = i32(np.concatenate([np.arange(n - m, n) for n, m in zip(lens, q_lens)]))
+    table = i32(kept.table)
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    call = lambda out: o.attention_kv4_rows(q, out, kept.k_cache, kept.v_cache, table, req, pos, heads, nkv, hd, 16, None, hd ** -0.5, cu_q=cu,  # noqa: E731
+                                            kv_lens=kv, q_lens=q_lens, max_kv_len=400)
+    call(outs[2])
+    torch.cuda.synchronize()
+    graphs = []
+    for out in outs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(out)
+        graphs.append(g)
+    for other in (caches[2], caches[1]):
+        kept.k_cache.copy_(other.k_cache); kept.v_cache.copy_(other.v_cache); table.copy_(i32(other.table))
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        graphs[1].replay()
+        call(outs[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2])
+        check_attention(other, q, outs[2], [0, 150, 151, 351], q_lens, lens, heads, torch.bfloat16, rounded_keys=(0, 2))
+
+
 class Clipped:
     def __init__(self, cache, lens):
         self.hd = cache.hd
