@@ -1,0 +1,71 @@
+"""The attention over the 4-bit cache, each way against the bound of its own arithmetic (kv4_paths)."""
+import numpy as np
+import pytest
+import torch
+
+import kv4_paths as kp
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16 = torch.bfloat16
+
+
+def ops():
+    from coheryn_ai_studio_b200 import ops as o
+    return o
+
+
+@pytest.fixture(autouse=True)
+def no_status_left():
+    yield
+    torch.cuda.synchronize()
+    word = ops().tc_status(torch.device(DEV))
+    code = int(word.item())
+    word.zero_()
+    assert code == 0
+
+
+def queries(seed, q_lens, heads, hd, spread=1.5, dtype=BF16):
+    """[T, heads * hd]; ``spread`` one number, or one per request."""
+    rng = np.random.default_rng(seed)
+    by = np.repeat(np.broadcast_to(np.asarray(spread, np.float32), len(q_lens)), q_lens)[:, None]
+    return torch.from_numpy(rng.standard_normal((sum(q_lens), heads * hd)).astype(np.float32) * by).to(dtype).to(DEV)
+
+
+# ------------------------------------------------------------------------------------ every way, every head size
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
+def test_runs_of_every_length(hd, heads, nkv, window):
+    o = ops()
+    limit = o.kv4_direct_rows(hd) // (heads // nkv)
+    q_lens = [1, 5, limit, limit + 1, 0, limit + 40, 2]
+    lens = [700, 5, limit + 30, limit + 1, 0, limit + 300, 90]
+    k, v = kp.random_rows(16, lens, nkv, hd)
+    rows = kp.Rows(k, v, 32)
+    q = queries(17, q_lens, heads, hd)
+    kp.check(rows, q, kp.attend(o, rows, q, q_lens, heads, window), q_lens, heads, BF16, window, direct_rows=o.kv4_direct_rows(hd))
+    few = [1, 2, 0, 3, 0, 1, 1]
+    for x, simple in ((q[:8], True), (q[:8].float(), False)):
+        kp.check(rows, x, kp.attend(o, rows, x, few, heads, window, simple=simple), few, heads, x.dtype, window, simple=True)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q_lens,lens", [([1, 2], [2000, 40]), ([5, 1], [300, 5000]), ([70, 40], [200, 1500])])
+def test_sharp_scores(hd, q_lens, lens):
+    """Scores in the hundreds, where a key that has lost bits shows: a key rounded to bfloat16 moves them by tenths."""
+    heads, nkv = 4, 1
+    k, v = kp.random_rows(18, lens, nkv, hd, k_spread=6.0)
+    rows = kp.Rows(k, v)
+    q = queries(19, q_lens, heads, hd, 8.0)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
+    some = q[:2].float()
+    kp.check(rows, some, kp.attend(ops(), rows, some, [1, 1], heads), [1, 1], heads, torch.float32)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_parts_joined_over_a_long_context(hd):
+    heads, nkv, q_lens, lens = 8, 2, [33, 150], [3000, 2600]
+    k, v = kp.random_rows(20, lens, nkv, hd)
+    rows = kp.Rows(k, v)
+    q = queries(21, q_lens, heads, hd)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
