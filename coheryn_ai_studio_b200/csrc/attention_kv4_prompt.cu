@@ -24,6 +24,8 @@
 // Every wait is bounded: on expiry the kernel records a code in `status` and winds down.
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "tc_common.cuh"
 
 #ifndef CO_HEAD_DIM
@@ -285,7 +287,10 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);          // 2^(e - 127) <= most
       const float down = __uint_as_float((unsigned)(254 - e) << 23);
-      row_scale = sh.scale_log2 * factors[0] * __uint_as_float((unsigned)e << 23);
+      // A normal number: a factor of zero (a row of zeros over small keys), or one that is not finite, would turn the masked scores' -inf, or a
+      // score of zero, into not-a-number.  Scores that meet either bound are zero to working precision, or beyond float32.  The powers of
+      // two first, whose product is exact where the factor is normal.
+      row_scale = fminf(fmaxf(factors[0] * __uint_as_float((unsigned)e << 23) * sh.scale_log2, FLT_MIN), FLT_MAX);
 #pragma unroll
       for (int c = 0; c < KCH; ++c)
 #pragma unroll

@@ -32,6 +32,29 @@ def queries(seed, q_lens, heads, hd, spread=1.5, dtype=BF16):
     return torch.from_numpy(rng.standard_normal((sum(q_lens), heads * hd)).astype(np.float32) * by).to(dtype).to(DEV)
 
 
+# ------------------------------------------------------------------------------------ query rows and keys of zeros
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window", [None, 50])
+@pytest.mark.parametrize("spread", [1e-4, 0.0])
+def test_query_rows_of_zeros(hd, window, spread):
+    """Scores of zero: the mean of the values that a row sees; over small keys, and over keys that are zeros."""
+    heads, nkv, q_lens, lens = 4, 2, [130, 1, 70], [190, 33, 70]
+    k, v = kp.random_rows(1, lens, nkv, hd, k_spread=spread)
+    rows = kp.Rows(k, v)
+    q = queries(2, q_lens, heads, hd)
+    q[::3] = 0
+    q[128:] = 0
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads, window), q_lens, heads, BF16, window)
+
+
+def test_a_zeroed_cache():
+    heads, nkv, hd, q_lens, lens = 4, 1, 64, [140, 1], [300, 20]
+    rows = kp.Rows(*[[np.zeros((n, nkv, hd), np.float32) for n in lens] for _ in range(2)])
+    rows.k_cache.zero_(), rows.v_cache.zero_()
+    for q in (queries(3, q_lens, heads, hd), torch.zeros(141, heads * hd, dtype=BF16, device=DEV)):
+        assert (kp.attend(ops(), rows, q, q_lens, heads) == 0).all()
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
