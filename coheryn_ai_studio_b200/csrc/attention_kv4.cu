@@ -355,9 +355,10 @@ kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     partial[blockIdx.x] = make_float2(k_most, v_most);
   }
 }
-// The power of two that brings a largest magnitude to 2^13..2^14, and its inverse.
+// The power of two that brings a largest magnitude to 2^13..2^14, and its inverse; both are normal numbers for every finite one (magnitudes
+// under 2^-113 are brought up by 2^126).  A group whose m + 15 s passes the largest float32 stands for an infinity there, here as well.
 __device__ __forceinline__ float2 to_float16_range(float most) {
-  const int e = min(max((int)(__float_as_uint(most) >> 23), 14), 240);
+  const int e = min(max((int)(__float_as_uint(most) >> 23), 14), 254);
   return make_float2(__uint_as_float((unsigned)(267 - e) << 23), __uint_as_float((unsigned)(e - 13) << 23));
 }
 

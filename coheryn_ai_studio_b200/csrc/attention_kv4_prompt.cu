@@ -410,8 +410,9 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (active && ok) {
       // Rows leave by way of the tile's probabilities' place, 64 columns at a time: written by a thread a row each, every store to memory
       // would meet 32 rows (9,500 cycles a CTA instead of 6,000).
-      const float v_factor = factors[1];
-      const float mul = sh.parts > 1 ? v_factor : l == 0.f ? 0.f : v_factor / l;
+      // The sum first, then the values' factor (for parts: behind the join), so that neither passes the range of float32 before the answer does.
+      const float v_factor = sh.parts > 1 ? 1.f : factors[1];
+      const float inv = sh.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       if (sh.parts > 1 && valid)
         *reinterpret_cast<float2*>(scratch + (size_t)blockIdx.x * PART_FLOATS + 256 * HD + (t * 128 + row) * 2) = make_float2(m, l);
       const int token = (row_first + row) / G;
@@ -431,7 +432,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             for (int c = 0; c < 32; ++c) o[c] = 0;
           }
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * mul);
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * inv * v_factor);
 #pragma unroll
           for (int c = 0; c < 8; ++c)
             st_shared(stage + row * 256 + (((h * 8 + c) ^ (row & 7)) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
@@ -476,7 +477,8 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
 // Joins the parts of every row, a warp per row, parts in ascending order.  Bound by what the parts left (3 parts of 10,752 rows: 17 MB).
 __global__ void __launch_bounds__(256)
-kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out, long out_stride, const int* __restrict__ cu_q, Shape sh) {
+kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out, long out_stride, const int* __restrict__ cu_q,
+                       const float* __restrict__ factors, Shape sh) {
   constexpr int C = SUPPORTED ? HD / 32 : 2;         // neighbouring columns per lane: 2 or 4
   co_pdl_launch_dependents();
   const int rr = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z, G = sh.G, RT = sh.TOK * G;
@@ -508,12 +510,12 @@ kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = acc[c] * f + x[c] * g;
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const float inv = den == 0.f ? 0.f : 1.f / den, v_factor = factors[1];
   bf16* dst = out + (size_t)(tok0 + rr / G) * out_stride + (size_t)(kvh * G + rr % G) * HD + lane * C;
   unsigned w[C / 2];
 #pragma unroll
   for (int c = 0; c < C / 2; ++c) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * c] * inv * v_factor, acc[2 * c + 1] * inv * v_factor);
     w[c] = *reinterpret_cast<const unsigned*>(&v);
   }
   if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
@@ -582,7 +584,7 @@ CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens,
   CO_CHECK_LAUNCH("kv4_prompt");
   if (parts > 1) {
     co_launch(kv4_prompt_join_kernel, dim3((unsigned)((max_rows + 7) / 8), (unsigned)nkv, (unsigned)n), dim3(256), 0, stream, (const float*)scratch,
-              (bf16*)out, out_stride, cu_q, sh);
+              (bf16*)out, out_stride, cu_q, factors, sh);
     CO_CHECK_LAUNCH("kv4_prompt_join");
   }
   return 0;

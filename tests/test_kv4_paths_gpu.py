@@ -55,6 +55,18 @@ def test_a_zeroed_cache():
         assert (kp.attend(ops(), rows, q, q_lens, heads) == 0).all()
 
 
+# ------------------------------------------------------------------------------------ magnitudes
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("k_spread,v_spread", [(1e36, 1e36), (1.0, 3e37), (1e-36, 1e-36), (1e36, 1e-36), (1.0, 1e-37)])
+@pytest.mark.parametrize("context", [200, 2500])         # one CTA per pair of row tiles, and parts that are joined
+def test_portions_of_any_magnitude(hd, k_spread, v_spread, context):
+    heads, nkv, q_lens, lens = 4, 1, [70], [context]
+    k, v = kp.random_rows(4, lens, nkv, hd, k_spread, v_spread)
+    rows = kp.Rows(k, v)
+    q = queries(5, q_lens, heads, hd, 1.5 / k_spread)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
