@@ -311,23 +311,24 @@ __device__ __forceinline__ int rows_needed(const int* cu_q, const int* lens, int
   return (j + 1) * page_size <= first_key ? 0 : max(0, min(page_size, len - j * page_size));
 }
 
-// The largest magnitude among the keys, and among the values, that the requests' new tokens see, from the pairs alone (a group's
-// values lie between m and m + 15 s): RANGE_BLOCKS partial answers.  A fifth of the pages' bytes; bound by a warp's chain of reads, an item after
+// The largest magnitude among the keys, and among the values, that a request's new tokens see of a kv head, from the pairs alone (a group's
+// values lie between m and m + 15 s): `parts` partial answers per list (request, kv head), so that a list's factors, and with them its
+// rows' rounding, do not depend on what others hold.  A fifth of the pages' bytes; bound by a warp's chain of reads, an entry after
 // the other, so as many warps as an SM holds (384 tokens after 8,191 beside 15 requests, the whole call: 99 us, 102 with 8 warps a block).
 constexpr int RANGE_BLOCKS = 128, RANGE_WARPS = 32;
+int range_parts(long long lists) { return lists < RANGE_BLOCKS ? (int)(RANGE_BLOCKS / (lists < 1 ? 1 : lists)) : 1; }
 __global__ void __launch_bounds__(32 * RANGE_WARPS)
 kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
-                 const int* __restrict__ table, int table_ld, int width, int n, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
-                 float2* __restrict__ partial) {
-  __shared__ float2 part[RANGE_WARPS];
+                 const int* __restrict__ table, int table_ld, int width, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
+                 int parts, float2* __restrict__ partial) {
+  __shared__ float2 most[RANGE_WARPS];
   co_pdl_launch_dependents();
   co_pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_page = page_size >> 4;
+  const int list = blockIdx.x / parts, part = blockIdx.x - list * parts, b = list / nkv, kvh = list - b * nkv;
   float k_most = 0.f, v_most = 0.f;
-  // A warp takes a (request, entry, kv head) at a time.
-  const long long items = (long long)n * width * nkv;
-  for (long long x = (long long)blockIdx.x * RANGE_WARPS + warp; x < items; x += RANGE_BLOCKS * RANGE_WARPS) {
-    const int kvh = (int)(x % nkv), j = (int)(x / nkv % width), b = (int)(x / nkv / width);
+  // A warp takes an entry at a time.
+  for (int j = part * RANGE_WARPS + warp; j < width; j += parts * RANGE_WARPS) {
     const int page = table[(size_t)b * table_ld + j], rows = rows_needed(cu_q, lens, b, j, page_size, window);    // (asked for at once)
     if (rows == 0 || page < 0 || page >= num_pages) continue;
     for (int tile = 0; tile < per_page && tile * 16 < rows; ++tile) {
@@ -348,10 +349,10 @@ kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   }
   k_most = co_warp_max(k_most);
   v_most = co_warp_max(v_most);
-  if (lane == 0) part[warp] = make_float2(k_most, v_most);
+  if (lane == 0) most[warp] = make_float2(k_most, v_most);
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < RANGE_WARPS; ++w) { k_most = fmaxf(k_most, part[w].x); v_most = fmaxf(v_most, part[w].y); }
+    for (int w = 1; w < RANGE_WARPS; ++w) { k_most = fmaxf(k_most, most[w].x); v_most = fmaxf(v_most, most[w].y); }
     partial[blockIdx.x] = make_float2(k_most, v_most);
   }
 }
@@ -366,8 +367,8 @@ template <typename T>
 __global__ void __launch_bounds__(128)
 kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
                  const int* __restrict__ table, int table_ld, int width, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
-                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, const float2* __restrict__ range,
-                 float* __restrict__ factors, int* __restrict__ status) {
+                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, const float2* __restrict__ range, int range_parts,
+                 float2* __restrict__ factors, int* __restrict__ status) {
   constexpr bool HALF = sizeof(T) == 2 && !std::is_same<T, bf16>::value;
   __shared__ float2 most[4];
   co_pdl_launch_dependents();
@@ -379,8 +380,9 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   int valid = lens ? rows_needed(cu_q, lens, b, j, page_size, window) : page_size;      // rows of the page that hold something
   float k_by = 1.f, v_by = 1.f;
   if constexpr (HALF) {             // float16: times the powers of two that the largest values ask for
-    static_assert(RANGE_BLOCKS == 128, "a thread per partial answer");
-    const float2 x = range[threadIdx.x];
+    static_assert(RANGE_BLOCKS <= 128, "a thread per partial answer of a list");
+    const int list = b * nkv + kvh;
+    const float2 x = (int)threadIdx.x < range_parts ? range[(size_t)list * range_parts + threadIdx.x] : make_float2(0.f, 0.f);
     const float kx = co_warp_max(x.x), vx = co_warp_max(x.y);
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = make_float2(kx, vx);
     __syncthreads();
@@ -388,7 +390,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     const float2 v2 = to_float16_range(fmaxf(fmaxf(most[0].y, most[1].y), fmaxf(most[2].y, most[3].y)));
     k_by = k2.x;
     v_by = v2.x;
-    if (j == 0 && kvh == 0 && b == 0 && threadIdx.x == 0) { factors[0] = k2.y; factors[1] = v2.y; }
+    if (j == 0 && threadIdx.x == 0) factors[list] = make_float2(k2.y, v2.y);
   }
   if (!valid) {
     if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
@@ -1521,13 +1523,13 @@ constexpr int PAGES_F16 = 2;      // beside the dtype codes
 
 static int launch_pages(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
                         int width, int n, const int* cu_q, const int* lens, int window, void* k_out, void* v_out, int dtype, int* out_table,
-                        const float2* range, float* factors, int* status, cudaStream_t stream) {
+                        const float2* range, int parts, float2* factors, int* status, cudaStream_t stream) {
   if (nkv > 65535 || n > 65535) CO_FAIL("kv4_pages: %d requests, %d kv heads", n, nkv);
   const dim3 grid((unsigned)width, (unsigned)nkv, (unsigned)n);
   auto with = [&](auto* x) {
     typedef decltype(x) P;
     co_launch(kv4_pages_kernel<std::remove_pointer_t<P>>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
-              num_pages, nkv, page_size, table, table_ld, width, cu_q, lens, window, (P)k_out, (P)v_out, out_table, range, factors, status);
+              num_pages, nkv, page_size, table, table_ld, width, cu_q, lens, window, (P)k_out, (P)v_out, out_table, range, parts, factors, status);
   };
   if (dtype == CO_F32) with((float*)nullptr);
   else if (dtype == PAGES_F16) with((__half*)nullptr);
@@ -1543,7 +1545,7 @@ CO_EXPORT int coheryn_kv4_pages(const void* k_cache, const void* v_cache, int nu
   if (check_pages("kv4_pages", nkv, page_size, num_pages)) return 1;
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
     CO_FAIL("kv4_pages: operands must be 16-byte aligned");
-  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, nullptr,
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, nullptr, 0,
                       nullptr, status, stream);
 }
 
@@ -1627,9 +1629,16 @@ CO_EXPORT int coheryn_kv4_attention(const void* q, long q_ld, void* out, long ou
   return 0;
 }
 
+// Floats that the factors of coheryn_kv4_expand take: two per list (request, kv head), then the partial answers that they are formed from.
+CO_EXPORT long coheryn_kv4_factor_floats(int n, int nkv) {
+  const long lists = (long)n * nkv;
+  return 2 * lists + 2 * lists * range_parts(lists);
+}
+
 // The pages of requests b = 0..n-1 of a block table, dense: entry (b, j) becomes page b * width + j of k_out and v_out [n * width, nkv, page_size, HD]
 // and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length are zeros.  In bfloat16, or, with `factors` (float32
-// [2 + 2 * 128], of which the first two are what keys and values have to be multiplied by), in scaled float16.
+// [coheryn_kv4_factor_floats(n, nkv)]; place 2 (b nkv + kv head) gets what that list's keys have to be multiplied by, the next what its values do), in
+// scaled float16.
 CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
                                  int width, int n, const int* cu_q, const int* kv_lens, int window, void* k_out, void* v_out, int* out_table,
                                  float* factors, int* status, cudaStream_t stream) {
@@ -1638,12 +1647,15 @@ CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int n
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || ((uintptr_t)factors & 7))
     CO_FAIL("kv4_expand: operands must be 16-byte aligned");
   if (width > table_ld) CO_FAIL("kv4_expand: %d entries of rows of %d", width, table_ld);
-  float2* range = factors ? reinterpret_cast<float2*>(factors + 2) : nullptr;
+  const long long lists = (long long)n * nkv;
+  const int parts = range_parts(lists);
+  float2* range = factors ? reinterpret_cast<float2*>(factors) + lists : nullptr;
   if (factors) {
-    co_launch(kv4_range_kernel, dim3(RANGE_BLOCKS), dim3(32 * RANGE_WARPS), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache, num_pages, nkv,
-              page_size, table, table_ld, width, n, cu_q, kv_lens, window, range);
+    if (lists * parts > 0x7fffffffLL) CO_FAIL("kv4_expand: %d requests of %d kv heads", n, nkv);
+    co_launch(kv4_range_kernel, dim3((unsigned)(lists * parts)), dim3(32 * RANGE_WARPS), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
+              num_pages, nkv, page_size, table, table_ld, width, cu_q, kv_lens, window, parts, range);
     CO_CHECK_LAUNCH("kv4_range");
   }
   return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, n, cu_q, kv_lens, window, k_out, v_out,
-                      factors ? PAGES_F16 : CO_BF16, out_table, (const float2*)range, factors, status, stream);
+                      factors ? PAGES_F16 : CO_BF16, out_table, (const float2*)range, parts, reinterpret_cast<float2*>(factors), status, stream);
 }

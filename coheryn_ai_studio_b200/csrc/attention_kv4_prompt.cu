@@ -3,9 +3,9 @@
 //
 // Float16 and not bfloat16: a value s c + m has up to twelve bits, of which bfloat16 keeps eight; the rounded keys alone moved the
 // outputs by 2.4 times their own rounding (2,048 tokens of 28 heads over 4: 3.8e-3 against 64 bits, 1.7e-3 now).  Its range is
-// made enough by powers of two: keys, and values, are divided by the one that brings the largest of the call to 2^13..2^14
-// (found on the device), a query row by its own that brings its largest to 1..2.  That is exact but for what lies under 2^-24 of the
-// largest.  The factors meet again in the exponent's factor and in the last division.
+// made enough by powers of two: keys, and values, of a (request, kv head) are divided by the one that brings the largest of them to 2^13..2^14
+// (found on the device), a query row by its own that brings its largest to 1..2.  A value keeps eleven bits, or what lies over 2^-38 of
+// that largest (float16's last step, 2^-24).  The factors meet again in the exponent's factor and behind the last division.
 //
 // The arrangement is near that of the framework's two-tile prompt kernel: a CTA owns two consecutive tiles of TOK = 128 / G tokens times
 // the G heads of a group (rows r = token * G + head) and fetches every tile of 128 keys once for both.  Warp 0 fetches Q and
@@ -98,7 +98,7 @@ constexpr int THREADS = 384;
 __global__ void __launch_bounds__(THREADS, 1)
 kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   bf16* __restrict__ out, long out_stride, const int* __restrict__ block_tables, const int* __restrict__ cu_q,
-                  const int* __restrict__ kv_lens, const float* __restrict__ factors, Shape sh, float* __restrict__ scratch,
+                  const int* __restrict__ kv_lens, const float2* __restrict__ factors, Shape sh, float* __restrict__ scratch,
                   int* __restrict__ status) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -290,7 +290,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // A normal number: a factor of zero (a row of zeros over small keys), or one that is not finite, would turn the masked scores' -inf, or a
       // score of zero, into not-a-number.  Scores that meet either bound are zero to working precision, or beyond float32.  The powers of
       // two first, whose product is exact where the factor is normal.
-      row_scale = fminf(fmaxf(factors[0] * __uint_as_float((unsigned)e << 23) * sh.scale_log2, FLT_MIN), FLT_MAX);
+      row_scale = fminf(fmaxf(factors[b * sh.nkv + kvh].x * __uint_as_float((unsigned)e << 23) * sh.scale_log2, FLT_MIN), FLT_MAX);
 #pragma unroll
       for (int c = 0; c < KCH; ++c)
 #pragma unroll
@@ -411,7 +411,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // Rows leave by way of the tile's probabilities' place, 64 columns at a time: written by a thread a row each, every store to memory
       // would meet 32 rows (9,500 cycles a CTA instead of 6,000).
       // The sum first, then the values' factor (for parts: behind the join), so that neither passes the range of float32 before the answer does.
-      const float v_factor = sh.parts > 1 ? 1.f : factors[1];
+      const float v_factor = sh.parts > 1 ? 1.f : factors[b * sh.nkv + kvh].y;
       const float inv = sh.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       if (sh.parts > 1 && valid)
         *reinterpret_cast<float2*>(scratch + (size_t)blockIdx.x * PART_FLOATS + 256 * HD + (t * 128 + row) * 2) = make_float2(m, l);
@@ -478,7 +478,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 // Joins the parts of every row, a warp per row, parts in ascending order.  Bound by what the parts left (3 parts of 10,752 rows: 17 MB).
 __global__ void __launch_bounds__(256)
 kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out, long out_stride, const int* __restrict__ cu_q,
-                       const float* __restrict__ factors, Shape sh) {
+                       const float2* __restrict__ factors, Shape sh) {
   constexpr int C = SUPPORTED ? HD / 32 : 2;         // neighbouring columns per lane: 2 or 4
   co_pdl_launch_dependents();
   const int rr = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z, G = sh.G, RT = sh.TOK * G;
@@ -510,7 +510,7 @@ kv4_prompt_join_kernel(const float* __restrict__ scratch, bf16* __restrict__ out
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = acc[c] * f + x[c] * g;
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den, v_factor = factors[1];
+  const float inv = den == 0.f ? 0.f : 1.f / den, v_factor = factors[b * sh.nkv + kvh].y;
   bf16* dst = out + (size_t)(tok0 + rr / G) * out_stride + (size_t)(kvh * G + rr % G) * HD + lane * C;
   unsigned w[C / 2];
 #pragma unroll
@@ -547,8 +547,8 @@ CO_EXPORT long coheryn_kv4_prompt_scratch_floats(int nh, int nkv, int n, int max
   return parts > 1 ? (long)pairs_of(nh, nkv, max_rows) * n * nkv * parts * PART_FLOATS : 0;
 }
 
-// q: [total_tokens, >= nh * HD] bfloat16 rows of stride q_stride; k, v: float16 pages [num_pages, nkv, page_size, HD], and factors[2] that
-// multiply them back (device); requests 0..n-1 all go through this kernel.
+// q: [total_tokens, >= nh * HD] bfloat16 rows of stride q_stride; k, v: float16 pages [num_pages, nkv, page_size, HD], and the factors [n, nkv, 2]
+// that multiply them back (device); requests 0..n-1 all go through this kernel.
 CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens, void* out, long out_stride, const void* k, const void* v, int num_pages,
                                  const int* block_tables, int table_ld, const int* cu_q, const int* kv_lens, int n, int nh, int nkv, int page_size,
                                  int window, float scale, int max_rows, const float* factors, int parts, float* scratch, long scratch_floats,
@@ -559,6 +559,7 @@ CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens,
   const long cache_rows = (long)num_pages * nkv * page_size;
   const long ctas = (long)pairs_of(nh, nkv, max_rows) * n * nkv * parts;
   if (cache_rows >= (1L << 31) || ctas >= (1L << 31) || n > 65535 || nkv > 65535) CO_FAIL("kv4_prompt: %ld rows of pages, %ld CTAs", cache_rows, ctas);
+  if ((uintptr_t)factors & 7) CO_FAIL("kv4_prompt: the factors must be 8-byte aligned");
   if (parts < 1 || scratch_floats < coheryn_kv4_prompt_scratch_floats(nh, nkv, n, max_rows, parts) || ((uintptr_t)scratch & 15))
     CO_FAIL("kv4_prompt: %d parts in a scratch of %ld floats", parts, scratch_floats);
   const int G = nh / nkv, TOK = 128 / G;
@@ -580,11 +581,11 @@ CO_EXPORT int coheryn_kv4_prompt(const void* q, long q_stride, int total_tokens,
   cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) CO_FAIL("kv4_prompt: %d bytes of shared memory: %s", SMEM_BYTES, cudaGetErrorString(e));
   co_launch(kv4_prompt_kernel, dim3((unsigned)ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, mq, mk, mv, (bf16*)out, out_stride, block_tables, cu_q, kv_lens,
-            factors, sh, scratch, status);
+            (const float2*)factors, sh, scratch, status);
   CO_CHECK_LAUNCH("kv4_prompt");
   if (parts > 1) {
     co_launch(kv4_prompt_join_kernel, dim3((unsigned)((max_rows + 7) / 8), (unsigned)nkv, (unsigned)n), dim3(256), 0, stream, (const float*)scratch,
-              (bf16*)out, out_stride, cu_q, factors, sh);
+              (bf16*)out, out_stride, cu_q, (const float2*)factors, sh);
     CO_CHECK_LAUNCH("kv4_prompt_join");
   }
   return 0;

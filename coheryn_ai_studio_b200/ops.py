@@ -2281,6 +2281,7 @@ def kv4_lib(head_dim: int):
         lib.coheryn_last_error.restype = ctypes.c_char_p
         lib.coheryn_launch_count.restype = ctypes.c_ulonglong
         lib.coheryn_kv4_scratch_floats.restype = c_long
+        lib.coheryn_kv4_factor_floats.restype = c_long
         lib.coheryn_kv4_prompt_scratch_floats.restype = c_long
         if lib.coheryn_kv4_head_dim() != head_dim:
             raise KernelError(f"the library of the 4-bit cache was built for head size {lib.coheryn_kv4_head_dim()}, not {head_dim}")
@@ -2476,7 +2477,7 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         n, rows = e - b, max(q_lens[b:e]) * G
         k, v = q.new_empty((2, n * width, num_kv_heads, page_size, head_dim)).unbind(0)       # (16 bits a value, whichever kind)
         table = block_tables.new_empty((n, width))
-        factors = torch.empty(2 + 2 * 128, dtype=torch.float32, device=q.device) if half else None
+        factors = torch.empty(int(lib.coheryn_kv4_factor_floats(c_int(n), c_int(num_kv_heads))), dtype=torch.float32, device=q.device) if half else None
         cu, lens = cu_q.data_ptr() + 4 * b, kv_lens.data_ptr() + 4 * b
         rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiippipppppp")(
             k_cache.data_ptr(), v_cache.data_ptr(), num_pages, num_kv_heads, page_size, block_tables.data_ptr() + 4 * W * b, W, width, n, cu, lens,

@@ -67,6 +67,24 @@ def test_portions_of_any_magnitude(hd, k_spread, v_spread, context):
     kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,nkv", [(4, 1), (6, 2)])
+def test_requests_of_one_call_keep_their_own_magnitudes(hd, heads, nkv):
+    """A request's answer does not depend on what other requests, or other kv heads, hold."""
+    q_lens, lens, spread = [70, 140, 1, 70], [200, 150, 40, 90], np.array([1e12, 1e-7, 1.0, 1e-3])
+    parts = [kp.random_rows(10 + b, [n], nkv, hd, s, s) for b, (n, s) in enumerate(zip(lens, spread))]
+    k, v = [p[0][0] for p in parts], [p[1][0] for p in parts]
+    k[3][:, 0] *= np.float32(1e9)
+    v[3][:, 0] *= np.float32(1e9)
+    rows = kp.Rows(k, v)
+    q = queries(6, q_lens, heads, hd, 1.5 / spread)
+    q.view(-1, nkv, heads // nkv, hd)[sum(q_lens[:3]):, 0] *= 1e-9
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
+    alone = kp.Rows(k[1:2], v[1:2])
+    again = kp.attend(ops(), alone, q[70:210], [140], heads)
+    kp.check(alone, q[70:210], again, [140], heads, BF16)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
