@@ -45,6 +45,10 @@ constexpr int K_STAGES = 2;
 constexpr int SMEM_BYTES = 2 * TILE_BYTES + K_STAGES * TILE_BYTES + TILE_BYTES + 2 * P_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
 static_assert(SMEM_BYTES <= 227 * 1024, "two query tiles, the stages and the probabilities fit shared memory");
 constexpr unsigned FLOAT16 = ~((1u << 7) | (1u << 10));      // of an instruction descriptor: both operands float16, not bfloat16
+// Probabilities are 2^LIFT times over their reference, which the maximum passes by 2^8 at most (2^15 at most enter the products): what
+// float16 drops then lies under 2^-32 of a reference that the sum holds, where without it 131,072 keys of just under 2^-25 would be 0.4 % of the
+// sum and nothing of the products.
+constexpr float LIFT = 7.f;
 constexpr int PART_FLOATS = 256 * (HD + 2);      // what a CTA of a part leaves: 256 rows, then their references and sums
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -343,7 +347,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
           for (int c = 0; c < 32; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[i][c]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        // The reference m follows the running maximum lazily (p stays below 2^8, far inside float16's range), and the warp
+        // The reference m follows the running maximum lazily (p stays below 2^(8 + LIFT), inside float16's range), and the warp
         // decides together, because rescaling O is a warp-wide access to tensor memory.
         const float m_row = fmaxf(m, mx * row_scale);            // scale > 0 keeps the order
         const bool move = m == -INFINITY ? m_row != -INFINITY : m_row - m > 8.0f;
@@ -376,7 +380,7 @@ kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         // Exponentials, 32 columns at a time, each group packed and stored at once: row `row` of chunk i / 2 of the P tile,
         // 16-byte piece c at c ^ (row % 8).
-        const unsigned scale_bits = __float_as_uint(row_scale), use_bits = __float_as_uint(-m_use);
+        const unsigned scale_bits = __float_as_uint(row_scale), use_bits = __float_as_uint(LIFT - m_use);
         const unsigned long long scale2 = pair_f32(scale_bits, scale_bits), use2 = pair_f32(use_bits, use_bits);
         unsigned long long sum2[4] = {0, 0, 0, 0};
 #pragma unroll

@@ -85,6 +85,25 @@ def test_requests_of_one_call_keep_their_own_magnitudes(hd, heads, nkv):
     kp.check(alone, q[70:210], again, [140], heads, BF16)
 
 
+@pytest.mark.parametrize("hd,top", [(64, 2.203125), (128, 1.5546875)])
+@pytest.mark.parametrize("context", [600, 3000])
+def test_many_keys_of_little_weight(hd, top, context):
+    """One key in front of all others by 25.4 powers of two and a value of zero: what comes out is the others' share."""
+    heads, nkv, q_lens, lens = 4, 1, [70], [context]
+    k, v = np.zeros((context, nkv, hd), np.float32), np.ones((context, nkv, hd), np.float32)
+    k[0], v[0] = top, 0
+    rows = kp.Rows([k], [v])
+    q = torch.ones(70, heads * hd, dtype=BF16, device=DEV)
+    out = kp.attend(ops(), rows, q, q_lens, heads)
+    # by hand: every p of the others is 2^-x of the first's
+    p = np.exp(-top * hd ** 0.5)
+    n = np.arange(context - 69, context + 1)[:, None] - 1.0
+    want = n * p / (1 + n * p)
+    # half a bfloat16 step, a float16 subnormal's step (2^-32 against p = 2^-25.4), float32 sums
+    assert (np.abs(out.double().cpu().numpy() - want) <= want * (2.0 ** -8 + 2.0 ** -32 / p + context * 2.0 ** -22)).all()
+    kp.check(rows, q, out, q_lens, heads, BF16)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
