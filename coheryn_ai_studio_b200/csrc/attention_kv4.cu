@@ -291,8 +291,8 @@ kv4_write_kernel(const T* __restrict__ qkv, long ld, const int* __restrict__ pos
 
 // ------------------------------------------------------------------------------------
 // Pages as values: [entry, kv head, page_size, HD] in float32, bfloat16, or scaled float16 (for attention_kv4_prompt.cu).  One block per (page, kv head).
-// With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length are
-// zeros, entries that lie wholly behind it or in front of the window of its first new token are left out, and
+// With `lens` the entries are rows of a block table (request = blockIdx.z): rows at or behind the request's length, or in front of the
+// window of its first new token, are zeros (whatever they hold, it meets probabilities of zero), entries that lie wholly there are left out, and
 // `out_table` gets the entry's place among the output pages, or -1.
 // Bound by the bytes written (16 of 21 bits a value).
 // ------------------------------------------------------------------------------------
@@ -304,11 +304,13 @@ template <>
 __device__ __forceinline__ void store4<__half>(__half* p, float a, float b, float c, float d) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_f16(a, b), pack_f16(c, d));
 }
-// How many rows of entry j of request b's block table hold something that its new tokens see (0: the entry is not needed).
-__device__ __forceinline__ int rows_needed(const int* cu_q, const int* lens, int b, int j, int page_size, int window) {
+// The rows [lo, hi) of entry j of request b's block table that its new tokens see (hi = 0: the entry is not needed).
+struct Seen { int lo, hi; };
+__device__ __forceinline__ Seen rows_seen(const int* cu_q, const int* lens, int b, int j, int page_size, int window) {
   const int len = lens[b], first_new = len - (cu_q[b + 1] - cu_q[b]);
   const int first_key = window > 0 ? max(0, first_new - window + 1) : 0;
-  return (j + 1) * page_size <= first_key ? 0 : max(0, min(page_size, len - j * page_size));
+  const int lo = max(0, first_key - j * page_size), hi = min(page_size, len - j * page_size);
+  return hi > lo ? Seen{lo, hi} : Seen{0, 0};
 }
 
 // The largest magnitude among the keys, and among the values, that a request's new tokens see of a kv head, from the pairs alone (a group's
@@ -329,21 +331,25 @@ kv4_range_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   float k_most = 0.f, v_most = 0.f;
   // A warp takes an entry at a time.
   for (int j = part * RANGE_WARPS + warp; j < width; j += parts * RANGE_WARPS) {
-    const int page = table[(size_t)b * table_ld + j], rows = rows_needed(cu_q, lens, b, j, page_size, window);    // (asked for at once)
-    if (rows == 0 || page < 0 || page >= num_pages) continue;
-    for (int tile = 0; tile < per_page && tile * 16 < rows; ++tile) {
+    const int page = table[(size_t)b * table_ld + j];                                   // (asked for at once with the lengths)
+    const Seen rows = rows_seen(cu_q, lens, b, j, page_size, window);
+    if (rows.hi == 0 || page < 0 || page >= num_pages) continue;
+    for (int tile = rows.lo >> 4; tile < per_page && tile * 16 < rows.hi; ++tile) {
       const size_t at = tile_at(page, nkv, kvh, page_size, tile * 16) + CODES;
       for (int i = lane; i < 16 * NG; i += 32) {         // keys: row i / NG
         const unsigned w = reinterpret_cast<const unsigned*>(k_cache + at)[i];
         const float m = hi_bf16(w);
-        if (tile * 16 + i / NG < rows) k_most = fmaxf(k_most, fmaxf(fabsf(m), fabsf(fmaf(15.f, lo_bf16(w), m))));
+        const int r = tile * 16 + i / NG;
+        if (r >= rows.lo && r < rows.hi) k_most = fmaxf(k_most, fmaxf(fabsf(m), fabsf(fmaf(15.f, lo_bf16(w), m))));
       }
       for (int i = lane; i < 4 * NG; i += 32) {          // values: rows 4 (i % 4)..
         const uint4 w = reinterpret_cast<const uint4*>(v_cache + at)[i];
         const float sc[4] = {lo_bf16(w.x), hi_bf16(w.x), lo_bf16(w.y), hi_bf16(w.y)}, mn[4] = {lo_bf16(w.z), hi_bf16(w.z), lo_bf16(w.w), hi_bf16(w.w)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (tile * 16 + (i & 3) * 4 + e < rows) v_most = fmaxf(v_most, fmaxf(fabsf(mn[e]), fabsf(fmaf(15.f, sc[e], mn[e]))));
+        for (int e = 0; e < 4; ++e) {
+          const int r = tile * 16 + (i & 3) * 4 + e;
+          if (r >= rows.lo && r < rows.hi) v_most = fmaxf(v_most, fmaxf(fabsf(mn[e]), fabsf(fmaf(15.f, sc[e], mn[e]))));
+        }
       }
     }
   }
@@ -377,7 +383,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   const long long entry = (long long)b * width + j;
   // The loads that depend on nothing first: a block lives for little more than its chain of them.
   const int page = table[(size_t)b * table_ld + j];
-  int valid = lens ? rows_needed(cu_q, lens, b, j, page_size, window) : page_size;      // rows of the page that hold something
+  Seen seen = lens ? rows_seen(cu_q, lens, b, j, page_size, window) : Seen{0, page_size};
   float k_by = 1.f, v_by = 1.f;
   if constexpr (HALF) {             // float16: times the powers of two that the largest values ask for
     static_assert(RANGE_BLOCKS <= 128, "a thread per partial answer of a list");
@@ -392,12 +398,12 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     v_by = v2.x;
     if (j == 0 && threadIdx.x == 0) factors[list] = make_float2(k2.y, v2.y);
   }
-  if (!valid) {
+  if (seen.hi == 0) {
     if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
     return;
   }
   const bool known = page >= 0 && page < num_pages;
-  if (!known) valid = 0;
+  if (!known) seen.hi = 0;
   if (kvh == 0 && threadIdx.x == 0) {
     if (out_table) out_table[entry] = known ? (int)entry : -1;
     if (status && (!known || (lens && lens[b] > width * page_size))) *status = BAD_INDEX;      // (or the table ends before the request)
@@ -410,7 +416,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     for (int i = threadIdx.x; i < 16 * 4 * NG; i += 128) {
       const int r = i / (4 * NG), w = i % (4 * NG), u = w >> 2, t = w & 3;    // u, t: consecutive threads, consecutive channels
       float x[8];
-      const bool keep = tile * 16 + r < valid;
+      const bool keep = tile * 16 + r >= seen.lo && tile * 16 + r < seen.hi;
       const unsigned word = reinterpret_cast<const unsigned*>(kt)[r * (4 * NG) + t * NG + u];
       const unsigned sm = reinterpret_cast<const unsigned*>(kt + CODES)[r * NG + u];
 #pragma unroll
@@ -434,7 +440,7 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float y = fmaf(sc[e], (float)((h >> (4 * c)) & 15), mn[e]);
-          x[c] = r < valid ? (HALF ? y * v_by : y) : 0.f;
+          x[c] = r >= seen.lo && r < seen.hi ? (HALF ? y * v_by : y) : 0.f;
         }
         store4(vo + (size_t)r * HD + u * 32 + g * 4, x[0], x[1], x[2], x[3]);
       }
@@ -1636,7 +1642,7 @@ CO_EXPORT long coheryn_kv4_factor_floats(int n, int nkv) {
 }
 
 // The pages of requests b = 0..n-1 of a block table, dense: entry (b, j) becomes page b * width + j of k_out and v_out [n * width, nkv, page_size, HD]
-// and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length are zeros.  In bfloat16, or, with `factors` (float32
+// and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length, or in front of what its first new token sees, are zeros.  In bfloat16, or, with `factors` (float32
 // [coheryn_kv4_factor_floats(n, nkv)]; place 2 (b nkv + kv head) gets what that list's keys have to be multiplied by, the next what its values do), in
 // scaled float16.
 CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,

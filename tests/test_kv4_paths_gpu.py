@@ -104,6 +104,20 @@ def test_many_keys_of_little_weight(hd, top, context):
     kp.check(rows, q, out, q_lens, heads, BF16)
 
 
+# ------------------------------------------------------------------------------------ windows
+@pytest.mark.parametrize("hd,page_size", [(64, 64), (128, 16), (128, 256), (96, 32), (64, 48)])
+def test_what_lies_in_front_of_the_window(hd, page_size):
+    """Values, and keys, that are not numbers at positions that no row of the request sees, in the page of the first that one does."""
+    heads, nkv, window, q_lens, lens = 4, 1, 40, [70, 1, 66], [200, 90, 301]
+    k, v = kp.random_rows(7, lens, nkv, hd)
+    for b, (m, n) in enumerate(zip(q_lens, lens)):
+        k[b][:n - m - window + 1] = np.nan
+        v[b][:n - m - window + 1] = np.nan
+    rows = kp.Rows(k, v, page_size)
+    q = queries(8, q_lens, heads, hd)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads, window), q_lens, heads, BF16, window)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
