@@ -372,7 +372,7 @@ __device__ __forceinline__ float2 to_float16_range(float most) {
 template <typename T>
 __global__ void __launch_bounds__(128)
 kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, int num_pages, int nkv, int page_size,
-                 const int* __restrict__ table, int table_ld, int width, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
+                 const int* __restrict__ table, int table_ld, int width, int slots, const int* __restrict__ cu_q, const int* __restrict__ lens, int window,
                  T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ out_table, const float2* __restrict__ range, int range_parts,
                  float2* __restrict__ factors, int* __restrict__ status) {
   constexpr bool HALF = sizeof(T) == 2 && !std::is_same<T, bf16>::value;
@@ -380,10 +380,13 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
   co_pdl_launch_dependents();
   co_pdl_wait();
   const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const long long entry = (long long)b * width + j;
   // The loads that depend on nothing first: a block lives for little more than its chain of them.
   const int page = table[(size_t)b * table_ld + j];
   Seen seen = lens ? rows_seen(cu_q, lens, b, j, page_size, window) : Seen{0, page_size};
+  // A request's entries that are seen lie side by side: the first of them takes the first of its `slots` pages.
+  const int slot = lens && window > 0 ? j - max(0, lens[b] - (cu_q[b + 1] - cu_q[b]) - window + 1) / page_size : j;
+  const long long entry = (long long)b * slots + slot;
+  int* place = out_table ? out_table + (size_t)b * width + j : nullptr;
   float k_by = 1.f, v_by = 1.f;
   if constexpr (HALF) {             // float16: times the powers of two that the largest values ask for
     static_assert(RANGE_BLOCKS <= 128, "a thread per partial answer of a list");
@@ -398,14 +401,15 @@ kv4_pages_kernel(const unsigned char* __restrict__ k_cache, const unsigned char*
     v_by = v2.x;
     if (j == 0 && threadIdx.x == 0) factors[list] = make_float2(k2.y, v2.y);
   }
-  if (seen.hi == 0) {
-    if (out_table && kvh == 0 && threadIdx.x == 0) out_table[entry] = -1;
+  if (seen.hi == 0 || slot >= slots) {       // (more than there is room for: lengths that are not those the call was sized by)
+    if (place && kvh == 0 && threadIdx.x == 0) *place = -1;
+    if (seen.hi && status && threadIdx.x == 0) *status = BAD_INDEX;
     return;
   }
   const bool known = page >= 0 && page < num_pages;
   if (!known) seen.hi = 0;
   if (kvh == 0 && threadIdx.x == 0) {
-    if (out_table) out_table[entry] = known ? (int)entry : -1;
+    if (place) *place = known ? (int)entry : -1;
     if (status && (!known || (lens && lens[b] > width * page_size))) *status = BAD_INDEX;      // (or the table ends before the request)
   }
   T* ko = k_out + ((size_t)entry * nkv + kvh) * page_size * HD;
@@ -1528,14 +1532,14 @@ CO_EXPORT int coheryn_kv4_write(const void* qkv, long ld, int dtype, const int* 
 constexpr int PAGES_F16 = 2;      // beside the dtype codes
 
 static int launch_pages(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
-                        int width, int n, const int* cu_q, const int* lens, int window, void* k_out, void* v_out, int dtype, int* out_table,
+                        int width, int slots, int n, const int* cu_q, const int* lens, int window, void* k_out, void* v_out, int dtype, int* out_table,
                         const float2* range, int parts, float2* factors, int* status, cudaStream_t stream) {
   if (nkv > 65535 || n > 65535) CO_FAIL("kv4_pages: %d requests, %d kv heads", n, nkv);
   const dim3 grid((unsigned)width, (unsigned)nkv, (unsigned)n);
   auto with = [&](auto* x) {
     typedef decltype(x) P;
     co_launch(kv4_pages_kernel<std::remove_pointer_t<P>>, grid, dim3(128), 0, stream, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
-              num_pages, nkv, page_size, table, table_ld, width, cu_q, lens, window, (P)k_out, (P)v_out, out_table, range, parts, factors, status);
+              num_pages, nkv, page_size, table, table_ld, width, slots, cu_q, lens, window, (P)k_out, (P)v_out, out_table, range, parts, factors, status);
   };
   if (dtype == CO_F32) with((float*)nullptr);
   else if (dtype == PAGES_F16) with((__half*)nullptr);
@@ -1551,7 +1555,7 @@ CO_EXPORT int coheryn_kv4_pages(const void* k_cache, const void* v_cache, int nu
   if (check_pages("kv4_pages", nkv, page_size, num_pages)) return 1;
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15))
     CO_FAIL("kv4_pages: operands must be 16-byte aligned");
-  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, nullptr, 0,
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, pages, n, n, n, 1, nullptr, nullptr, 0, k_out, v_out, dtype, nullptr, nullptr, 0,
                       nullptr, status, stream);
 }
 
@@ -1641,18 +1645,19 @@ CO_EXPORT long coheryn_kv4_factor_floats(int n, int nkv) {
   return 2 * lists + 2 * lists * range_parts(lists);
 }
 
-// The pages of requests b = 0..n-1 of a block table, dense: entry (b, j) becomes page b * width + j of k_out and v_out [n * width, nkv, page_size, HD]
-// and of out_table [n, width] (-1: not needed).  Rows at or behind a request's length, or in front of what its first new token sees, are zeros.  In bfloat16, or, with `factors` (float32
+// The pages of requests b = 0..n-1 of a block table, dense: of request b's entries those that its new tokens see, `slots` at most,
+// become pages b * slots.. of k_out and v_out [n * slots, nkv, page_size, HD], and out_table [n, width] says which (-1: not needed).  Rows at or
+// behind a request's length, or in front of what its first new token sees, are zeros.  In bfloat16, or, with `factors` (float32
 // [coheryn_kv4_factor_floats(n, nkv)]; place 2 (b nkv + kv head) gets what that list's keys have to be multiplied by, the next what its values do), in
 // scaled float16.
 CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int num_pages, int nkv, int page_size, const int* table, int table_ld,
-                                 int width, int n, const int* cu_q, const int* kv_lens, int window, void* k_out, void* v_out, int* out_table,
+                                 int width, int slots, int n, const int* cu_q, const int* kv_lens, int window, void* k_out, void* v_out, int* out_table,
                                  float* factors, int* status, cudaStream_t stream) {
   if (n <= 0 || width <= 0) return 0;
   if (check_pages("kv4_expand", nkv, page_size, num_pages)) return 1;
   if (((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || ((uintptr_t)factors & 7))
     CO_FAIL("kv4_expand: operands must be 16-byte aligned");
-  if (width > table_ld) CO_FAIL("kv4_expand: %d entries of rows of %d", width, table_ld);
+  if (width > table_ld || slots < 1) CO_FAIL("kv4_expand: %d entries of rows of %d, %d pages", width, table_ld, slots);
   const long long lists = (long long)n * nkv;
   const int parts = range_parts(lists);
   float2* range = factors ? reinterpret_cast<float2*>(factors) + lists : nullptr;
@@ -1662,6 +1667,6 @@ CO_EXPORT int coheryn_kv4_expand(const void* k_cache, const void* v_cache, int n
               num_pages, nkv, page_size, table, table_ld, width, cu_q, kv_lens, window, parts, range);
     CO_CHECK_LAUNCH("kv4_range");
   }
-  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, n, cu_q, kv_lens, window, k_out, v_out,
+  return launch_pages(k_cache, v_cache, num_pages, nkv, page_size, table, table_ld, width, slots, n, cu_q, kv_lens, window, k_out, v_out,
                       factors ? PAGES_F16 : CO_BF16, out_table, (const float2*)range, parts, reinterpret_cast<float2*>(factors), status, stream);
 }

@@ -2464,7 +2464,9 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
     # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages.
     width = min(W, -(-max_kv_len // page_size))
-    most = max(1, min(65535, KV4_EXPAND_BYTES // max(1, width * num_kv_heads * page_size * head_dim * 4)))
+    # Pages that a request may need: all of its entries, or those that hold what its first new token sees and all behind.
+    slots = min(width, (window + longest - 2) // page_size + 2) if window else width
+    most = max(1, min(65535, KV4_EXPAND_BYTES // max(1, slots * num_kv_heads * page_size * head_dim * 4)))
     half = bool(lib.coheryn_kv4_prompt_takes(c_int(num_heads), c_int(num_kv_heads), c_int(page_size))) and scale > 0
     b = 0
     while b < B:
@@ -2475,12 +2477,12 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             b += 1
             continue
         n, rows = e - b, max(q_lens[b:e]) * G
-        k, v = q.new_empty((2, n * width, num_kv_heads, page_size, head_dim)).unbind(0)       # (16 bits a value, whichever kind)
+        k, v = q.new_empty((2, n * slots, num_kv_heads, page_size, head_dim)).unbind(0)       # (16 bits a value, whichever kind)
         table = block_tables.new_empty((n, width))
         factors = torch.empty(int(lib.coheryn_kv4_factor_floats(c_int(n), c_int(num_kv_heads))), dtype=torch.float32, device=q.device) if half else None
         cu, lens = cu_q.data_ptr() + 4 * b, kv_lens.data_ptr() + 4 * b
-        rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiippipppppp")(
-            k_cache.data_ptr(), v_cache.data_ptr(), num_pages, num_kv_heads, page_size, block_tables.data_ptr() + 4 * W * b, W, width, n, cu, lens,
+        rc = _entry(lib, "coheryn_kv4_expand", "ppiiipiiiippipppppp")(
+            k_cache.data_ptr(), v_cache.data_ptr(), num_pages, num_kv_heads, page_size, block_tables.data_ptr() + 4 * W * b, W, width, slots, n, cu, lens,
             window or 0, k.data_ptr(), v.data_ptr(), table.data_ptr(), _at(factors), status, stream)
         if rc:
             _check(lib, rc)
@@ -2490,7 +2492,7 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             floats = int(lib.coheryn_kv4_prompt_scratch_floats(c_int(num_heads), c_int(num_kv_heads), c_int(n), c_int(rows), c_int(parts)))
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
             rc = _entry(lib, "coheryn_kv4_prompt", "pliplppipippiiiiifipiplpp")(
-                q_at, q_ld, T, out_at, out_ld, k.data_ptr(), v.data_ptr(), n * width, table.data_ptr(), width, cu, lens, n, num_heads, num_kv_heads,
+                q_at, q_ld, T, out_at, out_ld, k.data_ptr(), v.data_ptr(), n * slots, table.data_ptr(), width, cu, lens, n, num_heads, num_kv_heads,
                 page_size, window or 0, scale, rows, factors.data_ptr(), parts, _at(scratch), floats, status, stream)
             if rc:
                 _check(lib, rc)
@@ -2499,5 +2501,5 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             _check(prompt, prompt.coheryn_attention_bf16(
                 c_void_p(q_at), c_long(q_ld), c_void_p(out_at), c_long(out_ld), _ptr(k), _ptr(v), _ptr(table), c_int(width), c_void_p(cu), c_void_p(lens),
                 c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
-                c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * width), c_int(0), c_void_p(stream)))
+                c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * slots), c_int(0), c_void_p(stream)))
         b = e

@@ -118,6 +118,29 @@ def test_what_lies_in_front_of_the_window(hd, page_size):
     kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads, window), q_lens, heads, BF16, window)
 
 
+def temporaries(call):
+    call()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("hd", [128, 96])
+def test_a_window_bounds_the_expanded_pages(hd):
+    """200 tokens at 16,384 positions that see 256 each: 456 positions of 8 kv heads in 16 bits are 1.9 MB at head size 128, all of them 67."""
+    heads, nkv, window, q_lens, lens = 8, 8, 256, [200], [16384]
+    rng = np.random.default_rng(9)
+    k, v = [rng.standard_normal((lens[0], nkv, hd)).astype(np.float32) for _ in range(2)]
+    rows = kp.Rows([k], [v])
+    q = queries(9, q_lens, heads, hd)
+    out = torch.zeros_like(q)
+    assert temporaries(lambda: kp.attend(ops(), rows, q, q_lens, heads, window, out=out)) < 4 << 20
+    kp.check(rows, q, out, q_lens, heads, BF16, window)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
