@@ -2389,17 +2389,18 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     """``attention`` over the 4-bit pages of ``group``."""
     attention_kv4_rows(q, out, k_cache, v_cache, step.block_tables[group], step.token_req, step.positions, num_heads, num_kv_heads,
                        head_dim, page_size, window, scale, cu_q=step.cu_q, kv_lens=step.kv_lens, q_lens=step.q_lens,
-                       max_kv_len=step.max_kv_len)
+                       max_kv_len=step.max_kv_len, kv_lens_host=step.kv_lens_host or None)
 
 
 def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads, num_kv_heads, head_dim, page_size, window,
-                       scale, cu_q=None, kv_lens=None, q_lens=None, max_kv_len=None, force_simple=False) -> None:
+                       scale, cu_q=None, kv_lens=None, q_lens=None, max_kv_len=None, force_simple=False, kv_lens_host=None) -> None:
     """Attention of rows (request token_req[i] at position positions[i]) over the 4-bit pages of a cache, causal, with an
     optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros.
     bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
     ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``kv4_direct_rows(head_dim)`` rows
     per kv head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
-    value and go through the prompt kernels.  Everything else goes to a kernel in float32 arithmetic."""
+    value and go through the prompt kernels; ``kv_lens_host`` (the requests' lengths once more, on the host) sizes what that takes by
+    the portions themselves and not by ``max_kv_len``.  Everything else goes to a kernel in float32 arithmetic."""
     if not force_simple and q.is_cuda:
         lib = kv4_lib(head_dim)
         rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
@@ -2446,6 +2447,8 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     _words(B + 1, cu_q=cu_q)
     if block_tables.shape[0] != B or B == 0:
         raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
+    if kv_lens_host is not None and len(kv_lens_host) != B:
+        raise KernelError(f"attention_kv4: {len(kv_lens_host)} lengths on the host for {B} requests")
     limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly
     longest = max(q_lens)
     direct = longest if longest <= limit else max((n for n in q_lens if n <= limit), default=0)
@@ -2463,15 +2466,19 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         return
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
     # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages.
-    width = min(W, -(-max_kv_len // page_size))
-    # Pages that a request may need: all of its entries, or those that hold what its first new token sees and all behind.
-    slots = min(width, (window + longest - 2) // page_size + 2) if window else width
-    most = max(1, min(65535, KV4_EXPAND_BYTES // max(1, slots * num_kv_heads * page_size * head_dim * 4)))
+    page_bytes = num_kv_heads * page_size * head_dim * 4
     half = bool(lib.coheryn_kv4_prompt_takes(c_int(num_heads), c_int(num_kv_heads), c_int(page_size))) and scale > 0
     b = 0
     while b < B:
-        e = b
-        while e < B and e - b < most and q_lens[e] > limit:
+        e, longest_kv, width, slots = b, 0, 0, 0
+        while e < B and e - b < 65535 and q_lens[e] > limit:
+            kv = kv_lens_host[e] if kv_lens_host is not None else max_kv_len
+            entries = min(W, -(-kv // page_size))
+            # Pages that the request may need: all of its entries, or those that hold what its first new token sees and all behind.
+            need = min(entries, (window + q_lens[e] - 2) // page_size + 2) if window else entries
+            if e > b and (e - b + 1) * max(slots, need) * page_bytes > KV4_EXPAND_BYTES:
+                break
+            longest_kv, width, slots = max(longest_kv, kv), max(width, entries), max(slots, need)
             e += 1
         if e == b:
             b += 1
@@ -2488,7 +2495,7 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             _check(lib, rc)
         if half:
             parts = int(lib.coheryn_kv4_prompt_parts(c_int(num_heads), c_int(num_kv_heads), c_int(n), c_int(sum(q_lens[b:e])), c_int(rows),
-                                                     c_int(max_kv_len), c_int(window or 0)))
+                                                     c_int(longest_kv), c_int(window or 0)))
             floats = int(lib.coheryn_kv4_prompt_scratch_floats(c_int(num_heads), c_int(num_kv_heads), c_int(n), c_int(rows), c_int(parts)))
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
             rc = _entry(lib, "coheryn_kv4_prompt", "pliplppipippiiiiifipiplpp")(
@@ -2501,5 +2508,5 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
             _check(prompt, prompt.coheryn_attention_bf16(
                 c_void_p(q_at), c_long(q_ld), c_void_p(out_at), c_long(out_ld), _ptr(k), _ptr(v), _ptr(table), c_int(width), c_void_p(cu), c_void_p(lens),
                 c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(page_size), c_int(window or 0), c_float(scale), c_int(rows), c_int(0), c_int(n),
-                c_int(max_kv_len), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * slots), c_int(0), c_void_p(stream)))
+                c_int(longest_kv), c_void_p(0), c_long(0), c_void_p(status), c_int(T), c_int(n * slots), c_int(0), c_void_p(stream)))
         b = e

@@ -141,6 +141,20 @@ def test_a_window_bounds_the_expanded_pages(hd):
     kp.check(rows, q, out, q_lens, heads, BF16, window)
 
 
+@pytest.mark.parametrize("hd", [64, 96])
+def test_a_portion_beside_a_long_context_takes_its_own_pages(hd):
+    """150 tokens beside a decoding request of 60,000 positions: 150 positions of 8 kv heads in 16 bits are 0.3 MB at head size 64, 60,000 123."""
+    heads, nkv, q_lens, lens = 8, 8, [1, 150, 140], [60000, 150, 300]
+    rng = np.random.default_rng(12)
+    base = rng.standard_normal((500, nkv, hd)).astype(np.float32)
+    k, v = kp.random_rows(12, lens[1:], nkv, hd)
+    rows = kp.Rows([np.tile(base, (120, 1, 1))] + k, [np.tile(base[::-1], (120, 1, 1))] + v)
+    q = queries(13, q_lens, heads, hd)
+    out = torch.zeros_like(q)
+    assert temporaries(lambda: kp.attend(ops(), rows, q, q_lens, heads, out=out, kv_lens_host=list(lens))) < 12 << 20
+    kp.check(rows, q, out, q_lens, heads, BF16)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
@@ -178,3 +192,17 @@ def test_parts_joined_over_a_long_context(hd):
     rows = kp.Rows(k, v)
     q = queries(21, q_lens, heads, hd)
     kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
+
+
+# ------------------------------------------------------------------------------------ refusals
+def portion_call(q_lens=(80, 1), **more):
+    k, v = kp.random_rows(22, [90, 20], 2, 64)
+    rows = kp.Rows(k, v)
+    q = queries(23, [81], 4, 64)
+    return kp.attend(ops(), rows, q, list(q_lens), 4, **more)
+
+
+def test_lengths_on_the_host_for_other_requests_are_refused():
+    portion_call(kv_lens_host=[90, 20])
+    with pytest.raises(ops().KernelError, match="lengths on the host"):
+        portion_call(kv_lens_host=[90])
