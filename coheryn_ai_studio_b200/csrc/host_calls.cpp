@@ -205,13 +205,15 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (!PyList_Check(a[18]) || a[16] == Py_None || a[17] == Py_None || a[19] == Py_None) return none();
     const long B = (long)PyList_GET_SIZE(a[18]), G = nh / nkv, longest_kv = c.number(a[19]);
-    long longest = 0;
+    long longest = 0, tokens = 0;
     for (long b = 0; b < B; ++b) {
       const long x = c.number(PyList_GET_ITEM(a[18], b));
+      if (x < 0) return none();
       longest = x > longest ? x : longest;
+      tokens += x;
     }
     int *cu_q = c.words(a[16], B + 1), *kv_lens = c.words(a[17], B);
-    if (!c.ok || B < 1 || B > 65535 || tt.size(0) != B || longest < 1 || longest * G > most || longest_kv < 0) return none();
+    if (!c.ok || B < 1 || B > 65535 || tt.size(0) != B || tokens > T || longest < 1 || longest * G > most || longest_kv < 0) return none();
     if (q->stride(0) % 8 || (uintptr_t)q->data_ptr() % 16 || out->stride(0) % 4 || (uintptr_t)out->data_ptr() % 8) return none();
     // The positions that a request's rows see, from a multiple of 16 on: by these the kernel's units are counted.
     const long seen = window > 0 ? std::min(longest_kv, window + longest + 14) : longest_kv;

@@ -2447,6 +2447,8 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     _words(B + 1, cu_q=cu_q)
     if block_tables.shape[0] != B or B == 0:
         raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
+    if min(q_lens) < 0 or sum(q_lens) > T:
+        raise KernelError(f"attention_kv4: requests of {sum(q_lens)} tokens in {T} rows (shortest {min(q_lens)})")
     if kv_lens_host is not None and len(kv_lens_host) != B:
         raise KernelError(f"attention_kv4: {len(kv_lens_host)} lengths on the host for {B} requests")
     limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly

@@ -206,3 +206,14 @@ def test_lengths_on_the_host_for_other_requests_are_refused():
     portion_call(kv_lens_host=[90, 20])
     with pytest.raises(ops().KernelError, match="lengths on the host"):
         portion_call(kv_lens_host=[90])
+
+
+@pytest.mark.parametrize("q_lens", [(81, 1), (1, 81), (82, -1), (-1, 1), (2, -1)])
+def test_lengths_that_do_not_fit_the_rows_are_refused(q_lens):
+    """Refused on the host, before a kernel would follow such offsets (those on the device here are all zeros)."""
+    k, v = kp.random_rows(22, [90, 20], 2, 64)
+    rows = kp.Rows(k, v)
+    q, none = queries(23, [81], 4, 64), torch.zeros(81, dtype=torch.int32, device=DEV)
+    with pytest.raises(ops().KernelError, match="in 81 rows"):
+        ops().attention_kv4_rows(q, torch.zeros_like(q), rows.k_cache, rows.v_cache, torch.from_numpy(rows.table).to(DEV), none, none, 4, 2, 64, 16, None,
+                                 0.125, cu_q=none[:3], kv_lens=none[:2], q_lens=list(q_lens), max_kv_len=90)
