@@ -2427,6 +2427,9 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         return
     lib = kv4_lib(head_dim)
     q_ld, out_ld, q_at, out_at = q.stride(0), out.stride(0), q.data_ptr(), out.data_ptr()
+    # The prompt kernels find a row's maximum before they scale it, which a scale that is not positive would turn round.
+    if not scale > 0 and q_lens is not None and len(q_lens) and max(q_lens) * (num_heads // num_kv_heads) > kv4_direct_rows(head_dim):
+        force_simple = True
     status, stream = tc_status(q.device).data_ptr(), _stream_number(device)
     num_pages, W = k_cache.shape[0], block_tables.shape[1]
     if (force_simple or q.dtype is not torch.bfloat16 or cu_q is None or kv_lens is None or q_lens is None or max_kv_len is None

@@ -155,6 +155,21 @@ def test_a_portion_beside_a_long_context_takes_its_own_pages(hd):
     kp.check(rows, q, out, q_lens, heads, BF16)
 
 
+# ------------------------------------------------------------------------------------ scales
+@pytest.mark.parametrize("hd", [64, 128, 96, 256])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales_that_are_not_positive(hd, scale):
+    heads, nkv, q_lens, lens = 4, 2, [90, 1, 70], [120, 33, 70]
+    k, v = kp.random_rows(14, lens, nkv, hd)
+    rows = kp.Rows(k, v)
+    q = queries(15, q_lens, heads, hd)
+    for lens_of_call in (q_lens, [1, 1, 2]):
+        some = q[:sum(lens_of_call)]
+        out = kp.attend(ops(), rows, some, lens_of_call, heads, scale=scale)
+        direct = ops().kv4_direct_rows(hd) if max(lens_of_call) * 2 <= ops().kv4_direct_rows(hd) else 0         # all rows, or none
+        kp.check(rows, some, out, lens_of_call, heads, BF16, scale=scale, direct_rows=direct)
+
+
 # ------------------------------------------------------------------------------------ every way, every head size
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("heads,nkv,window", [(6, 2, None), (3, 1, 37), (4, 4, None)])
