@@ -188,23 +188,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& tt = THPVariable_Unpack(a[7]);
     if (tt.dim() != 2 || tt.size(0) > 0x7fffffffL || tt.size(1) > 0x7fffffffL) return none();
     const float scale = (float)PyFloat_AS_DOUBLE(a[15]);
-    if (code == 0) {
-      int *req = c.words(a[8], T), *pos = c.words(a[9], T);
-      const long longest = a[19] == Py_None ? 0 : c.number(a[19]);
-      if (!c.ok) return none();
-      typedef int (*Parts)(int, int, int, int);
-      const int parts = ((Parts)address(a[22]))((int)T, (int)nkv, (int)longest, (int)window);
-      const long floats = parts > 1 ? T * nh * parts * (hd + 2) : 0;
-      at::Tensor scratch;
-      if (floats) scratch = at::empty({floats}, q->options().dtype(at::kFloat));
-      typedef int (*Fn)(const void*, long, void*, long, int, const void*, const void*, int, const int*, int, int, const int*, const int*, int, int, int, int, int,
-                        float, int, float*, long, int*, void*);
-      return PyLong_FromLong(((Fn)address(a[2]))(q->data_ptr(), (long)q->stride(0), out->data_ptr(), (long)out->stride(0), code, k, v, (int)pages, table,
-                                                 (int)tt.size(1), (int)tt.size(0), req, pos, (int)T, (int)nh, (int)nkv, (int)page_size, (int)window, scale, parts,
-                                                 floats ? (float*)scratch.data_ptr() : nullptr, floats, status, c.stream()));
-    }
-    if (!PyList_Check(a[18]) || a[16] == Py_None || a[17] == Py_None || a[19] == Py_None) return none();
-    const long B = (long)PyList_GET_SIZE(a[18]), G = nh / nkv, longest_kv = c.number(a[19]);
+    // The requests' tokens; rows behind the last one's stay as they are.
+    const bool runs = PyList_Check(a[18]);
+    const long B = runs ? (long)PyList_GET_SIZE(a[18]) : 0;
     long longest = 0, tokens = 0;
     for (long b = 0; b < B; ++b) {
       const long x = c.number(PyList_GET_ITEM(a[18], b));
@@ -212,8 +198,26 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       longest = x > longest ? x : longest;
       tokens += x;
     }
+    if (!c.ok || tokens > T || (runs ? tokens < 1 : a[18] != Py_None)) return none();
+    if (code == 0) {
+      int *req = c.words(a[8], T), *pos = c.words(a[9], T);
+      const long rows = runs ? tokens : T, longest_kv = a[19] == Py_None ? 0 : c.number(a[19]);
+      if (!c.ok) return none();
+      typedef int (*Parts)(int, int, int, int);
+      const int parts = ((Parts)address(a[22]))((int)rows, (int)nkv, (int)longest_kv, (int)window);
+      const long floats = parts > 1 ? rows * nh * parts * (hd + 2) : 0;
+      at::Tensor scratch;
+      if (floats) scratch = at::empty({floats}, q->options().dtype(at::kFloat));
+      typedef int (*Fn)(const void*, long, void*, long, int, const void*, const void*, int, const int*, int, int, const int*, const int*, int, int, int, int, int,
+                        float, int, float*, long, int*, void*);
+      return PyLong_FromLong(((Fn)address(a[2]))(q->data_ptr(), (long)q->stride(0), out->data_ptr(), (long)out->stride(0), code, k, v, (int)pages, table,
+                                                 (int)tt.size(1), (int)tt.size(0), req, pos, (int)rows, (int)nh, (int)nkv, (int)page_size, (int)window, scale, parts,
+                                                 floats ? (float*)scratch.data_ptr() : nullptr, floats, status, c.stream()));
+    }
+    if (!runs || a[16] == Py_None || a[17] == Py_None || a[19] == Py_None) return none();
+    const long G = nh / nkv, longest_kv = c.number(a[19]);
     int *cu_q = c.words(a[16], B + 1), *kv_lens = c.words(a[17], B);
-    if (!c.ok || B < 1 || B > 65535 || tt.size(0) != B || tokens > T || longest < 1 || longest * G > most || longest_kv < 0) return none();
+    if (!c.ok || B < 1 || B > 65535 || tt.size(0) != B || longest * G > most || longest_kv < 0) return none();
     if (q->stride(0) % 8 || (uintptr_t)q->data_ptr() % 16 || out->stride(0) % 4 || (uintptr_t)out->data_ptr() % 8) return none();
     // The positions that a request's rows see, from a multiple of 16 on: by these the kernel's units are counted.
     const long seen = window > 0 ? std::min(longest_kv, window + longest + 14) : longest_kv;

@@ -2395,7 +2395,8 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
 def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positions, num_heads, num_kv_heads, head_dim, page_size, window,
                        scale, cu_q=None, kv_lens=None, q_lens=None, max_kv_len=None, force_simple=False, kv_lens_host=None) -> None:
     """Attention of rows (request token_req[i] at position positions[i]) over the 4-bit pages of a cache, causal, with an
-    optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros.
+    optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros; with ``q_lens`` the rows
+    behind the last request's stay as they are.
     bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
     ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``kv4_direct_rows(head_dim)`` rows
     per kv head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
@@ -2425,6 +2426,9 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         raise KernelError("an attention window must hold at least one position")
     if T == 0:
         return
+    tokens = T if q_lens is None else sum(q_lens)          # rows behind the last request stay as they are
+    if q_lens and (min(q_lens) < 0 or tokens > T):
+        raise KernelError(f"attention_kv4: requests of {tokens} tokens in {T} rows (shortest {min(q_lens)})")
     lib = kv4_lib(head_dim)
     q_ld, out_ld, q_at, out_at = q.stride(0), out.stride(0), q.data_ptr(), out.data_ptr()
     # The prompt kernels find a row's maximum before they scale it, which a scale that is not positive would turn round.
@@ -2435,12 +2439,12 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     if (force_simple or q.dtype is not torch.bfloat16 or cu_q is None or kv_lens is None or q_lens is None or max_kv_len is None
             or q_ld % 8 or q_at % 16 or out_ld % 4 or out_at % 8):
         _words(T, token_req=token_req, positions=positions)
-        parts = int(lib.coheryn_kv4_simple_parts(c_int(T), c_int(num_kv_heads), c_int(max_kv_len or 0), c_int(window or 0)))
-        floats = T * num_heads * parts * (head_dim + 2) if parts > 1 else 0
+        parts = int(lib.coheryn_kv4_simple_parts(c_int(tokens), c_int(num_kv_heads), c_int(max_kv_len or 0), c_int(window or 0)))
+        floats = tokens * num_heads * parts * (head_dim + 2) if parts > 1 else 0
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         rc = _entry(lib, "coheryn_kv4_attention_simple", "plplippipiippiiiiifiplpp")(
             q_at, q_ld, out_at, out_ld, _code(q), k_cache.data_ptr(), v_cache.data_ptr(), num_pages, block_tables.data_ptr(), W,
-            block_tables.shape[0], token_req.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, page_size, window or 0, scale, parts, _at(scratch), floats,
+            block_tables.shape[0], token_req.data_ptr(), positions.data_ptr(), tokens, num_heads, num_kv_heads, page_size, window or 0, scale, parts, _at(scratch), floats,
             status, stream)
         if rc:
             _check(lib, rc)
@@ -2450,8 +2454,6 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     _words(B + 1, cu_q=cu_q)
     if block_tables.shape[0] != B or B == 0:
         raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
-    if min(q_lens) < 0 or sum(q_lens) > T:
-        raise KernelError(f"attention_kv4: requests of {sum(q_lens)} tokens in {T} rows (shortest {min(q_lens)})")
     if kv_lens_host is not None and len(kv_lens_host) != B:
         raise KernelError(f"attention_kv4: {len(kv_lens_host)} lengths on the host for {B} requests")
     limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly

@@ -209,6 +209,27 @@ def test_parts_joined_over_a_long_context(hd):
     kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
 
 
+# ------------------------------------------------------------------------------------ rows behind the last request
+@pytest.mark.parametrize("dtype,simple,scale", [(BF16, False, 0.125), (BF16, True, 0.125), (BF16, False, -0.125), (torch.float32, False, 0.125)])
+@pytest.mark.parametrize("q_lens", [[3, 1], [80, 1], [0, 0]])
+def test_rows_behind_the_last_request_stay(dtype, simple, scale, q_lens):
+    """Whichever way the rows go; what a padded batch says about those rows is not read."""
+    heads, nkv, hd, lens = 4, 2, 64, [90, 20]
+    k, v = kp.random_rows(22, lens, nkv, hd)
+    rows = kp.Rows(k, v)
+    T = sum(q_lens)
+    q = queries(23, [T + 5], heads, hd, dtype=dtype)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)      # noqa: E731
+    req = np.concatenate([np.repeat([0, 1], q_lens), np.full(5, 9)])
+    pos = np.concatenate([np.arange(n - m, n) for n, m in zip(lens, q_lens)] + [np.full(5, 2 ** 30)])
+    out = torch.full_like(q, 7.0)
+    ops().attention_kv4_rows(q, out, rows.k_cache, rows.v_cache, i32(rows.table), i32(req), i32(pos), heads, nkv, hd, 16, None, scale,
+                             cu_q=i32(np.concatenate([[0], np.cumsum(q_lens)])), kv_lens=i32(lens), q_lens=q_lens, max_kv_len=90, force_simple=simple)
+    assert (out[T:] == 7).all()
+    # (a scale that is not positive takes the whole call to the float32 kernel when a portion is in it)
+    kp.check(rows, q[:T], out[:T], q_lens, heads, dtype, scale=scale, simple=simple or (scale < 0 and max(q_lens) > 64))
+
+
 # ------------------------------------------------------------------------------------ refusals
 def portion_call(q_lens=(80, 1), **more):
     k, v = kp.random_rows(22, [90, 20], 2, 64)
