@@ -317,10 +317,10 @@ class StepRunner:
         pieces = [dev[a:a + n] for a, n in zip(at.tolist(), sizes)]
         made = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.device)
         cu_q, kv_lens, positions, token_req = made(B + 1), made(B), made(T), made(T)
-        block_tables, slots = [], []
+        block_tables, slots, status = [], [], ops.tc_status(self.device)       # (one of the words that ``check_status`` reads)
         for g, lists in enumerate(tables):
             table, slot = made(B, max(1, max(len(l) for l in lists))), made(T)
-            ops.step_layout(pieces[0], pieces[1], pieces[2 + 2 * g], pieces[3 + 2 * g], self.cache.page_size, table, slot,
+            ops.step_layout(pieces[0], pieces[1], pieces[2 + 2 * g], pieces[3 + 2 * g], self.cache.page_size, table, slot, status=status,
                             **(dict(cu_q=cu_q, kv_lens=kv_lens, positions=positions, token_req=token_req) if g == 0 else {}))
             block_tables.append(table)
             slots.append(slot)
