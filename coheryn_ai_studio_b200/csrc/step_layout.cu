@@ -122,7 +122,7 @@ step_layout_kernel(const int* __restrict__ starts, const int* __restrict__ q_len
       if (j >= first && j - first < n) page = lists.pages[from + j - first];
       else if (j >= 0 && j < first && j < W) page = table[(long long)lo * W + j];
       const long long slot = page < 0 ? -1 : (long long)page * page_size + (pos - j * page_size);
-      if (slot < 0 || slot > 0x7fffffffLL) bad = BAD_PAGES;
+      if (slot < 0 || slot > 0x7fffffffLL) bad = pos < 0 ? BAD_LENGTH : BAD_PAGES;
       slots[t] = slot > 0x7fffffffLL ? -1 : (int)slot;
     }
   }

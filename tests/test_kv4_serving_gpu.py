@@ -39,6 +39,9 @@ def test_a_page_list_that_is_too_short_is_reported(runner):
         runner._step_arrays(starts, q_lens, tables, [])      # (-1 in the place of the slots behind the list)
         with pytest.raises(RuntimeError, match="pages do not hold"):
             runner.check_status()
+    runner._step_arrays(np.array([-1, 3], np.int32), q_lens, [whole, whole], [])
+    with pytest.raises(RuntimeError, match="lengths are negative"):
+        runner.check_status()
     runner.check_status()              # reported once
 
 
