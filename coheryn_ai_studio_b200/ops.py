@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import warnings
 from typing import Optional
 
 import torch
@@ -2190,11 +2191,20 @@ _calls_module = None
 
 def _calls():
     """The module whose functions check the operands in C++ and enter the library; each returns None for a call that is not
-    its ordinary one, which the code below then handles or refuses by name."""
+    its ordinary one, which the code below then handles or refuses by name.  Where it cannot be compiled (it needs the headers of the
+    interpreter and of torch, which no kernel does) or loaded, every call is of that kind: the same kernels, 7 to 10 us more host time."""
     global _calls_module
     if _calls_module is None:
-        _calls_module = build.calls_module()
+        try:
+            _calls_module = build.calls_module()
+        except (build.BuildError, ImportError, OSError) as e:
+            warnings.warn(f"the module of checked calls is not there, operands are checked in Python: {str(e).splitlines()[0]}", RuntimeWarning, stacklevel=3)
+            _calls_module = _NoCalls
     return _calls_module
+
+
+class _NoCalls:
+    layout = write = pages = attention = staticmethod(lambda *operands: None)
 
 
 STEP_LAYOUT_REQUESTS = 11999      # that one call of step_layout takes at most (csrc/step_layout.cu keeps their offsets in 48 KB)

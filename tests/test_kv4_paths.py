@@ -1,9 +1,11 @@
-"""The bounds of the 4-bit cache's attention without a GPU: what a way's own roundings give lies inside, a way that loses more lies outside."""
+"""The 4-bit cache without a GPU: calls without the module that checks operands, and the bounds of its attention (what a way's own roundings
+give lies inside, a way that loses more lies outside)."""
 import numpy as np
 import pytest
 import torch
 
 import kv4_paths as kp
+from coheryn_ai_studio_b200 import ops
 
 
 def rounded_output(rows, q, way, keys, probabilities, dtype=torch.bfloat16):
@@ -49,3 +51,20 @@ def test_rows_come_through_the_pool():
         for b, n in enumerate(rows.lens):
             got = held[[p for p in rows.table[b] if p >= 0]].transpose(0, 2, 1, 3).reshape(-1, 2, 96)
             assert np.array_equal(got[:n], kp.stored(x[b])[0]) and np.isnan(got[n:]).all()
+
+
+def test_without_the_module_of_checked_calls(monkeypatch):
+    """A machine without the headers that it needs runs the calls from Python, and says so once."""
+    import warnings
+    from coheryn_ai_studio_b200.csrc import build
+
+    def missing():
+        raise build.BuildError("the module of checked calls did not compile:\nPython.h: No such file or directory")
+    monkeypatch.setattr(build, "calls_module", missing)
+    monkeypatch.setattr(ops, "_calls_module", None)
+    with pytest.warns(RuntimeWarning, match="checked calls"):
+        calls = ops._calls()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert all(getattr(ops._calls(), n)(1, 2, 3) is None for n in ("layout", "write", "pages", "attention"))
+    assert ops._calls() is calls

@@ -230,6 +230,35 @@ def test_rows_behind_the_last_request_stay(dtype, simple, scale, q_lens):
     kp.check(rows, q[:T], out[:T], q_lens, heads, dtype, scale=scale, simple=simple or (scale < 0 and max(q_lens) > 64))
 
 
+# ------------------------------------------------------------------------------------ operands checked in Python
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_calls_without_the_module_give_the_same(dtype, monkeypatch):
+    """The four operators, with the module that checks their operands and without it: equal bits."""
+    o = ops()
+    heads, nkv, hd, q_lens, lens = 4, 2, 64, [3, 1], [90, 20]
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)      # noqa: E731
+    qkv = queries(24, [110], heads + 2 * nkv, hd, dtype=dtype)
+    table = torch.randn(200, hd // 2, 2, device=DEV)
+
+    def run():
+        entries, slots, pos, req = torch.full((2, 7), 5, dtype=torch.int32, device=DEV), i32(np.zeros(110)), i32(np.zeros(110)), i32(np.zeros(110))
+        o.step_layout(i32([0, 0]), i32([90, 20]), i32([0, 6, 8]), i32([7, 3, 1, 0, 5, 2, 6, 4]), 16, entries, slots, positions=pos, token_req=req)
+        caches = [torch.zeros((9,) + o.kv4_page_shape(nkv, 16, hd), dtype=torch.uint8, device=DEV) for _ in range(2)]
+        q = o.rope_kv4_write(qkv, pos, table, slots, *caches, heads, nkv, hd, hd, 16)
+        rows = torch.cat([q[87:90], q[109:]])
+        out = torch.zeros_like(rows)
+        o.attention_kv4_rows(rows, out, *caches, entries, i32([0, 0, 0, 1]), i32([87, 88, 89, 19]), heads, nkv, hd, 16, None, 0.125, cu_q=i32([0, 3, 4]),
+                             kv_lens=i32(lens), q_lens=q_lens, max_kv_len=90)
+        return [entries, slots, pos, req, *caches, q, out, *o.kv4_pages(*caches, i32([7, 4]), hd, 16, dtype)]
+    module = run()
+    called = []
+    monkeypatch.setattr(o, "_calls_module", o._NoCalls)
+    monkeypatch.setattr(o._NoCalls, "attention", staticmethod(lambda *operands: called.append(1)))
+    for a, b in zip(module, run()):
+        assert torch.equal(a, b)
+    assert called
+
+
 # ------------------------------------------------------------------------------------ refusals
 def portion_call(q_lens=(80, 1), **more):
     k, v = kp.random_rows(22, [90, 20], 2, 64)
