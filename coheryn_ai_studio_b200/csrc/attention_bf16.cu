@@ -338,9 +338,9 @@ attn_tiles_kernel(const bf16* __restrict__ q, long q_stride, bf16* __restrict__ 
   constexpr int TPR = largest_divisor_up_to(CHUNKS, 4);
   constexpr int PIECES = CHUNKS / TPR;
   const int c_row = tid >> 2, c_sub = tid & 3;
-  auto page_for = [&](int tile) -> int {     // block-table entry of this thread's row in a tile
-    const int pos = tile * TILE + c_row;
-    return (tile <= tile_last && pos >= key_first && pos < kv_end) ? table[pos / page_size] : -1;
+  auto page_for = [&](int tile) -> int {     // block-table entry of this thread's row in a tile (none behind the table's end)
+    const int pos = tile * TILE + c_row, blk = pos / page_size;
+    return (tile <= tile_last && pos >= key_first && pos < kv_end && blk < max_blocks) ? table[blk] : -1;
   };
   auto issue = [&](int tile, int page) {     // one commit group per call, possibly empty
     if (tile <= tile_last && c_sub < TPR) {

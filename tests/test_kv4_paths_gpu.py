@@ -155,6 +155,22 @@ def test_a_portion_beside_a_long_context_takes_its_own_pages(hd):
     kp.check(rows, q, out, q_lens, heads, BF16)
 
 
+# ------------------------------------------------------------------------------------ block tables that end early
+@pytest.mark.parametrize("hd", [32, 64, 96, 192])
+def test_a_block_table_that_ends_before_its_request(hd):
+    """Reported; nothing behind the table is read, and rows that see only pages that are there are right."""
+    heads, nkv, q_lens, lens = 4, 2, [90, 70], [90, 200]
+    k, v = kp.random_rows(28, lens, nkv, hd)
+    rows = kp.Rows(k, v)
+    rows.table = np.ascontiguousarray(rows.table[:, :8])
+    q = queries(29, q_lens, heads, hd)
+    out = kp.attend(ops(), rows, q, q_lens, heads)
+    word = ops().tc_status(DEV)
+    assert int(word.item()) == 41
+    word.zero_()
+    kp.check(rows, q[:90], out[:90], [90], heads, BF16, direct_rows=ops().kv4_direct_rows(hd))
+
+
 # ------------------------------------------------------------------------------------ scales
 @pytest.mark.parametrize("hd", [64, 128, 96, 256])
 @pytest.mark.parametrize("scale", [-0.11, 0.0])
