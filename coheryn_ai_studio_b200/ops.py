@@ -2408,10 +2408,12 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     optional ``window``; the arguments are those of ``attention_rows``.  A row that sees no position gives zeros; with ``q_lens`` the rows
     behind the last request's stay as they are.
     bfloat16 rows that are whole runs of consecutive positions per request, ending at the request's last position (``cu_q``,
-    ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host): requests with at most ``kv4_direct_rows(head_dim)`` rows
-    per kv head go to the kernel that reads the 4-bit pages directly, longer portions have their pages expanded to 16 bits a
-    value and go through the prompt kernels; ``kv_lens_host`` (the requests' lengths once more, on the host) sizes what that takes by
-    the portions themselves and not by ``max_kv_len``.  Everything else goes to a kernel in float32 arithmetic."""
+    ``kv_lens`` on the device, ``q_lens`` and ``max_kv_len`` on the host; a request's length counts its new tokens): requests with at
+    most ``kv4_direct_rows(head_dim)`` rows per kv head go to the kernel that reads the 4-bit pages directly, longer portions have
+    their pages expanded to 16 bits a value and go through the prompt kernels; ``kv_lens_host`` (the requests' lengths once more, on
+    the host) sizes what that takes by the portions themselves and not by ``max_kv_len``.  Everything else goes to a kernel in float32
+    arithmetic.  Sums are formed in float32: values of 2^100 and more, and queries of 2^114 and more, may pass its range where the
+    direct kernel adds them up."""
     if not force_simple and q.is_cuda:
         lib = kv4_lib(head_dim)
         rc = _calls().attention(_address(lib, "coheryn_kv4_scratch_floats"), _address(lib, "coheryn_kv4_attention"),
@@ -2439,11 +2441,19 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     tokens = T if q_lens is None else sum(q_lens)          # rows behind the last request stay as they are
     if q_lens and (min(q_lens) < 0 or tokens > T):
         raise KernelError(f"attention_kv4: requests of {tokens} tokens in {T} rows (shortest {min(q_lens)})")
+    if kv_lens_host is not None and (q_lens is None or len(kv_lens_host) != len(q_lens)):
+        raise KernelError(f"attention_kv4: {len(kv_lens_host)} lengths on the host for {len(q_lens or ())} requests")
     lib = kv4_lib(head_dim)
+    G = num_heads // num_kv_heads
+    limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly
+    longest = max(q_lens) if q_lens else 0
+    half = longest > limit and scale > 0 and bool(lib.coheryn_kv4_prompt_takes(c_int(num_heads), c_int(num_kv_heads), c_int(page_size)))
+    if longest > limit and not half and max_kv_len is not None:
+        # The framework's prompt kernels find a row's maximum before they scale it, which a scale that is not positive would turn round, and
+        # count on every row to see its own key.
+        if not scale > 0 or any(n > kv for n, kv in zip(q_lens, kv_lens_host or [max_kv_len] * len(q_lens))):
+            force_simple = True
     q_ld, out_ld, q_at, out_at = q.stride(0), out.stride(0), q.data_ptr(), out.data_ptr()
-    # The prompt kernels find a row's maximum before they scale it, which a scale that is not positive would turn round.
-    if not scale > 0 and q_lens is not None and len(q_lens) and max(q_lens) * (num_heads // num_kv_heads) > kv4_direct_rows(head_dim):
-        force_simple = True
     status, stream = tc_status(q.device).data_ptr(), _stream_number(device)
     num_pages, W = k_cache.shape[0], block_tables.shape[1]
     if (force_simple or q.dtype is not torch.bfloat16 or cu_q is None or kv_lens is None or q_lens is None or max_kv_len is None
@@ -2459,15 +2469,11 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         if rc:
             _check(lib, rc)
         return
-    B, G = len(q_lens), num_heads // num_kv_heads
+    B = len(q_lens)
     _words(B, kv_lens=kv_lens)
     _words(B + 1, cu_q=cu_q)
     if block_tables.shape[0] != B or B == 0:
         raise KernelError(f"attention_kv4: a block table of {block_tables.shape[0]} requests for lengths of {B}")
-    if kv_lens_host is not None and len(kv_lens_host) != B:
-        raise KernelError(f"attention_kv4: {len(kv_lens_host)} lengths on the host for {B} requests")
-    limit = max(kv4_direct_rows(head_dim) // G, 1)         # tokens that a request may bring to be read directly
-    longest = max(q_lens)
     direct = longest if longest <= limit else max((n for n in q_lens if n <= limit), default=0)
     if direct:
         seen = min(max_kv_len, window + direct + 14) if window else max_kv_len        # positions, from a multiple of 16 on
@@ -2484,13 +2490,12 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
     # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages.
     page_bytes = num_kv_heads * page_size * head_dim * 4
-    half = bool(lib.coheryn_kv4_prompt_takes(c_int(num_heads), c_int(num_kv_heads), c_int(page_size))) and scale > 0
     b = 0
     while b < B:
         e, longest_kv, width, slots = b, 0, 0, 0
         while e < B and e - b < 65535 and q_lens[e] > limit:
             kv = kv_lens_host[e] if kv_lens_host is not None else max_kv_len
-            entries = min(W, -(-kv // page_size))
+            entries = max(1, min(W, -(-kv // page_size)))
             # Pages that the request may need: all of its entries, or those that hold what its first new token sees and all behind.
             need = min(entries, (window + q_lens[e] - 2) // page_size + 2) if window else entries
             if e > b and (e - b + 1) * max(slots, need) * page_bytes > KV4_EXPAND_BYTES:

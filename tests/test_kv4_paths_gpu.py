@@ -32,6 +32,37 @@ def queries(seed, q_lens, heads, hd, spread=1.5, dtype=BF16):
     return torch.from_numpy(rng.standard_normal((sum(q_lens), heads * hd)).astype(np.float32) * by).to(dtype).to(DEV)
 
 
+# ------------------------------------------------------------------------------------ rows that see nothing
+@pytest.mark.parametrize("hd", [64, 96, 128, 192])
+@pytest.mark.parametrize("window", [None, 30])
+@pytest.mark.parametrize("lens", [(0, 0), (10, 0), (90, 40)])
+def test_portions_longer_than_their_requests(hd, window, lens):
+    """The first rows stand in front of position 0 and give zeros; the others as ever.  Also where no row of the call sees anything."""
+    heads, nkv, q_lens = 4, 2, [90, 70]
+    k, v = kp.random_rows(25, [90, 40], nkv, hd)
+    rows = kp.Rows(k, v)
+    rows.lens = list(lens)
+    q = queries(26, q_lens, heads, hd)
+    out = kp.attend(ops(), rows, q, q_lens, heads, window, kv_lens_host=list(lens))
+    rows.k, rows.v = ([x[:n] for x, n in zip(y, lens)] for y in (k, v))
+    at = 0
+    for n, length in zip(q_lens, lens):
+        assert (out[at:at + n - min(n, length)] == 0).all()
+        at += n
+    seen = [min(n, length) for n, length in zip(q_lens, lens)]
+    part = lambda x: torch.cat([x[q_lens[0] - seen[0]:q_lens[0]], x[sum(q_lens) - seen[1]:]])        # noqa: E731
+    kp.check(rows, part(q), part(out), seen, heads, BF16, window, simple=hd not in (64, 128), direct_rows=0)
+
+
+def test_a_block_table_without_entries_is_refused():
+    k, v = kp.random_rows(25, [90], 2, 96)
+    for hd in (64, 96):
+        rows = kp.Rows(*[[x[..., :hd] for x in y] for y in (k, v)])
+        rows.table = rows.table[:, :0]
+        with pytest.raises(ops().KernelError):
+            kp.attend(ops(), rows, queries(27, [80], 4, hd), [80], 4)
+
+
 # ------------------------------------------------------------------------------------ query rows and keys of zeros
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("window", [None, 50])
