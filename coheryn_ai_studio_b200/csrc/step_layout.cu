@@ -130,8 +130,6 @@ step_layout_kernel(const int* __restrict__ starts, const int* __restrict__ q_len
 }
 }  // namespace
 
-CO_EXPORT int coheryn_step_layout_max_requests() { return MAX_REQUESTS; }
-
 // cu_q [B + 1], kv_lens [B], positions [T], token_req [T] and slots [T] may be null; table [B, W] is written.
 CO_EXPORT int coheryn_step_layout(const int* starts, const int* q_lens, const int* page_cu, const int* pages, int n_pages,
                                   const int* first, int B, int T, int page_size, int* cu_q, int* kv_lens, int* positions,
