@@ -68,7 +68,7 @@ def way_of(rows, q_len, heads, dtype, scale, simple=False, direct_rows=128):
         return "float32"
     if q_len * (heads // rows.nkv) <= direct_rows:
         return "direct"
-    return "half" if rows.hd in (64, 128) and (128 % rows.page_size == 0 or rows.page_size % 128 == 0) else "bfloat16"
+    return "half" if rows.hd in (64, 128) and heads // rows.nkv <= 128 and (128 % rows.page_size == 0 or rows.page_size % 128 == 0) else "bfloat16"
 
 
 def expected(rows, b, q, scale, window, way, dtype):
@@ -101,8 +101,8 @@ def expected(rows, b, q, scale, window, way, dtype):
             A, d = w @ np.abs(vv), terms * steps * 2.0 ** -23
             # errors up to d in the scores move a probability by a factor within exp(-2 d)..exp(2 d); exponentials 2^-20; sums over the keys
             tol[i, h] = A * (np.expm1(min(2 * d, 5)) + weight + 2.0 ** -20 + (hi - lo + 16) * 2.0 ** -23)
-            if way == "half":       # below 2^-14 a float16 steps by 2^-24
-                tol[i, h] += (hi - lo) * 2.0 ** -32 * np.abs(vv).max(0)
+            # A probability under the smallest normal float32 is none; in float16, 2^7 over the reference, steps are 2^-24 under 2^-14.
+            tol[i, h] += (hi - lo) * (2.0 ** -32 if way == "half" else 2.0 ** -126) * np.abs(vv).max(0)
     return out, tol + np.abs(out) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23) + (2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -140)
 
 

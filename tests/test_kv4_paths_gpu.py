@@ -234,6 +234,14 @@ def test_runs_of_every_length(hd, heads, nkv, window):
         kp.check(rows, x, kp.attend(o, rows, x, few, heads, window, simple=simple), few, heads, x.dtype, window, simple=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("hd,rot,heads,nkv,page_size", [(192, 192, 4, 2, 16), (192, 64, 3, 1, 48), (192, 0, 2, 2, 16), (224, 224, 2, 1, 32), (224, 30, 5, 1, 16),
+                                                        (224, 0, 1, 3, 16), (96, 96, 2, 2, 16), (32, 10, 9, 3, 64)])
+def test_writes_and_pages_of_other_head_sizes(dtype, hd, rot, heads, nkv, page_size):
+    import test_kv4_gpu as base
+    base.test_write_and_pages(dtype, hd, rot, heads, nkv, page_size)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("q_lens,lens", [([1, 2], [2000, 40]), ([5, 1], [300, 5000]), ([70, 40], [200, 1500])])
 def test_sharp_scores(hd, q_lens, lens):
