@@ -2223,8 +2223,9 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
     ``slots`` (page * page_size + offset; -1 where the page is missing), each [T].  Rows of the latter behind the last token
     stay as they are.  With ``first`` [B] the listed pages are entries first[b].. of row b, and the rest of the row stays
     as it is: a table that is kept from step to step gets only what it has gained.
-    ``status`` (int32 [1]) is set to 51 when a length is negative or the tokens do not fit the arrays, to 52 when the
-    lists do not hold the positions; nothing outside the arrays is read or written then.
+    ``status`` (int32 [1]) is set to 51 when a length is negative or the tokens do not fit the arrays, to 52 when a list
+    does not fit the table or, where ``slots`` are asked for, does not hold a position; nothing outside the arrays is read or
+    written then.
 
     An ordinary launch: the arrays are complete before the next kernel in the stream begins, so kernels that look at a
     step's lengths ahead of their wait may follow it directly."""
@@ -2265,11 +2266,12 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
 _kv4_libs = {}
 
 # Requests with at most this many query rows (tokens times heads of a group) read the 4-bit pages directly; longer portions
-# have their pages expanded to 16 bits a value once and go through the prompt kernels.  Directly against expanded, in us: 112 rows
-# of 7 heads over each of 4, 1 x 1,024 positions 10 and 28, 8 x 8,192 103 and 120; 128 rows, 4 over each of 8, 1 x 65,536 210 and 221,
-# 8 x 1,024 52 and 43; 256 rows, 1 x 65,536 399 and 248.  Half as many at head sizes 192 and 256, which the direct kernel takes in tiles of
-# 8 rows instead of 16 and whose prompts have a tcgen05 kernel (256, 8 x 8,192: 64 rows 134 and 165, 128 rows 254 and 167); not at those between
-# (160, 8 x 8,192: 128 rows 183 and 415).
+# have their pages expanded to 16 bits a value once and go through the prompt kernels.  Directly against expanded, us of calls replayed
+# from a graph, head size 128: 112 rows of 7 heads over each of 4, 1 x 1,024 positions 9.9 and 25.2, 8 x 8,192 100 and 99; of 4 over each of
+# 8, 1 x 65,536 64 rows 110 and 180, 112 181 and 181, 128 205 and 181, 256 393 and 199; 8 x 1,024 64 rows 32 and 35, 128 53 and 36.  Half as
+# many at head sizes 192 and 256, which the direct kernel takes in tiles of 8 rows instead of 16 and whose prompts have a tcgen05 kernel
+# (4 heads over 4, 8 x 8,192: 256, 64 rows 132 and 170, 128 rows 252 and 173; 192, 107 and 146, 206 and 149); not at those between, whose
+# prompts have none (128 rows: 160, 181 and 415; 224, 236 and 554).
 KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "128"))
 
 
@@ -2329,7 +2331,7 @@ def rope_kv4_write(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin
     with a negative slot is not kept).  ``qkv`` [T, (heads + 2 kv heads) * head_dim] (rows may be strided) stays as it is;
     the rotated queries [T, heads * head_dim] are returned (a view of ``qkv`` when ``rotary_dim`` is 0; ``positions`` and
     ``cos_sin`` may then be None).  Keys are rounded to the compute type before they are quantised.  A group of 32
-    channels with a value that is not finite is kept as not-a-number.  Two rows with one slot: one of them is kept, or a
+    channels with a value that is not finite, or whose range or minimum passes the largest bfloat16, is kept as not-a-number.  Two rows with one slot: one of them is kept, or a
     mixture."""
     if qkv.is_cuda:
         lib = kv4_lib(head_dim)
@@ -2488,7 +2490,8 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
     if longest <= limit:
         return
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
-    # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages.
+    # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages: these round a key and a value
+    # that a page stands for to the compute type, as a bfloat16 cache does (3.1e-3 to 4.9e-3 against 64 bits, 1.7e-3 in float16).
     page_bytes = num_kv_heads * page_size * head_dim * 4
     b = 0
     while b < B:
