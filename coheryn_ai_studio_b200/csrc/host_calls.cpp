@@ -202,7 +202,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (code == 0) {
       int *req = c.words(a[8], T), *pos = c.words(a[9], T);
       const long rows = runs ? tokens : T, longest_kv = a[19] == Py_None ? 0 : c.number(a[19]);
-      if (!c.ok) return none();
+      if (!c.ok || longest_kv < 0) return none();
       typedef int (*Parts)(int, int, int, int);
       const int parts = ((Parts)address(a[22]))((int)rows, (int)nkv, (int)longest_kv, (int)window);
       const long floats = parts > 1 ? rows * nh * parts * (hd + 2) : 0;

@@ -2248,6 +2248,8 @@ def step_layout(starts: torch.Tensor, q_lens: torch.Tensor, page_cu: torch.Tenso
     _words(T, slots=slots, positions=positions, token_req=token_req)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise KernelError(f"a block table of shape {tuple(block_table.shape)} for {B} requests")
+    if not 1 <= page_size <= POSITIONS:
+        raise KernelError(f"step_layout: pages of {page_size} positions")
     if B == 0:
         if cu_q is not None:
             cu_q.zero_()
@@ -2278,6 +2280,8 @@ KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "128"))
 def kv4_direct_rows(head_dim: int) -> int:
     return KV4_DIRECT_ROWS // 2 if head_dim in (192, 256) else KV4_DIRECT_ROWS
 
+
+POSITIONS = 0x7fffffff      # that 32 bits number: what passes it would reach the kernels cut to its lowest 32 bits
 
 # The expanded pages of a call take at most about this many bytes at a time (one request always goes in one piece).
 KV4_EXPAND_BYTES = 1 << 30
@@ -2438,6 +2442,10 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         raise KernelError("attention_kv4: block_tables must be [requests, entries]")
     if window is not None and window < 1:
         raise KernelError("an attention window must hold at least one position")
+    if window is not None and window > POSITIONS:          # (of more positions than there are: none)
+        window = None
+    if not 0 <= (max_kv_len or 0) <= POSITIONS or any(not 0 <= n <= POSITIONS for n in kv_lens_host or ()):
+        raise KernelError(f"attention_kv4: lengths on the host are 0..{POSITIONS}")
     if T == 0:
         return
     tokens = T if q_lens is None else sum(q_lens)          # rows behind the last request stay as they are

@@ -337,3 +337,24 @@ def test_lengths_that_do_not_fit_the_rows_are_refused(q_lens):
     with pytest.raises(ops().KernelError, match="in 81 rows"):
         ops().attention_kv4_rows(q, torch.zeros_like(q), rows.k_cache, rows.v_cache, torch.from_numpy(rows.table).to(DEV), none, none, 4, 2, 64, 16, None,
                                  0.125, cu_q=none[:3], kv_lens=none[:2], q_lens=list(q_lens), max_kv_len=90)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_numbers_beyond_32_bits(dtype):
+    """A window of more positions than there are is none; lengths and page sizes of that size are refused, not cut to 32 bits."""
+    k, v = kp.random_rows(30, [90, 20], 2, 64)
+    rows = kp.Rows(k, v)
+    for q_lens in ([80, 1], [2, 1]):
+        q = queries(31, q_lens, 4, 64, dtype=dtype)
+        want = kp.attend(ops(), rows, q, q_lens, 4)
+        for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 3, 2 ** 40 + 1):
+            assert torch.equal(kp.attend(ops(), rows, q, q_lens, 4, window), want), window
+        for more in (dict(max_kv_len=2 ** 32 + 90), dict(max_kv_len=-1), dict(kv_lens_host=[2 ** 32 + 90, 20]), dict(kv_lens_host=[-1, 20])):
+            if "kv_lens_host" in more and (max(q_lens) == 2 or dtype == torch.float32):
+                continue                                   # (not looked at where nothing is sized by it)
+            with pytest.raises(ops().KernelError, match="on the host"):
+                kp.attend(ops(), rows, q, q_lens, 4, **more)
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for page_size in (2 ** 32 + 16, -16, 0):
+        with pytest.raises(ops().KernelError, match="pages|page size"):
+            ops().step_layout(one, one, torch.zeros(2, dtype=torch.int32, device=DEV), one[:0], page_size, torch.zeros(1, 1, dtype=torch.int32, device=DEV))

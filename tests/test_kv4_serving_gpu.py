@@ -51,6 +51,35 @@ def test_pages_that_a_window_has_given_back_are_not_reported(runner):
     runner.check_status()
 
 
+def test_the_largest_layout():
+    """As many requests as one call takes: their offsets fill the shared memory."""
+    from coheryn_ai_studio_b200 import ops
+    B, ps = ops.STEP_LAYOUT_REQUESTS, 16
+    rng = np.random.default_rng(8)
+    starts, q_lens = rng.integers(0, 60, B), rng.integers(0, 4, B)
+    counts = -(-(starts + q_lens) // ps)
+    page_cu = np.concatenate([[0], np.cumsum(counts)])
+    pages = rng.permutation(int(page_cu[-1]))
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)      # noqa: E731
+    T = int(q_lens.sum())
+    slots, pos, req, table = (torch.empty(n, dtype=torch.int32, device=DEV) for n in (T, T, T, (B, 5)))
+    cu, kv, status = (torch.empty(n, dtype=torch.int32, device=DEV) for n in (B + 1, B, 1))
+    status.zero_()
+    ops.step_layout(i32(starts), i32(q_lens), i32(page_cu), i32(pages), ps, table, slots, cu, kv, pos, req, status=status)
+    want_req = np.repeat(np.arange(B), q_lens)
+    want_cu = np.concatenate([[0], np.cumsum(q_lens)])
+    want_pos = starts[want_req] + np.arange(T) - want_cu[want_req]
+    want_table = np.full((B, 5), -1)
+    for b in range(B):
+        want_table[b, :counts[b]] = pages[page_cu[b]:page_cu[b + 1]]
+    for got, want in ((req, want_req), (cu, want_cu), (pos, want_pos), (kv, starts + q_lens), (table, want_table),
+                      (slots, want_table[want_req, want_pos // ps] * ps + want_pos % ps)):
+        assert np.array_equal(got.cpu().numpy(), want)
+    assert int(status) == 0
+    with pytest.raises(ops.KernelError, match="requests"):
+        ops.step_layout(*[torch.zeros(B + n, dtype=torch.int32, device=DEV) for n in (1, 1, 2)], i32([0]), ps, torch.zeros(B + 1, 1, dtype=torch.int32, device=DEV))
+
+
 # ------------------------------------------------------------------------------------ a model with a window and an entry that reads another's cache
 class Config(dict):
     def to_dict(self):
