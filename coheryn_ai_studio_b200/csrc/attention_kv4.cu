@@ -38,7 +38,8 @@ constexpr int BAD_INDEX = 41;         // status: a slot, a position or a block-t
 __device__ __forceinline__ float lo_bf16(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf16(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
-__device__ __forceinline__ __nv_bfloat162 pair_of(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
+__device__ __forceinline__ __half2 half_pair(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ unsigned pack(float a, float b) { return bits(__floats2bfloat162_rn(a, b)); }
 __device__ __forceinline__ unsigned pack_f16(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
@@ -777,12 +778,16 @@ kv4_simple_join_kernel(const float* __restrict__ scratch, int parts, T* __restri
 //    of m sum(q), is one product more over the groups in the place of the channels, with sum(q) as three bfloat16 terms.
 //    No key is rounded.  Queries enter as float16 times the power of two that brings the row's largest to 2^14..2^15:
 //    exact, but for elements under 2^-24 of it;
-//  * values: s c + m in bfloat16 with one rounding (128 + c - 128 is exact, then one fused multiply-add on pairs).  The scale
+//  * values: s c + m in float16 with one rounding (1024 + c - 1024 is exact, then one fused multiply-add on pairs).  A pair of tiles has its
+//    scales and minima turned to float16 in their place when it has landed (32 pieces of 16 bytes at head size 128, one a lane), times a
+//    power of two that follows the largest of them, so that a value keeps eleven bits, or what lies over 2^-34 of the largest.  In
+//    bfloat16 the values' rounding alone made 2.25e-3 against 64 bits; 1.7e-3 now, of which the outputs' own is 1.65e-3.  The scale
 //    put on the probability instead takes fewer instructions but rounds p s, whose error meets s c and not s c + m;
-//  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory, each as the sum
-//    of two bfloat16 terms: rounded to one they were the largest error of all (2.7e-3 against 64 bits, 2.3e-3 with two, for 6 % of the time);
+//  * probabilities leave the first product's registers for the second's by movmatrix (transposed), not through memory, in float16 and
+//    2^LIFT times over their reference: one term (as two bfloat16 terms, which the values' type asked for before, they took twice the
+//    products and movmatrix: 64 x up to 16,384 151 us, 143 now; 2 x up to 131,072 43.4, 40.6);
 //  * the reference that scores are counted from moves (and the accumulators are scaled) only when a score exceeds it by more
-//    than 2^SLACK: at most 2^8 then enters the products, whose relative precision does not depend on it.
+//    than 2^SLACK.
 //  * the values' product of a pair and the scores of the next stand in one run of code without a branch, so that a warp
 //    has work of both kinds to issue.
 // The rows' sums stay per lane and meet once at the end, as do the warps.
@@ -793,6 +798,7 @@ constexpr int PAIR = 2 * TB;
 constexpr int RING = (K_STAGES + V_STAGES) * PAIR;
 constexpr float NOTHING = -3.0e38f;      // a reference that no score has met
 constexpr float SLACK = 8.f;
+constexpr float LIFT = 7.f;              // probabilities are 2^LIFT times over their reference: 2^15 at most, and 2^-32 of it is float16's least
 
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -841,8 +847,8 @@ __device__ __forceinline__ unsigned masked(unsigned word, unsigned mask, unsigne
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(word), "r"(mask), "r"(constant));
   return r;
 }
-// Codes j and j + 4 of a word as the bfloat16 pair 128 + c, and as the float16 pair c 2^-24 (j even) or 16 c 2^-24 (j odd).
-__device__ __forceinline__ unsigned codes128(unsigned word, int j) { return masked(word >> (4 * j), 0x000f000fu, 0x43004300u); }
+// Codes j and j + 4 of a word as the float16 pair 1024 + c, and as the float16 pair c 2^-24 (j even) or 16 c 2^-24 (j odd).
+__device__ __forceinline__ unsigned codes1024(unsigned word, int j) { return masked(word >> (4 * j), 0x000f000fu, 0x64006400u); }
 __device__ __forceinline__ unsigned codes16(unsigned word, int j) { return (j < 2 ? word : word >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
 template <int N>
 __device__ __forceinline__ void load_words(const unsigned* p, unsigned (&w)[N]) {
@@ -994,28 +1000,26 @@ __device__ __forceinline__ void tile_scores(float (&s)[NT][4], const Queries<NT>
   }
 }
 
-// Adds a tile's values, weighted: pf[nt] holds the probabilities of the 16 positions for row g of every eight.
+// Adds a tile's values, weighted: pf[nt] holds the probabilities of the 16 positions for row g of every eight.  The tile's pairs are float16 (see `to_half`).
 template <int NT>
-__device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[NT][4], const unsigned char* vt) {
+__device__ __forceinline__ void tile_values(Sums<NT>& sm, const unsigned (&pf)[NT][2], const unsigned char* vt) {
   const int lane = threadIdx.x & 31, t = lane & 3;
-  const __nv_bfloat162 k128 = __floats2bfloat162_rn(128.f, 128.f);
+  const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f);
 #pragma unroll
   for (int u = 0; u < NG; ++u) {
     const uint2 w = reinterpret_cast<const uint2*>(vt)[u * 32 + lane];
     const uint4 pairs = reinterpret_cast<const uint4*>(vt + CODES)[u * 4 + t];
-    const __nv_bfloat162 s01 = pair_of(pairs.x), s23 = pair_of(pairs.y), m01 = pair_of(pairs.z), m23 = pair_of(pairs.w);
+    const __half2 s01 = half_pair(pairs.x), s23 = half_pair(pairs.y), m01 = half_pair(pairs.z), m23 = half_pair(pairs.w);
     unsigned a[4], b[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      a[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.x, j)), k128), s01, m01));
-      b[j] = bits(__hfma2(__hsub2(pair_of(codes128(w.y, j)), k128), s23, m23));
+      a[j] = bits(__hfma2(__hsub2(half_pair(codes1024(w.x, j)), k1024), s01, m01));
+      b[j] = bits(__hfma2(__hsub2(half_pair(codes1024(w.y, j)), k1024), s23, m23));
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      mma_bf16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
-      mma_bf16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
-      mma_bf16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][2], pf[nt][3]);
-      mma_bf16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][2], pf[nt][3]);
+      mma_f16(sm.o[u][0][nt], a[0], a[1], b[0], b[1], pf[nt][0], pf[nt][1]);
+      mma_f16(sm.o[u][1][nt], a[2], a[3], b[2], b[3], pf[nt][0], pf[nt][1]);
     }
   }
 }
@@ -1131,11 +1135,64 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     const int all_lo = window > 0 ? max(0, last - window + 1) : 0;
 
     float s[2][NT][4];
-    unsigned pf[2][NT][4];
+    unsigned pf[2][NT][2];
+    // The values' power of two: 2^(137 - v_exp) brings what was the largest magnitude when it was chosen to 2^10..2^11; up to v_limit it stays.
+    int v_exp = 137;
+    unsigned v_limit = 0;
+    // The pairs of a pair of value tiles from bfloat16 to float16 in their place, times that power of two (exact, but for what lies under
+    // 2^-34 of the largest).  Positions outside what any query sees may hold anything (a stale row, a page's end): their pairs become
+    // zero, so that nothing which is not finite meets a probability of zero.
+    auto to_half = [&](unsigned char* values, bool whole, int key0, unsigned there) {
+      constexpr int PIECES = 8 * NG, ROUNDS = (PIECES + 31) / 32;         // of four rows' scales and minima each
+      uint4 w[ROUNDS];
+      float most = 0.f;
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int x = r * 32 + lane, h = x / (4 * NG), p = x - h * (4 * NG);
+        w[r] = make_uint4(0, 0, 0, 0);
+        if (PIECES % 32 == 0 || x < PIECES) w[r] = reinterpret_cast<const uint4*>(values + h * TB + CODES)[p];
+        if (!whole) {
+          const int first = key0 + 16 * h + 4 * (p & 3);
+          const int lo = window > 0 ? all_hi - window + 1 : 0;
+          auto seen = [&](int pos) { return ((there >> h) & 1u) && pos <= last && pos >= lo; };
+          const unsigned k01 = (seen(first) ? 0xffffu : 0u) | (seen(first + 1) ? 0xffff0000u : 0u);
+          const unsigned k23 = (seen(first + 2) ? 0xffffu : 0u) | (seen(first + 3) ? 0xffff0000u : 0u);
+          w[r].x &= k01; w[r].y &= k23; w[r].z &= k01; w[r].w &= k23;
+        }
+        const float sc = fmaxf(fmaxf(lo_bf16(w[r].x), hi_bf16(w[r].x)), fmaxf(lo_bf16(w[r].y), hi_bf16(w[r].y)));
+        const float mn = fmaxf(fmaxf(fabsf(lo_bf16(w[r].z)), fabsf(hi_bf16(w[r].z))), fmaxf(fabsf(lo_bf16(w[r].w)), fabsf(hi_bf16(w[r].w))));
+        most = fmaxf(most, fmaxf(mn, 16.f * sc));          // a value is at most twice that
+      }
+      const unsigned all_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      if (all_most > v_limit) {
+        const int e = min(max((int)(all_most >> 23), 18), 254), by = 127 + v_exp - e;
+        const float f = by > 0 ? __uint_as_float((unsigned)by << 23) : 0.f;
+        v_exp = e;
+        v_limit = (unsigned)min(e + 4, 254) << 23;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int u = 0; u < NG; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sm.o[u][h][nt][i] *= f;
+      }
+      const float by = __uint_as_float((unsigned)(264 - v_exp) << 23);
+      auto half = [&](unsigned v) { return pack_f16(lo_bf16(v) * by, hi_bf16(v) * by); };
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int x = r * 32 + lane, h = x / (4 * NG), p = x - h * (4 * NG);
+        if (PIECES % 32 == 0 || x < PIECES)
+          reinterpret_cast<uint4*>(values + h * TB + CODES)[p] = make_uint4(half(w[r].x), half(w[r].y), half(w[r].z), half(w[r].w));
+      }
+      __syncwarp();
+    };
     // From the scores s of pair i, whose values are at `values`, to its probabilities pf.
     auto probabilities = [&](int i, unsigned char* values) {
       const int key0 = (tile0 + i * 2 * WARPS) * 16;
       const unsigned there = (known >> 2) & 3u;        // of pair i: pair i + 1 was issued last
+      const bool whole = there == 3u && key0 >= all_lo && key0 + 31 <= all_hi;
       float y[2][NT][4];            // exponents: scores (times log2 e) from the row's reference
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -1143,7 +1200,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 4; ++x) y[h][nt][x] = fmaf(s[h][nt][x], qr.cs[nt][x & 1], -sm.m[nt][x & 1]);
-      if (!(there == 3u && key0 >= all_lo && key0 + 31 <= all_hi)) {
+      if (!whole) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1155,21 +1212,12 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
               if (!((there >> h) & 1u) || pos > hi || (window > 0 && pos <= hi - window)) y[h][nt][x] = -INFINITY;
             }
           }
-        // Rows of the tiles outside what any query sees may hold anything (a stale row, a page's end): their pairs of
-        // the values become zero, so that nothing which is not finite meets a probability of zero.
-        const int row = lane & 15, h = lane >> 4, pos = key0 + lane;
-        if (!((there >> h) & 1u) || pos > last || (window > 0 && pos <= all_hi - window)) {
-          unsigned short* pairs = reinterpret_cast<unsigned short*>(values + h * TB + CODES) + (row >> 2) * 8 + (row & 3);
-#pragma unroll
-          for (int u = 0; u < NG; ++u) pairs[u * 32] = pairs[u * 32 + 4] = 0;
-        }
-        __syncwarp();
       }
       bool grew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) grew = grew || fmaxf(y[0][nt][x], y[1][nt][x]) > SLACK;
+        for (int x = 0; x < 4; ++x) grew = grew || fmaxf(y[0][nt][x], y[1][nt][x]) > SLACK + LIFT;
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -1179,7 +1227,7 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int x = e; x < 4; x += 2) M = y[h][nt][x] == -INFINITY ? M : fmaxf(M, s[h][nt][x] * qr.cs[nt][e]);
+              for (int x = e; x < 4; x += 2) M = y[h][nt][x] == -INFINITY ? M : fmaxf(M, fmaf(s[h][nt][x], qr.cs[nt][e], -LIFT));
 #pragma unroll
             for (int x = 4; x <= 16; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
             const float f = ex2(sm.m[nt][e] - M);
@@ -1205,13 +1253,9 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
             sm.l[nt][x & 1] += y[h][nt][x];
           }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float a = y[h][nt][2 * x], b = y[h][nt][2 * x + 1];
-            const unsigned w = pack(a, b);
-            pf[h][nt][x] = transposed(w);
-            pf[h][nt][2 + x] = transposed(pack(a - lo_bf16(w), b - hi_bf16(w)));
-          }
+          for (int x = 0; x < 2; ++x) pf[h][nt][x] = transposed(pack_f16(y[h][nt][2 * x], y[h][nt][2 * x + 1]));
         }
+      to_half(values, whole, key0, there);
     };
 
     unsigned char* values = ring + K_STAGES * PAIR;            // of pair i
@@ -1249,6 +1293,8 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
     cp_async_wait<0>();
     __syncthreads();                 // the rings become the warps' meeting
     float* merge = reinterpret_cast<float*>(smem);
+    const float v_back = __uint_as_float((unsigned)(v_exp - 17) << 23), lift_back = 1.f / 128.f;         // 2^(v_exp - 137 - LIFT), 2^-LIFT
+    static_assert(LIFT == 7.f, "the exponents of the factors back");
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1257,11 +1303,11 @@ kv4_items_kernel(const bf16* __restrict__ q, long q_ld, bf16* __restrict__ out, 
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         float* dst = merge + (size_t)(warp * COLS + nt * 8 + 2 * t + e) * MLD;
-        if (g == 0) { dst[HD] = sm.m[nt][e]; dst[HD + 1] = sum; }
+        if (g == 0) { dst[HD] = sm.m[nt][e]; dst[HD + 1] = sum * lift_back; }
 #pragma unroll
         for (int u = 0; u < NG; ++u)
           *reinterpret_cast<float4*>(dst + u * 32 + g * 4) =
-              make_float4(sm.o[u][0][nt][e], sm.o[u][0][nt][2 + e], sm.o[u][1][nt][e], sm.o[u][1][nt][2 + e]);
+              make_float4(sm.o[u][0][nt][e] * v_back, sm.o[u][0][nt][2 + e] * v_back, sm.o[u][1][nt][e] * v_back, sm.o[u][1][nt][2 + e] * v_back);
       }
     __syncthreads();
     const int slot = 2 * blockIdx.x + (first_list ? 0 : 1);

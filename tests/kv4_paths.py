@@ -1,7 +1,8 @@
 """Attention over the 4-bit cache by each of its ways, in 64 bits with the roundings that the way makes of keys and values, and how far a
 kernel of that way may be from it.
 
-* "direct": keys as codes, scales and minima (nothing rounded); values s c + m in bfloat16; probabilities as two bfloat16 terms.
+* "direct": keys as codes, scales and minima (nothing rounded); values s c + m in float16 after a power of two that follows the largest
+  magnitude, 2^14 at most, which is brought to 2^10 at least; probabilities in float16, 2^7 over the reference.
 * "half": keys and values in float16 after a power of two that brings the largest magnitude that a (request, kv head) sees to 2^13..2^14;
   probabilities in float16, 2^7 over the reference.
 * "bfloat16": keys, values and probabilities in bfloat16.
@@ -79,12 +80,14 @@ def expected(rows, b, q, scale, window, way, dtype):
     with np.errstate(invalid="ignore"):
         (k, k_terms, k_most), (v, _, v_most) = (stored(x[b][lo_all:]) for x in (rows.k, rows.v))
         kr = {"half": lambda: as_half(k, k_most), "bfloat16": lambda: as_bfloat16(k)}.get(way, lambda: k)()
-        vr = {"half": lambda: as_half(v, v_most), "float32": lambda: v}.get(way, lambda: as_bfloat16(v))()
+        vr = {"half": lambda: as_half(v, v_most), "bfloat16": lambda: as_bfloat16(v)}.get(way, lambda: v)()
     out, tol = np.zeros((n, heads, hd)), np.zeros((n, heads, hd))
     # roundings of a score, in units of 2^-23 of the sum of its terms' magnitudes: a group's 32 products, the groups' and the sum of the minima's;
     # or hd products; and the factors' roundings beside
     steps = 64 + hd // 32 if way == "direct" else hd + 16
-    weight = {"direct": 2.0 ** -15, "half": 2.0 ** -11, "bfloat16": 2.0 ** -8, "float32": 2.0 ** -23}[way]     # a probability's rounding, and a value's second one
+    # the rounding of a probability, and of a value where it is not in vr
+    weight = {"direct": 2.0 ** -10, "half": 2.0 ** -11, "bfloat16": 2.0 ** -8, "float32": 2.0 ** -23}[way]
+    least = np.nanmax(v_most.transpose(1, 0, 2).reshape(G, -1), axis=1, initial=0.0) * 2.0 ** -34 if way == "direct" else np.zeros(G)      # a value's absolute rounding
     for i in range(n):
         pos = L - n + i
         lo, hi = (max(0, pos - window + 1) if window else 0) - lo_all, pos + 1 - lo_all
@@ -102,7 +105,7 @@ def expected(rows, b, q, scale, window, way, dtype):
             # errors up to d in the scores move a probability by a factor within exp(-2 d)..exp(2 d); exponentials 2^-20; sums over the keys
             tol[i, h] = A * (np.expm1(min(2 * d, 5)) + weight + 2.0 ** -20 + (hi - lo + 16) * 2.0 ** -23)
             # A probability under the smallest normal float32 is none; in float16, 2^7 over the reference, steps are 2^-24 under 2^-14.
-            tol[i, h] += (hi - lo) * (2.0 ** -32 if way == "half" else 2.0 ** -126) * np.abs(vv).max(0)
+            tol[i, h] += (hi - lo) * (2.0 ** -32 if way in ("half", "direct") else 2.0 ** -126) * np.abs(vv).max(0) + least[g]
     return out, tol + np.abs(out) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23) + (2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -140)
 
 

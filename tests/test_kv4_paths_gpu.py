@@ -98,6 +98,34 @@ def test_portions_of_any_magnitude(hd, k_spread, v_spread, context):
     kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads), q_lens, heads, BF16)
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128, 160, 256])
+@pytest.mark.parametrize("k_spread,v_spread", [(1e30, 1e29), (1e-30, 1e-30), (1.0, 1e-37)])
+@pytest.mark.parametrize("q_lens,lens", [([1, 3], [700, 40]), ([1], [5000])])
+def test_short_runs_of_any_magnitude(hd, k_spread, v_spread, q_lens, lens):
+    k, v = kp.random_rows(32, lens, 2, hd, k_spread, v_spread)
+    rows = kp.Rows(k, v)
+    q = queries(33, q_lens, 4, hd, 1.5 / k_spread)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, 4), q_lens, 4, BF16)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("steps", ["up", "down", "zeros first", "one", "back and forth"])
+def test_values_whose_magnitude_changes_along_the_context(hd, window, steps):
+    """The power of two that the values are taken to follows the largest; what was added up before is scaled."""
+    heads, nkv, q_lens, lens = 6, 2, [1, 4, 20], [900, 400, 130]
+    k, v = kp.random_rows(34, lens, nkv, hd)
+    for x in v:
+        p = np.arange(len(x))
+        by = {"up": 2.0 ** (p / 20), "down": 2.0 ** (-p / 20), "zeros first": np.where(p < 70, 0.0, 1.0), "one": np.where(p == 50, 2.0 ** 20, 1.0),
+              "back and forth": 2.0 ** (10 * np.sin(p / 15.0))}[steps]
+        x *= by[:, None, None].astype(np.float32)
+        x[:, 1] *= np.float32(2.0 ** -12)
+    rows = kp.Rows(k, v)
+    q = queries(35, q_lens, heads, hd)
+    kp.check(rows, q, kp.attend(ops(), rows, q, q_lens, heads, window), q_lens, heads, BF16, window)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("heads,nkv", [(4, 1), (6, 2)])
 def test_requests_of_one_call_keep_their_own_magnitudes(hd, heads, nkv):
