@@ -70,7 +70,7 @@ class Engine:
         books; the tokens a request receives are the same.  ``kv_bits`` = 4 keeps keys and values in 4 bits, with a scale and a
         minimum for every 32 channels: 3.2 times the tokens of a bfloat16 cache in the same memory, and that much less to
         read when decoding, at the price of their rounding (models of plain attention, head sizes of a multiple of 32).  Steps
-        are shorter where the cache's bytes count (7B sizes, 64 requests up to 8,192: 5.63 ms against 7.06), not at small batches and
+        are shorter where the cache's bytes count (7B sizes, 64 requests up to 8,192: 5.60 ms against 7.03), not at small batches and
         short contexts (1.5B, 8 up to 4,096: 1.47 against 1.40)."""
         self.model = model
         spec = model.spec

@@ -2269,11 +2269,11 @@ _kv4_libs = {}
 
 # Requests with at most this many query rows (tokens times heads of a group) read the 4-bit pages directly; longer portions
 # have their pages expanded to 16 bits a value once and go through the prompt kernels.  Directly against expanded, us of calls replayed
-# from a graph, head size 128: 112 rows of 7 heads over each of 4, 1 x 1,024 positions 9.9 and 25.2, 8 x 8,192 100 and 99; of 4 over each of
-# 8, 1 x 65,536 64 rows 110 and 180, 112 181 and 181, 128 205 and 181, 256 393 and 199; 8 x 1,024 64 rows 32 and 35, 128 53 and 36.  Half as
+# from a graph, head size 128: 112 rows of 7 heads over each of 4, 1 x 1,024 positions 9.9 and 25.4, 8 x 8,192 93 and 100; of 4 over each of
+# 8, 1 x 65,536 64 rows 101 and 180, 112 166 and 181, 128 188 and 182, 256 360 and 200; 8 x 1,024 64 rows 30 and 35, 128 52 and 36.  Half as
 # many at head sizes 192 and 256, which the direct kernel takes in tiles of 8 rows instead of 16 and whose prompts have a tcgen05 kernel
-# (4 heads over 4, 8 x 8,192: 256, 64 rows 132 and 170, 128 rows 252 and 173; 192, 107 and 146, 206 and 149); not at those between, whose
-# prompts have none (128 rows: 160, 181 and 415; 224, 236 and 554).
+# (4 heads over 4, 8 x 8,192: 256, 64 rows 126 and 170, 128 rows 242 and 172; 192, 108 and 146, 207 and 149); not at those between, whose
+# prompts have none (128 rows: 160, 187 and 415; 224, 233 and 554).
 KV4_DIRECT_ROWS = int(os.environ.get("COHERYN_KV4_DIRECT_ROWS", "128"))
 
 
