@@ -2499,7 +2499,8 @@ def attention_kv4_rows(q, out, k_cache, v_cache, block_tables, token_req, positi
         return
     # Longer portions: neighbouring requests together, as many as the expanded pages' bound allows.  Head sizes 64 and 128 go through the
     # float16 kernel of csrc/attention_kv4_prompt.cu, others through the framework's kernels for bfloat16 pages: these round a key and a value
-    # that a page stands for to the compute type, as a bfloat16 cache does (3.1e-3 to 4.9e-3 against 64 bits, 1.7e-3 in float16).
+    # that a page stands for to the compute type, as a bfloat16 cache does (1.8e-3 to 5.4e-3 against 64 bits, the more the larger the scores;
+    # 1.7e-3 in float16).
     page_bytes = num_kv_heads * page_size * head_dim * 4
     b = 0
     while b < B:
